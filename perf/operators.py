@@ -26,14 +26,20 @@ SIZE = {"bf16": 2, "f32": 4}
 EPS = 1e-6
 
 
-def _library():
-    """The package's modules, imported where the library's own kernels run."""
-    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ferrite-tpu_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    from ferrite.kernels import drafts, qk_norm_rope, tree_attention
+_calls = None
 
-    return qk_norm_rope.qk_norm_rope, tree_attention.tree_attention, drafts.accept_drafts, drafts.compact_cache
+
+def _library():
+    """The library's entry points, imported where its own kernels run, once."""
+    global _calls
+    if _calls is None:
+        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ferrite-tpu_amd")
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        from ferrite.kernels import drafts, qk_norm_rope, tree_attention
+
+        _calls = (qk_norm_rope.qk_norm_rope, tree_attention.tree_attention, drafts.accept_drafts, drafts.compact_cache)
+    return _calls
 
 
 # ---------------------------------------------------------------- cases
