@@ -73,4 +73,28 @@ int ferrite_internal_embed_bwd(const int64_t* tokens, const void* dh, void* dtok
                                int64_t period, int64_t dim, int64_t vocab, int64_t seq, int dh_dtype, int emb_dtype,
                                void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * The heads of a fused projection qkv [B, S, (H + 2 Hkv) D] (its last dimension dense; batch_stride and
+ * row_stride in elements), split, each q and k head normed and rotated: q [B, H, S, D], k and v
+ * [B, Hkv, S, D], dense. wq, wk [D] of w_dtype; cos and sin f32 [table, rot / 2]; pos [B, S], or null
+ * for position s of every sequence. A position outside the table gives NaN in its q and k rows. D even
+ * and at most 512, rot even and at most D.
+ */
+int ferrite_internal_heads_rope(const void* qkv, int64_t batch_stride, int64_t row_stride, const void* wq,
+                                const void* wk, const float* cos, const float* sin, const int32_t* pos, void* q, void* k,
+                                void* v, int64_t b, int64_t s, int64_t h, int64_t hkv, int64_t d, int64_t rot,
+                                int64_t table, int dtype, int w_dtype, int interleaved, float eps, void* stream);
+/*
+ * Its gradients from dense dq, dk and dv (null: zero): dqkv, dense, and the weights' in w_dtype, summed in f32
+ * in a fixed order. The workspace has ferrite_internal_heads_rope_bwd_workspace(...) bytes (-1: sizes out of
+ * range); its content need not survive the call.
+ */
+int64_t ferrite_internal_heads_rope_bwd_workspace(int64_t b, int64_t s, int64_t h, int64_t hkv, int64_t d);
+int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64_t row_stride, const void* wq,
+                                    const void* wk, const float* cos, const float* sin, const int32_t* pos,
+                                    const void* dq, const void* dk, const void* dv, void* dqkv, void* dwq, void* dwk,
+                                    int64_t b, int64_t s, int64_t h, int64_t hkv, int64_t d, int64_t rot, int64_t table,
+                                    int dtype, int w_dtype, int interleaved, float eps, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+
 }  // extern "C"

@@ -46,6 +46,13 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes_on(int64_t n, const Tensor& like) {
   return n > 0 ? at::empty({n}, like.options().dtype(at::kByte)) : Tensor();
 }
+// Whether autograd records a backward for a function of `inputs`.
+bool records(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : inputs)
+    if (t->requires_grad()) return true;
+  return false;
+}
 // Rows of a [..., last] tensor.
 int64_t rows_of(const Tensor& t) {
   if (t.dim() < 1 || t.size(-1) == 0) throw std::runtime_error("ferrite's kernels need a non-empty last dimension");
@@ -255,6 +262,76 @@ Tensor flash(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, dou
 Tensor flash_qkv(const Tensor& qkv, int64_t heads, double scale) { return FlashQkvFn::apply(qkv, heads, scale); }
 
 // ---------------------------------------------------------------------------
+// Heads split, normed and rotated
+// ---------------------------------------------------------------------------
+struct HeadsOptions {
+  int64_t h, hkv;
+  double eps;
+  bool interleaved;
+  Tensor pos;  // undefined: every sequence from position 0 (an autograd function's inputs are all defined)
+};
+// The projection with a dense last dimension; its other strides are read as they are.
+Tensor dense_rows(const Tensor& t) { return t.stride(2) == 1 ? t : t.contiguous(); }
+
+variable_list heads_forward(const Tensor& qkv, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin,
+                            const HeadsOptions& o) {
+  const int64_t b = qkv.size(0), s = qkv.size(1), d = wq.size(0);
+  Tensor q = at::empty({b, o.h, s, d}, qkv.options()), k = at::empty({b, o.hkv, s, d}, qkv.options()),
+         v = at::empty({b, o.hkv, s, d}, qkv.options());
+  check(ferrite_internal_heads_rope(ptr(qkv), qkv.stride(0), qkv.stride(1), ptr(wq), ptr(wk), (const float*)ptr(cos),
+                                    (const float*)ptr(sin), (const int32_t*)ptr(o.pos), ptr(q), ptr(k), ptr(v), b, s, o.h,
+                                    o.hkv, d, 2 * cos.size(1), cos.size(0), code(qkv), code(wq), o.interleaved,
+                                    (float)o.eps, stream_of(qkv)),
+        "ferrite_qk_norm_rope");
+  return {q, k, v};
+}
+
+struct HeadsFn : torch::autograd::Function<HeadsFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& wq, const Tensor& wk,
+                               const Tensor& cos, const Tensor& sin, HeadsOptions o) {
+    ctx->save_for_backward({qkv, wq, wk, cos, sin, o.pos});
+    ctx->saved_data["h"] = o.h;
+    ctx->saved_data["hkv"] = o.hkv;
+    ctx->saved_data["eps"] = o.eps;
+    ctx->saved_data["interleaved"] = o.interleaved;
+    ctx->set_materialize_grads(false);  // an output without a gradient is not read
+    return heads_forward(qkv, wq, wk, cos, sin, o);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gs) {
+    const auto sv = ctx->get_saved_variables();
+    const Tensor &qkv = sv[0], &wq = sv[1], &wk = sv[2], &cos = sv[3], &sin = sv[4], &pos = sv[5];
+    const int64_t b = qkv.size(0), s = qkv.size(1), d = wq.size(0);
+    const int64_t h = ctx->saved_data["h"].toInt(), hkv = ctx->saved_data["hkv"].toInt();
+    for (Tensor& g : gs)
+      if (g.defined()) g = g.to(qkv.scalar_type()).contiguous();
+    Tensor dqkv = at::empty(qkv.sizes(), qkv.options()), dwq = at::empty(wq.sizes(), wq.options()),
+           dwk = at::empty(wk.sizes(), wk.options());
+    const Tensor ws = bytes_on(ferrite_internal_heads_rope_bwd_workspace(b, s, h, hkv, d), qkv);
+    check(ferrite_internal_heads_rope_bwd(ptr(qkv), qkv.stride(0), qkv.stride(1), ptr(wq), ptr(wk),
+                                          (const float*)ptr(cos), (const float*)ptr(sin), (const int32_t*)ptr(pos),
+                                          ptr(gs[0]), ptr(gs[1]), ptr(gs[2]), ptr(dqkv), ptr(dwq), ptr(dwk), b, s, h, hkv,
+                                          d, 2 * cos.size(1), cos.size(0), code(qkv), code(wq),
+                                          ctx->saved_data["interleaved"].toBool(),
+                                          (float)ctx->saved_data["eps"].toDouble(), ptr(ws), size_of(ws), stream_of(qkv)),
+          "ferrite_qk_norm_rope_bwd");
+    return {dqkv, dwq, dwk, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qk_norm_rope(const Tensor& qkv0, const Tensor& wq0, const Tensor& wk0,
+                                                const Tensor& cos0, const Tensor& sin0, const std::optional<Tensor>& pos0,
+                                                int64_t h, int64_t hkv, double eps, bool interleaved) {
+  const Tensor qkv = dense_rows(qkv0), wq = wq0.contiguous(), wk = wk0.contiguous(), cos = cos0.contiguous(),
+               sin = sin0.contiguous();
+  Tensor pos;
+  if (pos0) pos = pos0->to(at::kInt).expand({qkv.size(0), qkv.size(1)}).contiguous();
+  const HeadsOptions o{h, hkv, eps, interleaved, pos};
+  const auto out =
+      records({&qkv, &wq, &wk}) ? HeadsFn::apply(qkv, wq, wk, cos, sin, o) : heads_forward(qkv, wq, wk, cos, sin, o);
+  return {out[0], out[1], out[2]};
+}
+
+// ---------------------------------------------------------------------------
 // Matmul, linear layer, MLP
 // ---------------------------------------------------------------------------
 // Whether the DMA-fed kernel takes the operands as they lie (ferrite_hip_matmul_ex's rule for a
@@ -347,12 +424,6 @@ struct MatmulFn : torch::autograd::Function<MatmulFn> {
 // that one has to find the forward's weight also after an update in place, so it keeps a rounded
 // copy, as larger products do. The weight's gradient comes back in the weight's own dtype,
 // unrounded if that is float.
-bool records(std::initializer_list<const Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : inputs)
-    if (t->requires_grad()) return true;
-  return false;
-}
 // us on one MI355X, the weight as it is / a rounded copy and its product: 64 x 16384 x 16384 240 / 458,
 // 64 x 768 x 32768 26.5 / 34.4; faster at all 24 sizes measured.
 bool reads_f32_weight(const Tensor& x, const Tensor& w) {
@@ -572,6 +643,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_forward", &flash_forward, nogil());
   m.def("flash_backward", &flash_backward, nogil());
   m.def("flash_qkv", &flash_qkv, nogil());
+  m.def("qk_norm_rope", &qk_norm_rope, nogil());
   m.def("matmul", &matmul, nogil());
   m.def("linear", &linear, nogil());
   m.def("mlp", &mlp, nogil());

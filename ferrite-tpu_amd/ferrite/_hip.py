@@ -144,6 +144,15 @@ INTERNAL: dict[str, tuple] = {
         _c_int,
         [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp],
     ),
+    "ferrite_internal_heads_rope": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, *[_vp] * 8, *[_c_i64] * 7, _c_int, _c_int, _c_int, _c_f32, _vp],
+    ),
+    "ferrite_internal_heads_rope_bwd_workspace": (_c_i64, [_c_i64] * 5),
+    "ferrite_internal_heads_rope_bwd": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, *[_vp] * 11, *[_c_i64] * 7, _c_int, _c_int, _c_int, _c_f32, _vp, _c_i64, _vp],
+    ),
 }
 
 _lock = threading.Lock()

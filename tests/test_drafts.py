@@ -1,0 +1,101 @@
+"""CPU tests of the drafted step's and the rotated heads' operators: what they refuse, before any launch."""
+
+import pytest
+import torch
+
+from ferrite import _hip
+from ferrite.kernels.qk_norm_rope import qk_norm_rope, qk_norm_rope_reference, rope_tables
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _heads(**change):
+    a = dict(qkv=torch.zeros(2, 3, 8 * 64), q_weight=torch.ones(64), k_weight=torch.ones(64), cos=torch.ones(8, 32),
+             sin=torch.zeros(8, 32), n_head=4, n_kv_head=2, positions=None)
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(n_head=3), "n_head"),
+    (dict(n_head=0), "at least one"),
+    (dict(n_kv_head=0), "at least one"),
+    (dict(qkv=torch.zeros(3, 512)), "qkv as"),
+    (dict(qkv=torch.zeros(2, 3, 0)), "qkv as"),
+    (dict(qkv=torch.zeros(2, 3, 8 * 63)), "even"),
+    (dict(qkv=torch.zeros(2, 3, 8 * 514)), "at most 512"),
+    (dict(q_weight=torch.ones(32)), "weights"),
+    (dict(k_weight=torch.ones(64, dtype=BF16)), "share a dtype"),
+    (dict(sin=torch.zeros(8, 16)), "pairs"),
+    (dict(cos=torch.ones(8, 33), sin=torch.ones(8, 33)), "pairs"),
+    (dict(cos=torch.ones(8, 0), sin=torch.ones(8, 0)), "pairs"),
+    (dict(cos=torch.ones(0, 8), sin=torch.ones(0, 8)), "pairs"),
+    (dict(cos=torch.ones(8, 32, dtype=BF16)), "float32"),
+    (dict(cos=torch.ones(8, 32, requires_grad=True)), "no gradient"),
+    (dict(cos=torch.ones(2, 32), sin=torch.ones(2, 32)), "longer"),
+    (dict(positions=torch.zeros(2, 4, dtype=torch.int32)), "positions"),
+    (dict(positions=torch.zeros(3)), "int32"),
+    (dict(qkv=torch.zeros(2, 3, 512, dtype=torch.float64)), "float32 or bfloat16"),
+    (dict(q_weight=torch.ones(64).half(), k_weight=torch.ones(64).half()), "float32 or bfloat16"),
+])
+def test_heads_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        qk_norm_rope(**_heads(**change))
+
+
+def test_heads_refuse_the_cpu():
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        qk_norm_rope(**_heads())
+
+
+def test_heads_abi_refusals():
+    lib = _hip.lib()
+    ok = dict(b=2, s=3, h=4, hkv=2, d=64, rot=64, table=8, dtype=_hip.BF16, w=_hip.F32)
+
+    def call(**change):
+        a = {**ok, **change}
+        args = (a["b"], a["s"], a["h"], a["hkv"], a["d"], a["rot"], a["table"], a["dtype"], a["w"], 0, 1e-6)
+        return (lib.ferrite_internal_heads_rope(None, 1, 1, *[None] * 8, *args, None),
+                lib.ferrite_internal_heads_rope_bwd(None, 1, 1, *[None] * 11, *args, None, 0, None))
+
+    for change, words in ((dict(), "null"), (dict(dtype=5), "dtype"), (dict(w=-1), "dtype"), (dict(h=0), "heads"),
+                          (dict(hkv=20000), "heads"), (dict(b=-1), "tokens"), (dict(b=1 << 20, s=1 << 20), "tokens"),
+                          (dict(d=63), "even"), (dict(d=514), "512"), (dict(rot=66), "even and within"), (dict(rot=3), "even"),
+                          (dict(table=0), "tables")):
+        assert call(**change) == (1, 1), change
+        assert words in _hip.last_error()
+    # nothing to do: no launch; the sums of no rows are still written by the backward, which needs its outputs
+    assert call(b=0) == (0, 1)
+    assert lib.ferrite_internal_heads_rope_bwd_workspace(1, 1, 1, 1, 3) == -1
+    assert lib.ferrite_internal_heads_rope_bwd_workspace(8, 1024, 12, 12, 64) > 0
+    # one token more than a launch's blocks hold
+    a = 1 << 12
+    assert lib.ferrite_internal_heads_rope(a, 2, 2, *[a] * 8, 1 << 14, 1 << 15, 1, 1, 2, 2, 1 << 15, _hip.BF16, _hip.F32, 0,
+                                           1e-6, None) == 1
+    assert "too many tokens" in _hip.last_error()
+
+
+def test_rope_tables():
+    cos, sin = rope_tables(5, 6, base=100.0)
+    assert cos.shape == sin.shape == (5, 3) and cos.dtype == F32
+    p = torch.arange(5, dtype=torch.float64)[:, None]
+    rate = torch.tensor([1.0, 100.0 ** (-1 / 3), 100.0 ** (-2 / 3)], dtype=torch.float64)
+    assert torch.allclose(cos.double(), (p * rate).cos(), atol=2.0**-24, rtol=0)
+    assert torch.allclose(sin.double(), (p * rate).sin(), atol=2.0**-24, rtol=0)
+    for n, d in ((0, 4), (4, 3), (4, 0)):
+        with pytest.raises(ValueError):
+            rope_tables(n, d)
+
+
+def test_heads_reference_keeps_lengths_and_turns_by_distance():
+    """A rotation keeps a head's length, and the product of two heads depends on the distance of their positions."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(1, 1, 3 * 8, generator=g, dtype=torch.float64)
+    one = torch.ones(8, dtype=torch.float64)
+    cos, sin = (t.double() for t in rope_tables(40, 8))
+    for inter in (False, True):
+        at = lambda p: qk_norm_rope_reference(x, one, one, cos, sin, n_head=1, positions=torch.tensor([p]),
+                                              interleaved=inter, eps=0.0)
+        assert abs(float(at(17)[0].square().sum()) - 8) <= 1e-6  # the tables are rounded to f32
+        a, b = (float((at(p + 5)[0] * at(p)[1]).sum()) for p in (0, 30))
+        assert abs(a - b) <= 1e-5
