@@ -97,4 +97,24 @@ int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64
                                     int dtype, int w_dtype, int interleaved, float eps, void* workspace,
                                     int64_t workspace_bytes, void* stream);
 
+/*
+ * The drafted nodes that greedy decoding would have taken: from node 0 (its parent -1), to the child that holds
+ * the argmax of the node's logits [B, T, V], while there is one. path [B, T] (-1 behind the visited nodes), count [B],
+ * following [B] (the argmax at the last node; -1 with count 0 where node 0 is absent). 1 <= T <= 64, B T <= 65535. A
+ * node whose parent is not -1 or an earlier one is absent and its logits are not read. The workspace has
+ * ferrite_internal_accept_drafts_workspace(...) bytes (-1: sizes out of range), 8-byte aligned.
+ */
+int64_t ferrite_internal_accept_drafts_workspace(int64_t b, int64_t t, int64_t v);
+int ferrite_internal_accept_drafts(const void* logits, const int64_t* tokens, const int32_t* parents, int32_t* path,
+                                   int32_t* count, int64_t* following, int64_t b, int64_t t, int64_t v, int dtype,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Rows pos[b] + path[b, i] of the caches [layers, B, H, max_len, D] to pos[b] + i, i < count[b], in place; a path ends
+ * at the first entry that is not larger than the one before (or negative) or whose row lies outside the cache. 1 <= T <= 64.
+ */
+int ferrite_internal_compact_cache(void* k_cache, void* v_cache, const int32_t* pos, const int32_t* path,
+                                   const int32_t* count, int64_t layers, int64_t b, int64_t h, int64_t max_len, int64_t d,
+                                   int64_t t, int dtype, void* stream);
+
 }  // extern "C"

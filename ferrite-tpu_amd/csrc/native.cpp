@@ -324,7 +324,7 @@ std::tuple<Tensor, Tensor, Tensor> qk_norm_rope(const Tensor& qkv0, const Tensor
   const Tensor qkv = dense_rows(qkv0), wq = wq0.contiguous(), wk = wk0.contiguous(), cos = cos0.contiguous(),
                sin = sin0.contiguous();
   Tensor pos;
-  if (pos0) pos = pos0->to(at::kInt).expand({qkv.size(0), qkv.size(1)}).contiguous();
+  if (pos0) pos = pos0->expand({qkv.size(0), qkv.size(1)}).contiguous();
   const HeadsOptions o{h, hkv, eps, interleaved, pos};
   const auto out =
       records({&qkv, &wq, &wk}) ? HeadsFn::apply(qkv, wq, wk, cos, sin, o) : heads_forward(qkv, wq, wk, cos, sin, o);
@@ -598,6 +598,31 @@ Tensor decode_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, co
 }
 
 // ---------------------------------------------------------------------------
+// Drafted step
+// ---------------------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor> accept_drafts(const Tensor& logits0, const Tensor& tokens0, const Tensor& parents0) {
+  const Tensor logits = logits0.contiguous(), tokens = tokens0.to(at::kLong).contiguous(),
+               parents = parents0.contiguous();
+  const int64_t b = logits.size(0), t = logits.size(1), v = logits.size(2);
+  Tensor path = at::empty({b, t}, parents.options()), count = at::empty({b}, parents.options()),
+         following = at::empty({b}, tokens.options());
+  const Tensor ws = bytes_on(ferrite_internal_accept_drafts_workspace(b, t, v), logits);
+  check(ferrite_internal_accept_drafts(ptr(logits), (const int64_t*)ptr(tokens), (const int32_t*)ptr(parents),
+                                       (int32_t*)ptr(path), (int32_t*)ptr(count), (int64_t*)ptr(following), b, t, v,
+                                       code(logits), ptr(ws), size_of(ws), stream_of(logits)),
+        "ferrite_accept_drafts");
+  return {path, count, following};
+}
+
+void compact_cache(const Tensor& kc, const Tensor& vc, const Tensor& pos0, const Tensor& path0, const Tensor& count0) {
+  const Tensor pos = pos0.contiguous(), path = path0.contiguous(), count = count0.contiguous();
+  check(ferrite_internal_compact_cache(ptr(kc), ptr(vc), (const int32_t*)ptr(pos), (const int32_t*)ptr(path),
+                                       (const int32_t*)ptr(count), kc.dim() == 5 ? kc.size(0) : 1, kc.size(-4),
+                                       kc.size(-3), kc.size(-2), kc.size(-1), path.size(1), code(kc), stream_of(kc)),
+        "ferrite_compact_cache");
+}
+
+// ---------------------------------------------------------------------------
 // Softmax cross-entropy
 // ---------------------------------------------------------------------------
 std::tuple<Tensor, Tensor> cross_entropy_rows(const Tensor& logits0, const Tensor& targets0) {
@@ -652,6 +677,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embed", &embed, nogil());
   m.def("embed_tokens", &embed_tokens, nogil());
   m.def("decode_attention", &decode_attention, nogil());
+  m.def("accept_drafts", &accept_drafts, nogil());
+  m.def("compact_cache", &compact_cache, nogil());
   m.def("cross_entropy", &cross_entropy, nogil());
   m.def("cross_entropy_rows", &cross_entropy_rows, nogil());
   m.def("cross_entropy_grad", &cross_entropy_grad, nogil());

@@ -50,8 +50,8 @@ def _check(qkv, q_weight, k_weight, cos, sin, n_head, n_kv_head, positions) -> N
         if qkv.shape[1] > cos.shape[0]:
             raise ValueError(f"sequence {qkv.shape[1]} longer than the tables' {cos.shape[0]} positions")
     else:
-        if positions.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"positions must be int32 or int64; got {positions.dtype}")
+        if positions.dtype != torch.int32:
+            raise ValueError(f"positions must be int32; got {positions.dtype}")
         if positions.shape not in (qkv.shape[:2], qkv.shape[1:2]):
             raise ValueError(f"expected positions as [B, S] or [S]; got {tuple(positions.shape)} for {tuple(qkv.shape)}")
 
@@ -65,7 +65,7 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, *, n_head: int, n_kv_head: i
     Every q and k head is divided by its root mean square (``eps`` added to the mean square) and multiplied by
     ``q_weight`` or ``k_weight`` [D]; then the pairs (i, i + pairs) of its first ``2 * pairs`` elements, or
     (2 i, 2 i + 1) when ``interleaved``, are rotated by the angles whose f32 ``cos`` and ``sin`` [positions,
-    pairs] (:func:`rope_tables`) lie at the token's position: ``positions`` [B, S] or [S], else 0..S-1. All of it
+    pairs] (:func:`rope_tables`) lie at the token's position: ``positions`` int32 [B, S] or [S], else 0..S-1. All of it
     in f32, rounded once. A position outside the tables gives NaN in its q and k rows. Head dims: even, up to 512.
 
     Differentiable in qkv and the weights, whose gradients are summed in f32 in a fixed order."""

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from ferrite import _hip
+from ferrite.kernels.drafts import accept_drafts, accept_drafts_reference, compact_cache, compact_cache_reference
 from ferrite.kernels.qk_norm_rope import qk_norm_rope, qk_norm_rope_reference, rope_tables
 
 F32, BF16 = torch.float32, torch.bfloat16
@@ -35,6 +36,7 @@ def _heads(**change):
     (dict(cos=torch.ones(2, 32), sin=torch.ones(2, 32)), "longer"),
     (dict(positions=torch.zeros(2, 4, dtype=torch.int32)), "positions"),
     (dict(positions=torch.zeros(3)), "int32"),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), "int32"),
     (dict(qkv=torch.zeros(2, 3, 512, dtype=torch.float64)), "float32 or bfloat16"),
     (dict(q_weight=torch.ones(64).half(), k_weight=torch.ones(64).half()), "float32 or bfloat16"),
 ])
@@ -99,3 +101,98 @@ def test_heads_reference_keeps_lengths_and_turns_by_distance():
         assert abs(float(at(17)[0].square().sum()) - 8) <= 1e-6  # the tables are rounded to f32
         a, b = (float((at(p + 5)[0] * at(p)[1]).sum()) for p in (0, 30))
         assert abs(a - b) <= 1e-5
+
+
+def _accept(**change):
+    a = dict(logits=torch.zeros(2, 3, 8), tokens=torch.zeros(2, 3, dtype=torch.long),
+             parents=torch.zeros(2, 3, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(logits=torch.zeros(6, 8)), "logits as"),
+    (dict(logits=torch.zeros(2, 65, 8)), "1 to 64"),
+    (dict(logits=torch.zeros(2, 0, 8)), "1 to 64"),
+    (dict(logits=torch.zeros(2, 3, 0)), "logits as"),
+    (dict(tokens=torch.zeros(2, 4, dtype=torch.long)), "tokens as"),
+    (dict(tokens=torch.zeros(2, 3)), "tokens must be int64 or int32"),
+    (dict(parents=torch.zeros(3, 2, dtype=torch.int32)), "parents as"),
+    (dict(parents=torch.zeros(2, 3, dtype=torch.long)), "parents must be int32"),
+    (dict(logits=torch.zeros(2, 3, 8).half()), "float32 or bfloat16"),
+])
+def test_accept_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        accept_drafts(**_accept(**change))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        accept_drafts(**_accept())
+
+
+def _compact(**change):
+    a = dict(k_cache=torch.zeros(2, 4, 16, 8), v_cache=torch.zeros(2, 4, 16, 8), pos=torch.zeros(2, dtype=torch.int32),
+             path=torch.zeros(2, 3, dtype=torch.int32), count=torch.zeros(2, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(k_cache=torch.zeros(4, 16, 8)), "caches"),
+    (dict(v_cache=torch.zeros(2, 4, 16, 9)), "one shape"),
+    (dict(v_cache=torch.zeros(2, 4, 16, 8, dtype=BF16)), "share a dtype"),
+    (dict(v_cache=torch.zeros(2, 4, 8, 16).transpose(2, 3)), "contiguous"),
+    (dict(pos=torch.zeros(3, dtype=torch.int32)), "pos as"),
+    (dict(pos=torch.zeros(2)), "pos must be int32"),
+    (dict(path=torch.zeros(2, dtype=torch.int32)), "path as"),
+    (dict(path=torch.zeros(2, 65, dtype=torch.int32)), "1 to 64"),
+    (dict(path=torch.zeros(2, 3, dtype=torch.long)), "path must be int32"),
+    (dict(count=torch.zeros(1, dtype=torch.int32)), "count as"),
+    (dict(k_cache=torch.zeros(2, 4, 16, 8).half(), v_cache=torch.zeros(2, 4, 16, 8).half()), "float32 or bfloat16"),
+])
+def test_compact_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        compact_cache(**_compact(**change))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        compact_cache(**_compact())
+
+
+def test_drafts_abi_refusals():
+    lib = _hip.lib()
+    a = 1 << 12
+    accept = lambda b, t, v, dtype=_hip.F32, ws=None, n=0, p=a: lib.ferrite_internal_accept_drafts(
+        p, a, a, a, a, a, b, t, v, dtype, ws, n, None)
+    assert accept(0, 4, 8) == 0
+    for args, words in (((2, 0, 8), "nodes"), ((2, 65, 8), "nodes"), ((2, 4, 0), "vocabulary"), ((2, 4, 1 << 31), "vocabulary"),
+                        ((-1, 4, 8), "nodes"), ((65535, 2, 8), "65535"), ((2, 4, 8, 7), "dtype")):
+        assert accept(*args) == 1 and words in _hip.last_error(), args
+    assert accept(2, 4, 8, p=None) == 1 and "null" in _hip.last_error()
+    need = lib.ferrite_internal_accept_drafts_workspace(2, 4, 50000)
+    assert need > 0 and accept(2, 4, 50000, ws=a, n=need - 1) == 1 and "workspace" in _hip.last_error()
+    assert accept(2, 4, 50000) == 1 and "workspace" in _hip.last_error()
+    assert lib.ferrite_internal_accept_drafts_workspace(2, 65, 8) == -1
+    compact = lambda layers, b, h, n, d, t, dtype=_hip.BF16, p=a: lib.ferrite_internal_compact_cache(
+        p, a, a, a, a, layers, b, h, n, d, t, dtype, None)
+    for zero in ((0, 2, 2), (2, 0, 2), (2, 2, 0)):
+        assert compact(*zero, 16, 8, 4) == 0
+    for args, words in (((1, 1, 1, 0, 8, 4), "max_len"), ((1, 1, 1, 16, 0, 4), "head dims"), ((1, 1, 1, 16, 8, 0), "nodes"),
+                        ((1, 1, 1, 16, 8, 65), "nodes"), ((1, 1 << 16, 1, 16, 8, 4), "sequences"), ((-1, 1, 1, 16, 8, 4), "layers"),
+                        ((65535, 1, 65535, 16, 65535, 4), "too many"), ((1, 1, 1, 16, 8, 4, 9), "dtype")):
+        assert compact(*args) == 1 and words in _hip.last_error(), args
+    assert compact(1, 1, 1, 16, 8, 4, p=None) == 1 and "null" in _hip.last_error()
+
+
+def test_references_of_the_walk_and_the_moves():
+    """By hand: node 0 wants token 5, its children 1 (token 4) and 2 (token 5); 2 wants 7, its children 3 and 4 both hold it;
+    3 wants 1 and has no child. The second sequence's node 0 is absent, the third's tokens are all wrong."""
+    logits = torch.zeros(3, 5, 9)
+    for node, want in enumerate((5, 0, 7, 1, 2)):
+        logits[:, node, want] = 1
+    tokens = torch.tensor([[3, 4, 5, 7, 7]] * 2 + [[3, 4, 4, 7, 7]])
+    parents = torch.tensor([[-1, 0, 0, 2, 2], [-2, 0, 0, 2, 2], [-1, 0, 0, 2, 2]], dtype=torch.int32)
+    path, count, following = accept_drafts_reference(logits, tokens, parents)
+    assert path.tolist() == [[0, 2, 3, -1, -1], [-1] * 5, [0, -1, -1, -1, -1]]
+    assert count.tolist() == [3, 0, 1] and following.tolist() == [1, -1, 5]
+    k = torch.arange(2 * 10.0).reshape(2, 1, 10, 1).clone()
+    v = -k
+    compact_cache_reference(k, v, torch.tensor([4, 8]), torch.tensor([[0, 2, 3], [0, 1, 2]]), torch.tensor([3, 3]))
+    assert k[0, 0, :, 0].tolist() == [0, 1, 2, 3, 4, 6, 7, 7, 8, 9] and torch.equal(v, -k)
+    assert k[1, 0, :, 0].tolist() == list(range(10, 20))

@@ -118,7 +118,7 @@ def _check_gradients(got, ref, grads, qkv, wq, wk, h, hkv, rot, inter, eps=1e-6)
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (F32, BF16), (BF16, F32)])
 def test_positions_strides_and_weight_types(dev, dtype, wdtype):
     """Views that a program has: columns of a wider row, every second token, sequences that overlap in nothing but
-    their order, an address off 16 bytes; positions per sequence and per token; int64."""
+    their order, an address off 16 bytes; positions per sequence and per token."""
     b, s, h, hkv, d, rot = 3, 17, 4, 2, 64, 32
     width = (h + 2 * hkv) * d
     big, wq, wk, cos, sin = _inputs(dev, b, 2 * s, h, hkv, d + 3, rot, dtype, wdtype, rows=900)
@@ -127,8 +127,8 @@ def test_positions_strides_and_weight_types(dev, dtype, wdtype):
              big[..., :width].flip(0)[:, :s], big[:1, :s, :width].expand(b, s, width)]
     for i, view in enumerate(views):
         n = view.shape[1]
-        pos = torch.randint(0, 900, (view.shape[0], n), generator=torch.Generator().manual_seed(i)).to(dev)
-        for p in (pos.int(), pos, pos[0].int(), pos.t().contiguous().t()):
+        pos = torch.randint(0, 900, (view.shape[0], n), generator=torch.Generator().manual_seed(i)).int().to(dev)
+        for p in (pos, pos[0], pos.t().contiguous().t()):
             leaves = [view.detach(), wq.detach().requires_grad_(), wk.detach().requires_grad_()]
             out = qk_norm_rope(*leaves, cos, sin, n_head=h, n_kv_head=hkv, positions=p)
             full = p.expand(view.shape[0], n)
