@@ -98,6 +98,22 @@ int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64
                                     int64_t workspace_bytes, void* stream);
 
 /*
+ * Attention of T <= 64 drafted nodes per sequence over the caches [B, Hkv, max_len, D] (D 64, 128 or 256): node t hangs on
+ * node parents[b, t] < t, or on the committed tokens (-1), and sees the rows 0 .. pos[b] - 1, its ancestors and itself. Nodes' keys and
+ * values go to rows pos[b] + t. A node whose parent is neither, or that hangs on such a one, is absent: nothing is written for it
+ * and its output is zero. Where pos[b] < 0 or pos[b] + T > max_len nothing is written and the sequence's outputs are NaN. q [B, H, T, D],
+ * k_new and v_new [B, Hkv, T, D] with dense last dimensions and the nine element strides (sequence, head, node of
+ * each; whole 16 bytes); out [B, T, H, D], dense. H is a multiple of Hkv. The workspace, 16-byte aligned, has
+ * ferrite_internal_tree_attention_workspace(...) bytes (-1: sizes out of range); its content need not survive the call.
+ */
+int64_t ferrite_internal_tree_attention_workspace(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d,
+                                                  int dtype);
+int ferrite_internal_tree_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                                    const int32_t* pos, const int32_t* parents, void* out, const int64_t* strides,
+                                    int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d, int dtype,
+                                    float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * The drafted nodes that greedy decoding would have taken: from node 0 (its parent -1), to the child that holds
  * the argmax of the node's logits [B, T, V], while there is one. path [B, T] (-1 behind the visited nodes), count [B],
  * following [B] (the argmax at the last node; -1 with count 0 where node 0 is absent). 1 <= T <= 64, B T <= 65535. A

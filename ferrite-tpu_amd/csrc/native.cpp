@@ -600,6 +600,30 @@ Tensor decode_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, co
 // ---------------------------------------------------------------------------
 // Drafted step
 // ---------------------------------------------------------------------------
+// q, k_new and v_new [B, H, T, D] are read as they lie where rows are dense and start at 16-byte boundaries. The
+// output is stored token-major and returned as its [B, H, T, D] view.
+Tensor tree_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& kc, const Tensor& vc,
+                      const Tensor& pos0, const Tensor& parents0, double scale) {
+  auto rows = [](const Tensor& t) {
+    const int64_t whole = 16 / t.element_size();
+    bool lies = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    for (int i = 0; i < 3; ++i) lies = lies && (t.size(i) == 1 || t.stride(i) % whole == 0);
+    return lies ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const Tensor q = rows(q0), k = rows(k0), v = rows(v0), pos = pos0.contiguous(), parents = parents0.contiguous();
+  const int64_t b = q.size(0), h = q.size(1), t = q.size(2), d = q.size(3), hkv = kc.size(1), max_len = kc.size(2);
+  int64_t strides[9];
+  const Tensor* of[3] = {&q, &k, &v};
+  for (int i = 0; i < 9; ++i) strides[i] = of[i / 3]->size(i % 3) == 1 ? 0 : of[i / 3]->stride(i % 3);
+  Tensor out = at::empty({b, t, h, d}, q.options());
+  const Tensor ws = bytes_on(ferrite_internal_tree_attention_workspace(b, h, hkv, t, max_len, d, code(q)), q);
+  check(ferrite_internal_tree_attention(ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), (const int32_t*)ptr(pos),
+                                        (const int32_t*)ptr(parents), ptr(out), strides, b, h, hkv, t, max_len, d, code(q),
+                                        (float)scale, ptr(ws), size_of(ws), stream_of(q)),
+        "ferrite_tree_attention");
+  return out.transpose(1, 2);
+}
+
 std::tuple<Tensor, Tensor, Tensor> accept_drafts(const Tensor& logits0, const Tensor& tokens0, const Tensor& parents0) {
   const Tensor logits = logits0.contiguous(), tokens = tokens0.to(at::kLong).contiguous(),
                parents = parents0.contiguous();
@@ -677,6 +701,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embed", &embed, nogil());
   m.def("embed_tokens", &embed_tokens, nogil());
   m.def("decode_attention", &decode_attention, nogil());
+  m.def("tree_attention", &tree_attention, nogil());
   m.def("accept_drafts", &accept_drafts, nogil());
   m.def("compact_cache", &compact_cache, nogil());
   m.def("cross_entropy", &cross_entropy, nogil());

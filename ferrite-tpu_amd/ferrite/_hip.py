@@ -153,6 +153,8 @@ INTERNAL: dict[str, tuple] = {
         _c_int,
         [_vp, _c_i64, _c_i64, *[_vp] * 11, *[_c_i64] * 7, _c_int, _c_int, _c_int, _c_f32, _vp, _c_i64, _vp],
     ),
+    "ferrite_internal_tree_attention_workspace": (_c_i64, [*[_c_i64] * 6, _c_int]),
+    "ferrite_internal_tree_attention": (_c_int, [*[_vp] * 9, *[_c_i64] * 6, _c_int, _c_f32, _vp, _c_i64, _vp]),
     "ferrite_internal_accept_drafts_workspace": (_c_i64, [_c_i64] * 3),
     "ferrite_internal_accept_drafts": (
         _c_int,

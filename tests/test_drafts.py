@@ -6,6 +6,7 @@ import torch
 from ferrite import _hip
 from ferrite.kernels.drafts import accept_drafts, accept_drafts_reference, compact_cache, compact_cache_reference
 from ferrite.kernels.qk_norm_rope import qk_norm_rope, qk_norm_rope_reference, rope_tables
+from ferrite.kernels.tree_attention import ancestors, tree_attention, tree_attention_reference
 
 F32, BF16 = torch.float32, torch.bfloat16
 
@@ -196,3 +197,78 @@ def test_references_of_the_walk_and_the_moves():
     compact_cache_reference(k, v, torch.tensor([4, 8]), torch.tensor([[0, 2, 3], [0, 1, 2]]), torch.tensor([3, 3]))
     assert k[0, 0, :, 0].tolist() == [0, 1, 2, 3, 4, 6, 7, 7, 8, 9] and torch.equal(v, -k)
     assert k[1, 0, :, 0].tolist() == list(range(10, 20))
+
+
+def _tree(**change):
+    a = dict(q=torch.zeros(2, 4, 3, 64), k_new=torch.zeros(2, 2, 3, 64), v_new=torch.zeros(2, 2, 3, 64),
+             k_cache=torch.zeros(2, 2, 16, 64), v_cache=torch.zeros(2, 2, 16, 64), pos=torch.zeros(2, dtype=torch.int32),
+             parents=torch.zeros(2, 3, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(q=torch.zeros(2, 3, 64)), "q as"),
+    (dict(q=torch.zeros(2, 3, 3, 64)), "multiple"),
+    (dict(q=torch.zeros(2, 0, 3, 64)), "multiple"),
+    (dict(k_new=torch.zeros(2, 2, 4, 64)), "k_new"),
+    (dict(v_new=torch.zeros(2, 2, 3, 32)), "v_new"),
+    (dict(k_new=torch.zeros(2, 0, 3, 64), v_new=torch.zeros(2, 0, 3, 64)), "multiple"),
+    (dict(q=torch.zeros(2, 4, 65, 64), k_new=torch.zeros(2, 2, 65, 64), v_new=torch.zeros(2, 2, 65, 64)), "1 to 64"),
+    (dict(q=torch.zeros(2, 4, 0, 64), k_new=torch.zeros(2, 2, 0, 64), v_new=torch.zeros(2, 2, 0, 64)), "1 to 64"),
+    (dict(k_cache=torch.zeros(2, 4, 16, 64)), "caches"),
+    (dict(v_cache=torch.zeros(2, 2, 17, 64)), "caches"),
+    (dict(v_new=torch.zeros(2, 2, 3, 64, dtype=BF16)), "share a dtype"),
+    (dict(v_cache=torch.zeros(2, 2, 64, 16).transpose(2, 3)), "contiguous"),
+    (dict(pos=torch.zeros(3, dtype=torch.int32)), "pos"),
+    (dict(parents=torch.zeros(2, 4, dtype=torch.int32)), "parents"),
+    (dict(pos=torch.zeros(2, dtype=torch.long)), "int32"),
+    (dict(parents=torch.zeros(2, 3)), "int32"),
+])
+def test_tree_refusals(change, words):
+    with pytest.raises(ValueError, match=words):
+        tree_attention(**_tree(**change))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        tree_attention(**_tree())
+
+
+def test_tree_abi_refusals():
+    lib = _hip.lib()
+    import ctypes
+
+    a = 1 << 12
+    strides = (ctypes.c_int64 * 9)(*[64] * 9)
+
+    def call(b=2, h=4, hkv=2, t=3, n=1 << 12, d=64, dtype=_hip.BF16, q=a, ws=None, size=0, st=strides):
+        return lib.ferrite_internal_tree_attention(q, a, a, a, a, a, a, a, st, b, h, hkv, t, n, d, dtype, 0.1, ws, size, None)
+
+    assert call(b=0) == 0
+    for change, words in ((dict(dtype=3), "dtype"), (dict(b=-1), "65535"), (dict(h=3), "multiple"), (dict(hkv=0), "multiple"),
+                          (dict(t=0), "nodes"), (dict(t=65), "nodes"), (dict(n=0), "max_len"), (dict(n=1 << 22), "max_len"),
+                          (dict(d=80), "head dim"), (dict(q=None), "null"), (dict(q=a + 8), "aligned"), (dict(), "workspace"),
+                          (dict(st=(ctypes.c_int64 * 9)(*[68] * 9)), "aligned"),
+                          (dict(b=65535, h=65535, hkv=65535, t=1, n=64), "too many heads")):
+        assert call(**change) == 1, change
+        assert words in _hip.last_error(), (change, _hip.last_error())
+    need = lib.ferrite_internal_tree_attention_workspace(2, 4, 2, 3, 1 << 12, 64, _hip.BF16)
+    assert need > 0 and call(ws=a, size=need - 1) == 1 and call(ws=a + 8, size=need) == 1
+    assert lib.ferrite_internal_tree_attention_workspace(2, 4, 2, 3, 64, 64, _hip.BF16) == 0
+    assert lib.ferrite_internal_tree_attention_workspace(2, 4, 3, 3, 64, 64, _hip.BF16) == -1
+
+
+def test_tree_reference_is_attention_along_each_branch():
+    """Each node's output is plain causal attention over the committed rows and the tokens of its own line."""
+    g = torch.Generator().manual_seed(0)
+    mk = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    q, kn, vn, kc, vc = mk(1, 2, 5, 64), mk(1, 1, 5, 64), mk(1, 1, 5, 64), mk(1, 1, 12, 64), mk(1, 1, 12, 64)
+    parents = torch.tensor([[-1, 0, 0, 2, 4]], dtype=torch.int32)  # the last is absent
+    k0, v0 = kc.clone(), vc.clone()
+    out = tree_attention_reference(q, kn, vn, kc, vc, torch.tensor([6]), parents)
+    for t, line in ((0, [0]), (1, [0, 1]), (2, [0, 2]), (3, [0, 2, 3])):
+        keys, values = torch.cat([k0[0, 0, :6], kn[0, 0, line]]), torch.cat([v0[0, 0, :6], vn[0, 0, line]])
+        for h in range(2):
+            e = torch.softmax(keys @ q[0, h, t] / 8, -1) @ values
+            assert torch.allclose(out[0, h, t], e, atol=1e-12)
+    assert not out[0, :, 4].any()
+    assert torch.equal(kc[0, 0, 6:10], kn[0, 0, :4]) and torch.equal(kc[0, 0, 10:], k0[0, 0, 10:])
+    assert ancestors(parents)[0].int().tolist() == [[1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 0, 1, 0, 0], [1, 0, 1, 1, 0], [0] * 5]

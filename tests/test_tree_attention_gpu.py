@@ -1,0 +1,237 @@
+"""GPU tests of the drafted tree's attention (csrc/tree.hip) against the same sums in 64 bits
+(tree_attention_reference on float64 copies).
+
+Tolerances. Inputs are N(0, 1), scale 1 / sqrt(D). f32, u = 2^-24: a score is a sum of D products, off by at
+most D u sum|q k| / sqrt(D), in practice by sqrt(D) u; taken as 32 u (D = 64 to 256, |q k| / sqrt(D) summed about 0.64 sqrt(D)), plus 3 u
+of |score| <= 8 in base-2 units for the scale's and exponent's rounding: 60 u on each weight. The output is a convex sum
+of values up to 5: 2 * 60 u * 5, and the f32 sums of the weights and of the products (each term rounded at the size of the
+partial sum: n u in the worst case, sqrt(n) u in practice, n <= 16384): 128 u * 1. Together under 800 u = 4.8e-5 at most;
+their norms (independent errors) under 1e-6 of the result's. bf16: the weights are rounded to 2^-8 of themselves (independent
+errors: 2^-8 * sqrt(sum p^2 v^2) <= 2^-8 max|v| / 1), and the output by half a step of itself; together 2^-8 (|out| + 5
+sqrt(sum p^2)) with sum p^2 <= 1: relative to the norm 2^-8 * sqrt(2)."""
+
+import pytest
+import torch
+
+from ferrite.kernels.decode_attention import decode_attention
+from ferrite.kernels.drafts import accept_drafts, compact_cache
+from ferrite.kernels.tree_attention import ancestors, tree_attention, tree_attention_reference
+from tests.test_drafts_gpu import trees
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _inputs(dev, b, h, hkv, t, length, d, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda *s: torch.randn(*s, generator=g).to(dtype).to(dev)
+    return mk(b, h, t, d), mk(b, hkv, t, d), mk(b, hkv, t, d), mk(b, hkv, length, d), mk(b, hkv, length, d)
+
+
+def _check(dev, q, kn, vn, kc, vc, pos, parents, scale=None):
+    """The call against the sums in 64 bits; the caches against the rows that belong in them; a second run bitwise."""
+    p, par = torch.tensor(pos, dtype=torch.int32, device=dev), parents.to(dev)
+    dbl = [x.double() for x in (q, kn, vn, kc, vc)]
+    ref = tree_attention_reference(*dbl, p, par, scale=scale)
+    k1, v1, k2, v2 = kc.clone(), vc.clone(), kc.clone(), vc.clone()
+    out = tree_attention(q, kn, vn, k1, v1, p, par, scale=scale)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.transpose(1, 2).is_contiguous()
+    assert torch.equal(k1.double(), dbl[3]) and torch.equal(v1.double(), dbl[4])
+    assert torch.equal(torch.isnan(out), torch.isnan(ref))
+    got, ref = out.double().nan_to_num(7), ref.nan_to_num(7)
+    absent = ~ancestors(par).diagonal(dim1=1, dim2=2)
+    assert not (got * absent[:, None, :, None])[(p >= 0) & (p + q.shape[2] <= kc.shape[2])].any()
+    size = float(ref.norm())
+    if q.dtype == F32:
+        assert float((got - ref).abs().max()) <= 4.8e-5
+        assert float((got - ref).norm()) <= 1e-6 * size
+    else:
+        assert bool(((got - ref).abs() <= 2.0**-8 * (ref.abs() + 5.5)).all())
+        assert float((got - ref).norm()) <= 2.0**-8 * 1.42 * size
+    again = tree_attention(q, kn, vn, k2, v2, p, par, scale=scale)
+    assert torch.equal(out.nan_to_num(7), again.nan_to_num(7))
+    return out
+
+
+CASES = [
+    # b, h, hkv, t, max_len, d, dtype, pos
+    (1, 1, 1, 1, 1, 64, BF16, [0]),
+    (2, 2, 2, 1, 300, 64, BF16, [0, 299]),
+    (3, 4, 4, 8, 512, 128, BF16, [504, 0, 31]),
+    (3, 4, 2, 5, 512, 256, BF16, [507, 32, 33]),
+    (2, 3, 1, 7, 700, 64, BF16, [693, 128]),          # 21 rows: two tiles
+    (2, 8, 2, 16, 1000, 128, BF16, [984, 511]),       # 64 rows: four tiles
+    (2, 8, 1, 13, 1000, 128, BF16, [512, 513]),       # 104 rows: two row blocks, the second short
+    (1, 16, 1, 64, 600, 64, BF16, [536]),             # 1024 rows
+    (2, 6, 1, 64, 900, 256, BF16, [836, 640]),
+    (2, 32, 32, 4, 4100, 128, BF16, [4096, 1]),
+    (9, 64, 64, 3, 2050, 64, BF16, [2047, 0, 1, 127, 128, 129, 1023, 1024, 2000]),
+    (1, 2, 1, 33, 16384, 64, BF16, [16351]),
+    (1, 1, 1, 1, 1, 64, F32, [0]),
+    (3, 4, 4, 8, 250, 128, F32, [242, 0, 17]),
+    (3, 6, 2, 13, 3001, 64, F32, [2988, 750, 1500]),
+    (2, 8, 2, 17, 800, 128, F32, [783, 64]),
+    (2, 2, 2, 40, 700, 256, F32, [660, 640]),
+    (1, 20, 1, 64, 500, 64, F32, [436]),
+    (16, 24, 24, 2, 1030, 64, F32, [1028 - 64 * i for i in range(16)]),
+]
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d,dtype,pos", CASES)
+def test_matches_64_bits(dev, b, h, hkv, t, length, d, dtype, pos):
+    x = _inputs(dev, b, h, hkv, t, length, d, dtype, seed=length + t)
+    _check(dev, *x, pos, trees(b, t, 1))
+    _check(dev, *x, pos, trees(b, t, 2, absent=0.3), scale=0.3 / d**0.5)
+
+
+def test_chains_stars_and_forests(dev):
+    """A chain, children of one node, roots only, the deepest branch, everything absent; 64 nodes and fewer."""
+    for t in (64, 20):
+        idx = torch.arange(t)
+        lines = [idx - 1, torch.where(idx > 0, 0, -1), torch.full((t,), -1), torch.full((t,), -2), torch.full((t,), t),
+                 torch.where(idx > 0, (idx - 1) // 2, -1), torch.where(idx > 1, idx - 2, -1), idx, -1 - idx]
+        parents = torch.stack([x.expand(t) for x in lines]).int()
+        for dtype in (BF16, F32):
+            x = _inputs(dev, len(lines), 4, 2, t, 333, 64, dtype, seed=t)
+            _check(dev, *x, [0, 333 - t, 100, 200, 50, 64, 96, 128, 31], parents)
+
+
+def test_positions_outside_the_cache(dev):
+    x = _inputs(dev, 6, 2, 2, 9, 600, 64, BF16)
+    _check(dev, *x, [-1, 592, 591, 2**31 - 1, -(2**31), 600], trees(6, 9, 3))
+
+
+def test_unseen_values_do_not_matter(dev):
+    """NaN and infinities in the cache's rows past pos, and in the keys and values of absent nodes."""
+    for dtype in (BF16, F32):
+        q, kn, vn, kc, vc = _inputs(dev, 3, 4, 2, 12, 600, 64, dtype)
+        pos, parents = [40, 588, 301], trees(3, 12, 4, absent=0.4)
+        clean = _check(dev, q, kn, vn, kc, vc, pos, parents)
+        there = ancestors(parents).diagonal(dim1=1, dim2=2).to(dev)
+        for bad in (float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min):
+            k, v, a, c = kc.clone(), vc.clone(), kn.clone(), vn.clone()
+            for i, p in enumerate(pos):
+                k[i, :, p:], v[i, :, p:] = bad, bad
+            a[~there[:, None, :, None].expand_as(a)] = bad
+            c[~there[:, None, :, None].expand_as(c)] = bad
+            p = torch.tensor(pos, dtype=torch.int32, device=dev)
+            assert torch.equal(tree_attention(q, a, c, k, v, p, parents.to(dev)), clean)
+
+
+def test_large_scores(dev):
+    """Scores of some hundreds: one key takes all the weight; rows whose keys are at -inf see only the others."""
+    for dtype in (BF16, F32):
+        q, kn, vn, kc, vc = _inputs(dev, 2, 4, 2, 6, 700, 64, dtype)
+        _check(dev, q.sign() * 8, kn.sign() * 4, vn, kc.sign() * 4, vc, [694, 333], trees(2, 6, 5))
+        k = kc.clone()
+        k[0, 0, 100:500, 0] = -float("inf")
+        qp = q.clone()
+        qp[..., 0] = qp[..., 0].abs() + 0.1
+        _check(dev, qp, kn, vn, k, vc, [600, 20], trees(2, 6, 5))
+
+
+def test_strided_inputs(dev):
+    """q, k_new and v_new where a projection leaves them (token-major, in one row), and views that need a copy."""
+    for dtype in (BF16, F32):
+        b, h, hkv, t, d = 2, 4, 2, 10, 64
+        g = torch.Generator().manual_seed(3)
+        qkv = torch.randn(b, t, (h + 2 * hkv), d, generator=g).to(dtype).to(dev)
+        q, kn, vn = (x.transpose(1, 2) for x in qkv.split([h, hkv, hkv], 2))
+        _, _, _, kc, vc = _inputs(dev, b, h, hkv, t, 500, d, dtype)
+        want = _check(dev, q, kn, vn, kc, vc, [480, 7], trees(b, t, 1))
+        assert torch.equal(want, _check(dev, q.contiguous(), kn.contiguous(), vn.contiguous(), kc, vc, [480, 7], trees(b, t, 1)))
+        odd = torch.randn(b, t, (h + 2 * hkv) * d + 1, generator=g).to(dtype).to(dev)[..., 1:].unflatten(2, (-1, d))
+        _check(dev, *(x.transpose(1, 2) for x in odd.split([h, hkv, hkv], 2)), kc, vc, [480, 7], trees(b, t, 1))
+        _check(dev, q, kn[:, :1].expand(b, hkv, t, d), vn[:1].expand(b, hkv, t, d), kc, vc, [480, 7], trees(b, t, 1))
+
+
+def test_one_node_is_decode_attention(dev):
+    q, kn, vn, kc, vc = _inputs(dev, 3, 4, 4, 1, 900, 128, F32)
+    pos = torch.tensor([0, 450, 899], dtype=torch.int32, device=dev)
+    k1, v1 = kc.clone(), vc.clone()
+    a = tree_attention(q, kn, vn, kc, vc, pos, torch.full((3, 1), -1, dtype=torch.int32, device=dev))
+    e = decode_attention(q[:, :, 0], kn[:, :, 0], vn[:, :, 0], k1, v1, pos)
+    assert torch.equal(kc, k1) and torch.equal(vc, v1) and float((a[:, :, 0] - e).abs().max()) <= 4.8e-5
+
+
+def test_empty_batch(dev):
+    q, kn, vn, kc, vc = _inputs(dev, 0, 4, 2, 3, 50, 64, BF16)
+    z = torch.zeros(0, dtype=torch.int32, device=dev)
+    assert tree_attention(q, kn, vn, kc, vc, z, z.reshape(0, 3)).shape == (0, 4, 3, 64)
+
+
+def test_long_cache_offsets(dev):
+    """A head whose cache passes 2^31 bytes: the last rows are read and written where they are."""
+    length, d = (1 << 21) + 300, 256
+    kc = torch.zeros(1, 1, length, d, device=dev, dtype=F32)
+    vc = torch.zeros(1, 1, length, d, device=dev, dtype=F32)
+    q, kn, vn = (torch.randn(1, 1, 3, d, device=dev) for _ in range(3))
+    pos = length - 3
+    kc[0, 0, pos - 5], vc[0, 0, pos - 5] = 40 * q[0, 0, 1] / q[0, 0, 1].norm(), 2.0
+    kc[0, 0, 17], vc[0, 0, 17] = 40 * q[0, 0, 0] / q[0, 0, 0].norm(), -3.0
+    out = tree_attention(q, kn * 0, vn, kc, vc, torch.tensor([pos], dtype=torch.int32, device=dev),
+                         torch.tensor([[-1, -1, -1]], dtype=torch.int32, device=dev), scale=1.0)
+    assert float((out[0, 0, 1] - 2.0).abs().max()) <= 1e-3 and float((out[0, 0, 0] + 3.0).abs().max()) <= 1e-3
+    assert torch.equal(vc[0, 0, pos:], vn[0, 0]) and not kc[0, 0, pos:].any() and not vc[0, 0, pos - 4:pos].any()
+
+
+@pytest.mark.parametrize("length", [200, 1500])
+def test_streams_and_graphs(dev, length):
+    """Other streams, two captured graphs replayed in turn on their own streams, positions and trees that change."""
+    b, t = 3, 12
+    q, kn, vn, kc, vc = _inputs(dev, b, 4, 2, t, length, 64, BF16)
+    pos = torch.tensor([5, length - t, 77], dtype=torch.int32, device=dev)
+    parents = trees(b, t, 1).to(dev)
+    call = lambda: tree_attention(q, kn, vn, kc, vc, pos, parents)
+    want = call().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call()
+        side.synchronize()
+        assert torch.equal(other, want)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out, torch.cuda.Stream()))
+    for seed in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(seed)))
+        pos.copy_(torch.tensor([seed, length - t - seed, 50 + seed], dtype=torch.int32))
+        parents.copy_(trees(b, t, seed, absent=0.2))
+        torch.cuda.synchronize()
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        for _, out, _ in graphs:
+            assert torch.equal(out, want)
+    for graph, _, _ in graphs:
+        graph.reset()
+
+
+def test_accepted_rows_make_the_cache_of_plain_decoding(dev):
+    """Tree attention, acceptance and compaction in turn: the cache then holds the accepted path's rows as decoding one
+    token after another would have left them."""
+    b, h, t, d, length, v = 2, 2, 10, 64, 128, 50
+    q, kn, vn, kc, vc = _inputs(dev, b, h, h, t, length, d, F32, seed=4)
+    pos = torch.tensor([20, 100], dtype=torch.int32, device=dev)
+    parents = trees(b, t, 8)
+    logits = torch.randn(b, t, v, generator=torch.Generator().manual_seed(2))
+    tokens = logits.argmax(-1).gather(1, parents.clamp(min=0).long())  # every draft is right: the walk takes first children
+    k0, v0 = kc.clone(), vc.clone()
+    out = tree_attention(q, kn, vn, kc, vc, pos, parents.to(dev))
+    path, count, _ = accept_drafts(logits.to(dev), tokens.to(dev), parents.to(dev))
+    compact_cache(kc, vc, pos, path, count)
+    assert int(count.min()) > 2
+    for i in range(b):
+        for n, node in enumerate(path[i, : count[i]].tolist()):
+            one = lambda x: x[i:i + 1, :, node]
+            at = pos[i:i + 1] + n
+            e = decode_attention(one(q), one(kn), one(vn), k0[i:i + 1], v0[i:i + 1], at)
+            assert float((e - out[i:i + 1, :, node]).abs().max()) <= 4.8e-5
+        rows = int(pos[i] + count[i])
+        assert torch.equal(kc[i, :, :rows], k0[i, :, :rows]) and torch.equal(vc[i, :, :rows], v0[i, :, :rows])
