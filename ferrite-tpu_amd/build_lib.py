@@ -57,9 +57,13 @@ HIPCC_FLAGS = [
 # loop left partly rolled indexes the fragment and accumulator arrays at run time, which puts them
 # in scratch (2,304 bytes per lane); fully unrolled it keeps them in registers (no scratch). The
 # other kernels come out the same.
+#
+# tree.hip: MFMA results in VGPRs, as in attention.hip: the softmax reads the scores on the VALU, and with the scores
+# in AGPRs the kernels of 64 query rows at head dim 128 need 440 to 720 bytes of scratch a lane (none so).
 SOURCE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-structurizecfg-skip-uniform-regions=true",
                       "-mllvm", "-pragma-unroll-threshold=200000"],
+    "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -608,6 +608,7 @@ Tensor tree_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, cons
     const int64_t whole = 16 / t.element_size();
     bool lies = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
     for (int i = 0; i < 3; ++i) lies = lies && (t.size(i) == 1 || t.stride(i) % whole == 0);
+    lies = lies && t.size(2) * t.stride(2) < (1 << 28);  // nodes within 32-bit offsets of a head's first
     return lies ? t : t.clone(at::MemoryFormat::Contiguous);
   };
   const Tensor q = rows(q0), k = rows(k0), v = rows(v0), pos = pos0.contiguous(), parents = parents0.contiguous();

@@ -31,12 +31,13 @@ struct TreeArgs {
   void *kc, *vc;
   const int32_t *pos, *parents;
   void* out;    // [B, T, H, D]
-  char* part;   // workspace, or null: one chunk, written to out
+  char* part;   // workspace, or null: every workgroup takes one whole head
   int64_t qs[3], ks[3], vs[3];  // element strides of q, k_new and v_new: sequence, head, node
-  int64_t items;                // B Hkv chunks
-  int H, Hkv, G, T, L, rows;    // rows = G T
-  int chunks, row_blocks, wave_rows;
-  float c;  // scale log2(e)
+  int B, H, Hkv, G, T, L, rows;  // rows = G T
+  int row_groups;                // workgroups' row blocks per head
+  int groups, least;             // workgroups that share the work, and steps of one at least
+  float c;                       // |scale| log2(e)
+  uint32_t flip;                 // sign bits to flip in q (a negative scale)
 };
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 acc, bf16) {
@@ -54,64 +55,58 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 ac
 template <typename T>
 constexpr int kTiles = sizeof(T) == 2 ? 2 : 1;
 
+// Bytes that a descriptor's range covers at most. What lies past it is past every range: loads there read zeros and touch
+// no memory.
+constexpr uint32_t kMostBytes = 0xfffe0000u;
+
 template <typename T, int D>
 struct Step {
   static constexpr int NS = kTiles<T>, KEYS = 16 * NS, RB = D * (int)sizeof(T), KB = RB / 64, VD = RB / 64;
   u32x4 k[NS][KB];           // key 16 n + lane % 16, bytes 64 c + 16 (lane / 16)
   uint32_t v[4 * NS][VD];    // key 16 n + 4 (lane / 16) + i, bytes (lane % 16) RB / 16 ..
 
-  // Rows key0 .. of a head's cache; past the descriptor's range they are zeros.
-  __device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t rs, int key0, int lane) {
-    const uint32_t at = (uint32_t)(key0 + (lane & 15)) * RB + (lane >> 4) * 16;
+  // Rows first .. of what the descriptor covers, `bytes` from one to the next; past its range they are zeros. Read once
+  // (non-temporal).
+  __device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t rs, uint32_t first, uint32_t bytes, int lane) {
+    const uint32_t at = first + (lane & 15) * bytes + (lane >> 4) * 16;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int c = 0; c < KB; ++c)
-        k[n][c] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(at + n * 16 * RB + c * 64), 0, 0);
+        k[n][c] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(at + n * 16 * bytes + c * 64), 0, 2);
   }
-  __device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t rs, int key0, int lane) {
-    const uint32_t at = (uint32_t)(key0 + 4 * (lane >> 4)) * RB + (lane & 15) * (RB / 16);
+  __device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t rs, uint32_t first, uint32_t bytes, int lane) {
+    const uint32_t at = first + 4 * (lane >> 4) * bytes + (lane & 15) * (RB / 16);
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int off = (int)(at + (16 * n + i) * RB);
+        const uint32_t off = at + (16 * n + i) * bytes;
         if constexpr (VD == 2) {
-          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0);
+          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, (int)off, 0, 2);
           v[4 * n + i][0] = x[0];
           v[4 * n + i][1] = x[1];
         } else {
 #pragma unroll
           for (int w = 0; w < VD; w += 4) {
-            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 4 * w, 0, 0);
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + 4 * w), 0, 2);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[4 * n + i][w + e] = x[e];
           }
         }
       }
   }
-  // The drafted nodes node0 .. ; zeros for one that is not there.
-  __device__ __forceinline__ void load_nodes(const T* kn, int64_t kstep, const T* vn, int64_t vstep, int node0, uint64_t there,
-                                             int lane) {
+  // Values of the keys whose bit of `there` (bit 0: the step's first) is not set, whatever they hold, as zeros.
+  __device__ __forceinline__ void drop_absent(uint32_t there, int lane) {
+    there >>= 4 * (lane >> 4);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const int node = node0 + 16 * n + (lane & 15);
-      const bool on = node < kMaxNodes && (there >> (node & 63) & 1);
-#pragma unroll
-      for (int c = 0; c < KB; ++c) {
-        k[n][c] = u32x4{0, 0, 0, 0};
-        if (on)
-          k[n][c] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(kn + node * kstep) + c * 64 + (lane >> 4) * 16);
-      }
+    for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = node0 + 16 * n + 4 * (lane >> 4) + i;
-        const bool von = at < kMaxNodes && (there >> (at & 63) & 1);
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(vn + at * vstep) + (lane & 15) * (RB / 16));
+        const uint32_t keep = there >> (16 * n + i) & 1 ? ~0u : 0u;
 #pragma unroll
-        for (int w = 0; w < VD; ++w) v[4 * n + i][w] = von ? p[w] : 0;
+        for (int w = 0; w < VD; ++w) v[4 * n + i][w] &= keep;
       }
-    }
   }
 };
 
@@ -138,12 +133,11 @@ __device__ __forceinline__ void add_pv(const Step<float, D>& st, const f32x4 (&p
       o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[i][j]), p[0][i], o[j], 0, 0, 0);
 }
 
-// The lanes' nodes: bit s of the result for node `lane` says whether it sees node s (its ancestors and itself); 0
+// The lanes' nodes, each with its parent (-2: no node): bit s of the result for node `lane` says whether it sees node s (its ancestors and itself); 0
 // where the node, or one that it hangs on, is absent (its parent neither -1 nor an earlier node). By doubling: after
 // round r a lane holds its 2^r nearest ancestors and points past them.
-__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int t, int lane) {
-  int up = lane < t ? parents[lane] : -2;
-  if (up < -1 || up >= lane) up = -2;
+__device__ __forceinline__ uint64_t ancestors(int parent, int lane) {
+  int up = parent < -1 || parent >= lane ? -2 : parent;
   uint64_t sees = 1ull << lane;
 #pragma unroll
   for (int r = 0; r < 6; ++r) {
@@ -175,320 +169,714 @@ __device__ __forceinline__ float sum16(float x) {
   return lane32_sum(x);
 }
 
-// Workspace: u64 [B Hkv] which nodes are there, then per chunk and row (m, l), then the unnormalised outputs.
-struct Parts {
-  uint64_t* there;
-  f32x2* ml;   // [B Hkv, chunks, rows]
-  float* acc;  // [B Hkv, chunks, rows, D]
+// The work is a line of steps: sequence by sequence, (head, row group) by (head, row group), the steps of its cached keys and
+// of its nodes (one step for a sequence that has no place in the cache). It is cut evenly over the workgroups, so each
+// has at most one (head, row group) that it shares with workgroups before it and one with workgroups
+// behind it; their states go to its two slots of the workspace.
+__device__ __forceinline__ int pos_of(const TreeArgs& a, int b) { return a.pos[min(b, a.B - 1)]; }
+__device__ __forceinline__ bool in_cache(const TreeArgs& a, int p) { return p >= 0 && p <= a.L - a.T; }
+template <int KEYS>
+__device__ __forceinline__ int steps_at(const TreeArgs& a, int b, int p) {
+  return b >= a.B ? 0 : in_cache(a, p) ? (p + KEYS - 1) / KEYS + (a.T + KEYS - 1) / KEYS : 1;
+}
+__device__ __forceinline__ int wave_total(int x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, kWave);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int share_of(const TreeArgs& a, int total) {  // steps of a workgroup
+  return max((total + a.groups - 1) / a.groups, a.least);
+}
+
+// Where a workgroup is on the line: steps [s0, ..) of the hr-th (head, row group) of sequence b, [cur, end) its own.
+template <int KEYS>
+struct Cursor {
+  int b, p, steps, hr, s0, cur, end;
+
+  // false: nothing to do.
+  __device__ __forceinline__ bool start(const TreeArgs& a, int lane) {
+    const int per_seq = a.Hkv * a.row_groups;
+    int seq_at = 0;  // where on the line the sequence begins
+    if (a.part) {
+      int sum = 0, p0 = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int x = pos_of(a, b0 + lane);
+        p0 = b0 ? p0 : x;
+        sum += steps_at<KEYS>(a, b0 + lane, x);
+      }
+      const int total = wave_total(sum) * per_seq, share = share_of(a, total);
+      if ((int64_t)blockIdx.x * share >= total) return false;
+      cur = (int)blockIdx.x * share;
+      end = min(cur + share, total);
+      int before = 0;
+      b = p = 0;
+      steps = 1;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int x = b0 ? pos_of(a, b0 + lane) : p0, mine = steps_at<KEYS>(a, b0 + lane, x);
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int y = __shfl_up(upto, off, kWave);
+          upto += lane >= off ? y : 0;
+        }
+        const uint64_t past = __ballot((before + upto) * per_seq > cur);
+        if (past) {
+          const int at = __builtin_ctzll(past);
+          b = b0 + at;
+          p = __shfl(x, at, kWave);
+          steps = __shfl(mine, at, kWave);
+          seq_at = (before + __shfl(upto, at, kWave) - steps) * per_seq;
+          break;
+        }
+        before += __shfl(upto, 63, kWave);
+      }
+    } else {
+      b = (int)(blockIdx.x / per_seq);
+      p = pos_of(a, b);
+      steps = steps_at<KEYS>(a, b, p);
+      cur = (int)(blockIdx.x % per_seq) * steps;
+      end = cur + steps;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    p = __builtin_amdgcn_readfirstlane(p);
+    steps = __builtin_amdgcn_readfirstlane(steps);
+    cur = __builtin_amdgcn_readfirstlane(cur);
+    end = __builtin_amdgcn_readfirstlane(end);
+    const int at = cur - __builtin_amdgcn_readfirstlane(seq_at);
+    hr = at / steps;
+    s0 = at - hr * steps;
+    return true;
+  }
+  // Behind steps [s0, s1).
+  __device__ __forceinline__ void pass(const TreeArgs& a, int s1) {
+    cur += s1 - s0;
+    s0 = 0;
+    if (++hr == a.Hkv * a.row_groups && cur < end) {
+      hr = 0;
+      ++b;
+      p = __builtin_amdgcn_readfirstlane(pos_of(a, b));
+      steps = steps_at<KEYS>(a, b, p);
+    }
+  }
 };
-__host__ __device__ inline int64_t parts_bytes(int64_t heads, int64_t chunks, int64_t rows, int64_t d) {
-  return cdiv(heads, 2) * 16 + cdiv(heads * chunks * rows, 2) * 16 + heads * chunks * rows * d * 4;
-}
-__device__ __forceinline__ Parts parts_of(char* ws, int64_t heads, int64_t chunks, int64_t rows) {
-  char* ml = ws + cdiv(heads, 2) * 16;
-  return {reinterpret_cast<uint64_t*>(ws), reinterpret_cast<f32x2*>(ml),
-          reinterpret_cast<float*>(ml + cdiv(heads * chunks * rows, 2) * 16)};
+
+// Slots of `rows` rows: (m, l) of each, then the unnormalised outputs.
+struct Parts {
+  f32x2* ml;   // [slots, rows]
+  float* acc;  // [slots, rows, D]
+};
+__host__ __device__ inline int64_t parts_bytes(int64_t slots, int64_t rows, int64_t d) { return slots * rows * (8 + 4 * d); }
+__device__ __forceinline__ Parts parts_of(char* ws, int64_t slots, int64_t rows) {
+  return {reinterpret_cast<f32x2*>(ws), reinterpret_cast<float*>(ws + slots * rows * 8)};
 }
 
-// One row block (16 NT rows) over one chunk of a head's cache; W waves with a stretch of it each. The last
-// chunk's last wave takes the drafted nodes too, which come from k_new and v_new: no workgroup reads a row that
-// another writes.
+// Where the query fragments would not fit in a wave's registers beside O and two steps of keys and values they lie in LDS.
+template <typename T, int D, int NT>
+constexpr bool kQueriesInLds = NT * D * (int)sizeof(T) / 64 >= 16 || D * (int)sizeof(T) >= 512;
+// Two steps of keys and values in registers, one under way, where they fit; else the next step's keys are loaded when the scores
+// are done, and its values when it begins.
+template <typename T, int D, int NT>
+constexpr bool kPingPong = D == 64 || (D == 128 && (sizeof(T) == 2 || NT < 4));
+// Waves that a SIMD is to hold.
+template <typename T, int D, int NT>
+constexpr int kWavesPerSimd = NT == 1 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : NT == 2 && D == 64 ? 2 : 1;
+// LDS: the queries, and after the last step the waves' O with its (m, l).
 template <typename T, int D, int NT, int W>
-__global__ __launch_bounds__(64 * W) void tree_attn_kernel(TreeArgs a) {
+constexpr int kTreeLds = std::max(kQueriesInLds<T, D, NT> ? NT * (D * (int)sizeof(T) / 64) * 1024 : 0,
+                                  W * NT * 16 * (D + 4 + 2) * 4);
+
+// A row group of 16 NT rows, its steps dealt to W waves.
+template <typename T, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
   typedef Step<T, D> S;
-  constexpr int NS = S::NS, KEYS = S::KEYS, KB = S::KB, VE = D / 16;
-  constexpr int DP = 512 / W < D ? 512 / W : D, PASSES = D / DP;  // columns per pass of the waves' merge
-  __shared__ __attribute__((aligned(16))) float red[W][16][DP + 4];
-  __shared__ float red_m[W][16], red_l[W][16];
+  constexpr int NS = S::NS, KEYS = S::KEYS, KB = S::KB, VE = D / 16, ROWS = 16 * NT;
+  constexpr bool QL = kQueriesInLds<T, D, NT>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  u32x4* const queries = reinterpret_cast<u32x4*>(lds);  // [NT KB][64]
+  float* const red = reinterpret_cast<float*>(lds);              // [W][16 NT][D + 4]
+  float *const red_m = red + W * NT * 16 * (D + 4), *const red_l = red_m + W * NT * 16;  // [W][16 NT]
 
-  // Row blocks of one item lie 8 workgroups apart: on one XCD, whose L2 then holds the chunk for all of them.
-  const int64_t group = blockIdx.x / (8 * a.row_blocks);
-  const int rest = (int)(blockIdx.x - group * 8 * a.row_blocks), block = rest / 8;
-  const int64_t item = group * 8 + rest % 8;
-  if (item >= a.items) return;
-  const int chunk = (int)(item % a.chunks);
-  const int64_t head = item / a.chunks;  // b Hkv + h
-  const int64_t b = head / a.Hkv;
-  const int h = (int)(head - b * a.Hkv);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, q0 = lane & 15;
-  const int p = a.pos[b];
-  const bool valid = p >= 0 && p <= a.L - a.T;
-  const int cached = valid ? p : 0;
-  const bool drafts = chunk == a.chunks - 1;
-  if (!drafts && (int64_t)chunk * W * a.wave_rows >= cached) return;  // an empty chunk, which nobody reads
+  Cursor<KEYS> at;
+  if (!at.start(a, lane)) return;
+  for (int slot = 2 * (int)blockIdx.x; at.cur < at.end; slot = 2 * (int)blockIdx.x + 1) {  // what it shares comes first or last
+    const int b = at.b, p = at.p, s0 = at.s0, s1 = min(at.steps, s0 + at.end - at.cur);
+    const int h = at.hr / a.row_groups, row0 = (at.hr % a.row_groups) * ROWS;
+    const bool valid = in_cache(a, p);
+    const int cached = valid ? p : 0, cached_steps = (cached + KEYS - 1) / KEYS;
 
-  // Query rows: row r is node r % T of head h G + r / T. Rows past the last read as zeros and are not stored.
-  u32x4 q[NT][KB];
-  int node[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = (block * NT + n) * 16 + q0;
-    const int gh = r / a.T;
-    node[n] = r - gh * a.T;
-    const char* src = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.qs[0] + (h * a.G + gh) * a.qs[1] + node[n] * a.qs[2]);
-#pragma unroll
-    for (int c = 0; c < KB; ++c) {
-      q[n][c] = u32x4{0, 0, 0, 0};
-      if (r < a.rows) q[n][c] = *reinterpret_cast<const u32x4*>(src + c * 64 + g * 16);
-    }
-  }
-
-  float m[NT], l[NT];
-  f32x4 o[NT][VE];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  S st;
-  f32x4 s[NT][NS];
-  auto scores = [&] {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int t = 0; t < NS; ++t) {
-        s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KB; ++c) s[n][t] = mfma16(st.k[t][c], q[n][c], s[n][t], T{});
-      }
-  };
-  // sees(n, t, i): whether row tile n's query of this lane sees key 16 t + 4 g + i of the step.
-  auto softmax_pv = [&](auto masked, auto&& sees) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < NS; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][t][i] *= a.c;
-          if (masked.value && !sees(n, t, i)) s[n][t][i] = -INFINITY;
-          mx = fmaxf(mx, s[n][t][i]);
-        }
-      mx = fmaxf(m[n], max16(mx));
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      if (__any(mx > m[n])) {
-        const float f = __builtin_amdgcn_exp2f(m[n] - ref);
-        l[n] *= f;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) o[n][j] *= f;
-      }
-      m[n] = mx;
-#pragma unroll
-      for (int t = 0; t < NS; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][t][i] = __builtin_amdgcn_exp2f(s[n][t][i] - ref);
-          l[n] += s[n][t][i];
-        }
-      add_pv<D>(st, s[n], o[n]);
-    }
-  };
-
-  const int64_t base = head * a.L * D;
-  const uint32_t bytes = (uint32_t)__builtin_amdgcn_readfirstlane(cached) * (uint32_t)S::RB;
-  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(static_cast<T*>(a.kc) + base), (short)0, (int)bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(static_cast<T*>(a.vc) + base), (short)0, (int)bytes, 0x00020000);
-  const int from = __builtin_amdgcn_readfirstlane((chunk * W + wave) * a.wave_rows);
-  const int to = __builtin_amdgcn_readfirstlane(min(from + a.wave_rows, cached));
-  if (from < to) st.load_k(krs, from, lane);
-  for (int key = from; key < to; key += KEYS) {
-    st.load_v(vrs, key, lane);
-    scores();
-    if (key + KEYS < to) st.load_k(krs, key + KEYS, lane);
-    if (key + KEYS <= cached)
-      softmax_pv(std::false_type{}, [](int, int, int) { return true; });
-    else
-      softmax_pv(std::true_type{}, [&](int, int t, int i) { return key + 16 * t + 4 * g + i < cached; });
-  }
-
-  uint64_t there = 0;
-  if (drafts && valid) {
-    const uint64_t line = ancestors(a.parents + b * a.T, a.T, lane);
-    there = __ballot(line != 0);
+    // This wave's steps: s0 + wave and every W-th after it, below s1. Those before whole_to are 16 NS cached keys each, then come the
+    // cache's last keys, from cached_steps on the nodes.
+    const int64_t base = ((int64_t)b * a.Hkv + h) * a.L * D;
     const T* kn = static_cast<const T*>(a.kn) + b * a.ks[0] + h * a.ks[1];
     const T* vn = static_cast<const T*>(a.vn) + b * a.vs[0] + h * a.vs[1];
-    if (wave == W - 1) {
-      uint64_t mine[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mine[n] = __shfl((unsigned long long)line, node[n], kWave);
-      for (int at = 0; at < a.T; at += KEYS) {
-        st.load_nodes(kn, a.ks[2], vn, a.vs[2], at, there, lane);
-        scores();
-        softmax_pv(std::true_type{}, [&](int n, int t, int i) {
-          const int k = at + 16 * t + 4 * g + i;
-          return k < kMaxNodes && (mine[n] >> (k & 63) & 1);
-        });
-      }
-    }
-    if (block == 0) {
-      constexpr int VEC = S::RB / 16;
-      for (int e = threadIdx.x; e < a.T * VEC; e += 64 * W) {
-        const int t = e / VEC, at = e % VEC;
-        if (!(there >> t & 1)) continue;
-        const int64_t row = (base + (int64_t)(p + t) * D) / (16 / (int)sizeof(T)) + at;
-        static_cast<u32x4*>(a.kc)[row] = reinterpret_cast<const u32x4*>(kn + t * a.ks[2])[at];
-        static_cast<u32x4*>(a.vc)[row] = reinterpret_cast<const u32x4*>(vn + t * a.vs[2])[at];
-      }
-    }
-  }
+    const uint32_t kbytes = (uint32_t)a.ks[2] * sizeof(T), vbytes = (uint32_t)a.vs[2] * sizeof(T);
+    int s = valid ? s0 + wave : s1;
+    const int whole_to = cached / KEYS;
+    // A load past the last step goes out too, from past every range, which reads nothing: behind a branch the waits would count on
+    // none of it and wait for the step under way too.
+    auto range = [](const T* x, uint32_t bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(const_cast<T*>(x)), (short)0, (int)bytes, 0x00020000);
+    };
+    auto load_k = [&](S& st, int at) {
+      const bool old = at < cached_steps;
+      const uint32_t step = old ? S::RB : kbytes, first = (uint32_t)(at - (old ? 0 : cached_steps)) * KEYS * step;
+      st.load_k(range(old ? static_cast<const T*>(a.kc) + base : kn, old ? (uint32_t)cached * S::RB : (a.T - 1) * step + S::RB),
+                                 at < s1 ? first : kMostBytes, at < s1 ? step : 0, lane);
+    };
+    auto load_v = [&](S& st, int at) {
+      const bool old = at < cached_steps;
+      const uint32_t step = old ? S::RB : vbytes, first = (uint32_t)(at - (old ? 0 : cached_steps)) * KEYS * step;
+      st.load_v(range(old ? static_cast<const T*>(a.vc) + base : vn, old ? (uint32_t)cached * S::RB : (a.T - 1) * step + S::RB),
+                                 at < s1 ? first : kMostBytes, at < s1 ? step : 0, lane);
+    };
+    const int parent = a.parents[(int64_t)b * a.T + min(lane, a.T - 1)];
+    S even;
+    load_k(even, s);
+    if constexpr (kPingPong<T, D, NT>) load_v(even, s);
 
-  // The waves' states, 16 rows at a time: weights 2^(m_w - max), then the sums over the waves in their order.
-  Parts parts{};
-  if (a.part) {
-    parts = parts_of(a.part, a.items / a.chunks, a.chunks, a.rows);
-    if (drafts && block == 0 && threadIdx.x == 0) parts.there[head] = there;
-  }
+    // Query rows: row r is node r % T of head h G + r / T. In place of rows past the last it is read again, and not stored. No load
+    // behind a branch of its own: each would be waited for alone.
+    u32x4 q[NT][QL ? 1 : KB];
+    int node[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const float lt = sum16(l[n]);
+    for (int n = 0; n < NT; ++n) {
+      const int r = min(row0 + n * 16 + q0, a.rows - 1);
+      const int gh = r / a.T;
+      node[n] = r - gh * a.T;
+      if (QL && wave != 0) continue;
+      const char* src = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.qs[0] + (h * a.G + gh) * a.qs[1] + node[n] * a.qs[2]);
 #pragma unroll
-    for (int pass = 0; pass < PASSES; ++pass) {
-      __syncthreads();
+      for (int c = 0; c < KB; ++c) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(src + c * 64 + g * 16) ^ a.flip;
+        if constexpr (QL)
+          queries[(n * KB + c) * 64 + lane] = x;
+        else
+          q[n][c] = x;
+      }
+    }
+    uint64_t there = 0, line = 0;
+    const bool drafts = valid && s1 > cached_steps;
+    if (drafts) {
+      line = ancestors(lane < a.T ? parent : -2, lane);
+      there = __ballot(line != 0);
+    }
+    if (QL) __syncthreads();
+
+    float m[NT], l[NT];
+    f32x4 o[NT][VE];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < VE; ++j) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Step `at`: scores of its keys, the running maximum (m, in units of log2) and sum, O.
+    auto add_step = [&](S& st, int at, auto&& after_scores) {
+      f32x4 x[NT][NS];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int t = 0; t < NS; ++t) x[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KB; ++c) {
+          u32x4 y;
+          if constexpr (QL)
+            y = queries[(n * KB + c) * 64 + lane];
+          else
+            y = q[n][c];
+#pragma unroll
+          for (int t = 0; t < NS; ++t) x[n][t] = mfma16(st.k[t][c], y, x[n][t], T{});
+        }
+      }
+      after_scores();
+      if (at >= whole_to) {  // not every row sees every key: bit k of `sees` is the step's key k
+        const bool old = at < cached_steps;
+        const int first = old ? 0 : (at - cached_steps) * KEYS;
+        if (!old) st.drop_absent((uint32_t)(there >> first), lane);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint64_t mine = __shfl((unsigned long long)line, node[n], kWave) >> first;
+          const uint32_t sees = (old ? (1u << (cached - at * KEYS)) - 1 : (uint32_t)mine) >> (4 * g);
+#pragma unroll
+          for (int t = 0; t < NS; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[n][t][i] = sees >> (16 * t + i) & 1 ? x[n][t][i] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[n][t][i]);
+        mx = fmaxf(m[n], max16(mx) * a.c);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx > m[n])) {
+          const float f = __builtin_amdgcn_exp2f(m[n] - ref);
+          l[n] *= f;
+#pragma unroll
+          for (int j = 0; j < VE; ++j) o[n][j] *= f;
+        }
+        m[n] = mx;
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[n][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][t][i], a.c, -ref));
+            l[n] += x[n][t][i];
+          }
+        add_pv<D>(st, x[n], o[n]);
+      }
+    };
+
+    // The next step's loads are under way while one is added.
+    if constexpr (kPingPong<T, D, NT>) {
+      S odd;
+      auto load = [&](S& st, int at) {
+        asm volatile("" ::: "memory");  // the queries' LDS reads stay in their step
+        load_k(st, at);
+        load_v(st, at);
+      };
+      while (s < s1) {
+        load(odd, s + W);
+        add_step(even, s, [] {});
+        s += W;
+        if (s >= s1) break;
+        load(even, s + W);
+        add_step(odd, s, [] {});
+        s += W;
+      }
+    } else {
+      for (; s < s1; s += W) {
+        asm volatile("" ::: "memory");
+        load_v(even, s);
+        add_step(even, s, [&] { load_k(even, s + W); });
+      }
+    }
+
+    // The nodes' rows of the cache, by the workgroup that has the first step of nodes of the head's first rows.
+    if (drafts && s0 <= cached_steps && row0 == 0) {
+      constexpr int VEC = S::RB / 16, N = 4;
+      for (int e0 = threadIdx.x; e0 < a.T * VEC; e0 += N * 64 * W) {
+        u32x4 xk[N], xv[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          const int e = min(e0 + u * 64 * W, a.T * VEC - 1);
+          xk[u] = reinterpret_cast<const u32x4*>(kn + e / VEC * a.ks[2])[e % VEC];
+          xv[u] = reinterpret_cast<const u32x4*>(vn + e / VEC * a.vs[2])[e % VEC];
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          const int e = e0 + u * 64 * W;
+          if (e >= a.T * VEC || !(there >> (e / VEC) & 1)) continue;
+          const int64_t row = (base + (int64_t)p * D) / (16 / (int)sizeof(T)) + e;
+          static_cast<u32x4*>(a.kc)[row] = xk[u];
+          static_cast<u32x4*>(a.vc)[row] = xv[u];
+        }
+      }
+    }
+
+    // The waves' states through LDS: weights 2^(m_w - max), then the sums over the waves of a row block in their order, to the
+    // output or to this workgroup's slot.
+    if (QL) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = wave * NT * 16 + n * 16 + q0;
+      const float lt = sum16(l[n]);
       if (g == 0) {
-        red_m[wave][q0] = m[n];
-        red_l[wave][q0] = lt;
+        red_m[row] = m[n];
+        red_l[row] = lt;
       }
       // A lane's elements: 4 VE in a row from g D / 4.
-      if (g * (D / 4) / DP == pass) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < VE; ++j) red[wave][q0][g * (D / 4) % DP + i * VE + j] = o[n][j][i];
+        for (int j = 0; j < VE; j += 4)
+          *reinterpret_cast<f32x4*>(&red[row * (D + 4) + g * (D / 4) + i * VE + j]) =
+              f32x4{o[n][j][i], o[n][j + 1][i], o[n][j + 2][i], o[n][j + 3][i]};
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == at.steps;
+    const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, ROWS);
+    for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * W) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4;  // row r of the row group
+      if (row0 + r >= a.rows) break;
+      float mx = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mx = fmaxf(mx, red_m[r + w * ROWS]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = __builtin_amdgcn_exp2f(red_m[r + w * ROWS] - ref);
+        lsum += red_l[r + w * ROWS] * f;
+        sum += *reinterpret_cast<const f32x4*>(&red[(r + w * ROWS) * (D + 4) + d]) * f;
       }
-      __syncthreads();
-      for (int e = threadIdx.x; e < 16 * (DP / 4); e += 64 * W) {
-        const int row = e / (DP / 4), d = e % (DP / 4) * 4, r = (block * NT + n) * 16 + row;
-        if (r >= a.rows) continue;
-        float mx = -INFINITY, lsum = 0.f;
+      if (whole) {
+        const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
+        T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
+        const bool zero = !(there >> t & 1) || lsum == 0.f;
+        float y[4];
 #pragma unroll
-        for (int w = 0; w < W; ++w) mx = fmaxf(mx, red_m[w][row]);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float f = __builtin_amdgcn_exp2f(red_m[w][row] - ref);
-          lsum += red_l[w][row] * f;
-          sum += *reinterpret_cast<const f32x4*>(&red[w][row][d]) * f;
-        }
-        if (a.part) {
-          const int64_t at = (head * a.chunks + chunk) * a.rows + r;
-          *reinterpret_cast<f32x4*>(parts.acc + at * D + pass * DP + d) = sum;
-          if (pass == 0 && d == 0) parts.ml[at] = f32x2{mx, lsum};
-        } else {
-          const int gh = r / a.T, t = r - gh * a.T;
-          T* out = static_cast<T*>(a.out) + ((b * a.T + t) * a.H + h * a.G + gh) * D + pass * DP + d;
-          const bool zero = !(there >> t & 1) || lsum == 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) out[i] = Elem<T>::from_f32(!valid ? NAN : zero ? 0.f : sum[i] / lsum);
-        }
+        for (int i = 0; i < 4; ++i) y[i] = !valid ? NAN : zero ? 0.f : sum[i] / lsum;
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+        else
+          *reinterpret_cast<f32x4*>(out) = f32x4{y[0], y[1], y[2], y[3]};
+      } else {
+        const int64_t i = (int64_t)slot * ROWS + r;
+        *reinterpret_cast<f32x4*>(parts.acc + i * D + d) = sum;
+        if (d == 0) parts.ml[i] = f32x2{mx, lsum};
       }
     }
+    __syncthreads();
+
+    at.pass(a, s1);
   }
 }
 
-// Four elements of a row per thread: the chunks' weights 2^(m_c - max), then the sums in eight lines of chunks.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int chunk_rows) {
-  constexpr int PER = D / 4, ROWS = 256 / PER, N = 8;
-  const int64_t head = blockIdx.y + (int64_t)blockIdx.z * a.Hkv;
-  const int64_t b = blockIdx.z;
-  const int h = blockIdx.y, r = (int)blockIdx.x * ROWS + threadIdx.x / PER, d = threadIdx.x % PER * 4;
-  if (r >= a.rows) return;
-  const Parts parts = parts_of(a.part, a.items / a.chunks, a.chunks, a.rows);
-  const int p = a.pos[b];
-  const bool valid = p >= 0 && p <= a.L - a.T;
-  const uint64_t there = parts.there[head];
-  const int gh = r / a.T, t = r - gh * a.T;
-  const int full = valid ? min(a.chunks - 1, (p + chunk_rows - 1) / chunk_rows) : 0, used = full + 1;  // the last: the drafts'
-  auto at = [&](int c) { return (head * a.chunks + (c < full ? c : a.chunks - 1)) * a.rows + r; };
-  float mx = -INFINITY;
-  for (int c = 0; c < used; c += N) {
-    float mc[N];
+// Many query rows (bf16): W waves of 32 rows each over the same keys, which go through LDS once for all of them. A stage of KEYS keys
+// and values is copied straight into LDS (three stages, two under way), 16-byte piece c of row r at place c ^ r of its
+// row, so that neither the reads of 32 rows' pieces (keys) nor the transposing ones (values) meet in a bank.
+// S^T = K Q^T and O^T = V^T P^T in 32x32 tiles: a lane has 16 of a tile's 32 scores of one query.
+template <int D>
+struct WideShape {
+  static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
+  static constexpr int STAGE = 2 * KEYS * RB;                     // keys, then values
+  static constexpr int COPIES = STAGE / 16 / (64 * W);            // per thread
+  static constexpr int LDS = std::max(3 * STAGE, ROWS * (D + 4) * 4);
+  static __device__ __forceinline__ int place(int row, int piece) { return row * RB + ((piece ^ row) & (PIECES - 1)) * 16; }
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArgs a) {
+  typedef WideShape<D> C;
+  constexpr int KEYS = C::KEYS, RB = C::RB, W = C::W, ROWS = C::ROWS, NT = KEYS / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float* const red = reinterpret_cast<float*>(lds);  // [ROWS][D + 4]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, q0 = lane & 31;
+  Cursor<KEYS> at;
+  if (!at.start(a, lane)) return;
+  for (int slot = 2 * (int)blockIdx.x; at.cur < at.end; slot = 2 * (int)blockIdx.x + 1) {
+    const int b = at.b, p = at.p, s0 = at.s0, s1 = min(at.steps, s0 + at.end - at.cur);
+    const int h = at.hr / a.row_groups, row0 = (at.hr % a.row_groups) * ROWS;
+    const bool valid = in_cache(a, p);
+    const int cached = valid ? p : 0, cached_steps = (cached + KEYS - 1) / KEYS, whole_to = cached / KEYS;
+    const int to = valid ? s1 : s0;
+    const int64_t base = ((int64_t)b * a.Hkv + h) * a.L * D;
+    const bf16* kn = static_cast<const bf16*>(a.kn) + b * a.ks[0] + h * a.ks[1];
+    const bf16* vn = static_cast<const bf16*>(a.vn) + b * a.vs[0] + h * a.vs[1];
+    const uint32_t kbytes = (uint32_t)a.ks[2] * 2, vbytes = (uint32_t)a.vs[2] * 2;
+    const bool mine = row0 + wave * 32 < a.rows;  // whether this wave has rows; it copies in any case
+
+    // Step `s` into its stage; one past the last from past every range, so that the copies under way can be counted.
+    auto copy = [&](int s) {
+      const bool old = s < cached_steps;
+      const int from = (s - (old ? 0 : cached_steps)) * KEYS;
+      char* const stage = lds + (s - s0) % 3 * C::STAGE;
 #pragma unroll
-    for (int u = 0; u < N; ++u) mc[u] = parts.ml[at(min(c + u, used - 1))][0];
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t step = old ? RB : half ? vbytes : kbytes;
+        const bf16* src = old ? static_cast<const bf16*>(half ? a.vc : a.kc) + base : half ? vn : kn;
+        const u32x4 rsrc = buffer_rsrc(src, old ? (uint32_t)cached * RB : (a.T - 1) * step + RB);
 #pragma unroll
-    for (int u = 0; u < N; ++u) mx = fmaxf(mx, mc[u]);
+        for (int u = 0; u < C::COPIES / 2; ++u) {
+          const int piece = u * 64 * W + wave * 64 + lane, row = piece / C::PIECES;
+          const uint32_t off = (uint32_t)(from + row) * step + ((piece ^ row) & (C::PIECES - 1)) * 16;
+          dma16(rsrc, stage + half * KEYS * RB + (u * 64 * W + wave * 64) * 16, s < to ? off : kMostBytes);
+        }
+      }
+    };
+    const int parent = a.parents[(int64_t)b * a.T + min(lane, a.T - 1)];
+    // Query rows, as B operands: row r is node r % T of head h G + r / T; in place of rows past the last it is read again.
+    bf16x8 q[D / 16];
+    const int r = min(row0 + wave * 32 + q0, a.rows - 1), gh = r / a.T, node = r - gh * a.T;
+    {
+      const char* src = reinterpret_cast<const char*>(static_cast<const bf16*>(a.q) + b * a.qs[0] + (h * a.G + gh) * a.qs[1] + node * a.qs[2]);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+        q[c] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + c * 32 + g * 16) ^ a.flip);
+    }
+    uint64_t there = 0, line = 0;
+    const bool drafts = valid && s1 > cached_steps;
+    if (drafts) {
+      line = ancestors(lane < a.T ? parent : -2, lane);
+      there = __ballot(line != 0);
+      line = __shfl((unsigned long long)line, node, kWave);
+    }
+    // The nodes' rows of the cache, by the workgroup that has the first step of nodes of the head's first rows.
+    if (drafts && s0 <= cached_steps && row0 == 0) {
+      for (int e = threadIdx.x; e < a.T * C::PIECES; e += 64 * W) {
+        const int t = e / C::PIECES, c = e % C::PIECES;
+        if (!(there >> t & 1)) continue;
+        const int64_t row = (base + (int64_t)p * D) / 8 + e;
+        static_cast<u32x4*>(a.kc)[row] = reinterpret_cast<const u32x4*>(kn + t * a.ks[2])[c];
+        static_cast<u32x4*>(a.vc)[row] = reinterpret_cast<const u32x4*>(vn + t * a.vs[2])[c];
+      }
+    }
+    wait_vmem<0>();  // from here on the copies alone are counted
+    copy(s0);
+    copy(s0 + 1);
+
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+
+    for (int s = s0; s < to; ++s) {
+      wait_vmem<C::COPIES>();
+      lds_barrier();  // this step's stage is there for all, and the one before is read
+      copy(s + 2);
+      char* const ks = lds + (s - s0) % 3 * C::STAGE;
+      char* const vs = ks + KEYS * RB;
+      const bool special = s >= whole_to, old = s < cached_steps;
+      const int first = old ? 0 : (s - cached_steps) * KEYS;  // first node
+      if (!old) {  // values of absent nodes, whatever they hold, as zeros: their weight is 0
+        for (int e = threadIdx.x; e < KEYS * C::PIECES; e += 64 * W) {
+          const int k = first + e / C::PIECES;
+          if (k >= kMaxNodes || !(there >> (k & 63) & 1)) *reinterpret_cast<u32x4*>(vs + e * 16) = u32x4{0, 0, 0, 0};
+        }
+        lds_barrier();
+      }
+      if (!mine) continue;
+      f32x16 x[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+          mma32(*reinterpret_cast<const bf16x8*>(ks + C::place(32 * t + q0, 2 * c + g)), q[c], x[t]);
+      }
+      if (special) {
+        const uint64_t sees = (old ? (1ull << (cached - s * KEYS)) - 1 : line >> first) >> (4 * g);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[t][i] = sees >> (32 * t + 8 * (i / 4) + i % 4) & 1 ? x[t][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
+      mx = fmaxf(m, lane32_max(mx) * a.c);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      if (__any(mx > m)) {
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[j][i] *= f;
+      }
+      m = mx;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], a.c, -ref));
+          l += x[t][i];
+        }
+      // 16 keys at a time: a lane's weights are of keys 4 g .. and 8 + 4 g .., and so are its values.
+#pragma unroll
+      for (int c = 0; c < KEYS / 16; ++c) {
+        const f32x16& w = x[c / 2];
+        const int e = c % 2 * 8;
+        const u32x4 pb = {pack_bf16(w[e], w[e + 1]), pack_bf16(w[e + 2], w[e + 3]), pack_bf16(w[e + 4], w[e + 5]),
+                          pack_bf16(w[e + 6], w[e + 7])};
+        const int row = 16 * c + 4 * g + (lane & 15) / 4;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const int piece = 4 * j + (lane >> 4 & 1) * 2 + (lane & 3) / 2, in = (lane & 1) * 8;
+          const char* lo = vs + C::place(row, piece) + in;
+          const char* hi = vs + C::place(row + 8, piece) + in;
+          mma32(tr_frag(lo, (int)(hi - lo)), __builtin_bit_cast(bf16x8, pb), o[j]);
+        }
+      }
+    }
+
+    // O through LDS, rows whole, to the output or to this workgroup's slot.
+    wait_vmem<0>();
+    lds_barrier();
+    {
+      const float lt = lane32_sum(l);
+      const int row = wave * 32 + q0;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<f32x4*>(&red[row * (D + 4) + 32 * j + 2 * i + 4 * g]) = f32x4{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
+      if (g == 0) *reinterpret_cast<f32x2*>(&red[row * (D + 4) + D]) = f32x2{m, lt};
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == at.steps;
+    const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, ROWS);
+    for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * W) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4;  // row r of the row group
+      if (row0 + r >= a.rows) break;
+      const f32x4 sum = *reinterpret_cast<const f32x4*>(&red[r * (D + 4) + d]);
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(&red[r * (D + 4) + D]);
+      if (whole) {
+        const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
+        bf16* out = static_cast<bf16*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
+        const bool zero = !(there >> t & 1) || ml[1] == 0.f;
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = !valid ? NAN : zero ? 0.f : sum[i] / ml[1];
+        *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+      } else {
+        const int64_t i = (int64_t)slot * ROWS + r;
+        *reinterpret_cast<f32x4*>(parts.acc + i * D + d) = sum;
+        if (d == 0) parts.ml[i] = ml;
+      }
+    }
+    wait_vmem<0>();
+    __syncthreads();
+    at.pass(a, s1);
   }
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float ls[N] = {};
-  f32x4 as[N] = {};
-  for (int c = 0; c < used; c += N) {
+}
+
+// Joins what several workgroups have of a row: its pieces are dealt to LINES threads for every four elements, each adding
+// up eight at a time under a running maximum; then the lines in their order.
+template <typename T, int D, int KEYS>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_rows) {
+  constexpr int PER = D / 4, LINES = 4, ROWS = 256 / PER / LINES, N = 8;
+  __shared__ __attribute__((aligned(16))) float red[LINES][ROWS][D + 4];  // D sums, m, l
+  const int b = blockIdx.z, h = blockIdx.y, block = (int)blockIdx.x * ROWS, lane = threadIdx.x & 63, per_seq = a.Hkv * a.row_groups;
+  const int d = threadIdx.x % PER * 4, row = threadIdx.x / PER % ROWS, part = threadIdx.x / PER / ROWS, r = block + row;
+  const int p = pos_of(a, b), parent = lane < a.T ? a.parents[(int64_t)b * a.T + lane] : -2;
+  int sum = 0, before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int mine = steps_at<KEYS>(a, b0 + lane, pos_of(a, b0 + lane));
+    sum += mine;
+    before += b0 + lane < b ? mine : 0;
+  }
+  const int share = share_of(a, wave_total(sum) * per_seq), steps = steps_at<KEYS>(a, b, p);
+  const int x0 = wave_total(before) * per_seq + (h * a.row_groups + block / slot_rows) * steps;
+  const int w0 = x0 / share, used = (x0 + steps - 1) / share - w0 + 1;
+  if (used == 1) return;  // one workgroup had it all
+  const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, slot_rows);
+  auto at = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 && x0 != w0 * share)) * slot_rows + r % slot_rows; };
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c = part; c < used; c += N * LINES) {
     f32x2 ml[N];
-    f32x4 acc[N];
+    f32x4 x[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int64_t i = at(min(c + u, used - 1));
+      const int64_t i = at(min(c + u * LINES, used - 1));
       ml[u] = parts.ml[i];
-      acc[u] = *reinterpret_cast<const f32x4*>(parts.acc + i * D + d);
+      x[u] = *reinterpret_cast<const f32x4*>(parts.acc + i * D + d);
     }
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) mx = fmaxf(mx, ml[u][0]);
+    const float ref = mx == -INFINITY ? 0.f : mx, f = __builtin_amdgcn_exp2f(m - ref);
+    l *= f;
+    acc *= f;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      if (c + u >= used) continue;
-      const float f = __builtin_amdgcn_exp2f(ml[u][0] - ref);
-      ls[u] += ml[u][1] * f;
-      as[u] += acc[u] * f;
+      if (c + u * LINES >= used) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[u][0] - ref);
+      l += ml[u][1] * w;
+      acc += x[u] * w;
     }
+    m = mx;
   }
+  *reinterpret_cast<f32x4*>(&red[part][row][d]) = acc;
+  if (d == 0) {
+    red[part][row][D] = m;
+    red[part][row][D + 1] = l;
+  }
+  const uint64_t there = __ballot(ancestors(parent, lane) != 0);  // split: the sequence has its place
+  __syncthreads();
+  if (part != 0 || r >= a.rows) return;
+  float mx = -INFINITY, lsum = 0.f;
 #pragma unroll
-  for (int n = N / 2; n > 0; n /= 2)
+  for (int u = 0; u < LINES; ++u) mx = fmaxf(mx, red[u][row][D]);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  f32x4 total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < n; ++u) {
-      ls[u] += ls[u + n];
-      as[u] += as[u + n];
-    }
-  T* out = static_cast<T*>(a.out) + ((b * a.T + t) * a.H + h * a.G + gh) * D + d;
-  const bool zero = !(there >> t & 1) || ls[0] == 0.f;
+  for (int u = 0; u < LINES; ++u) {
+    const float w = __builtin_amdgcn_exp2f(red[u][row][D] - ref);
+    lsum += red[u][row][D + 1] * w;
+    total += *reinterpret_cast<const f32x4*>(&red[u][row][d]) * w;
+  }
+  const int gh = r / a.T, t = r - gh * a.T;
+  T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
+  const bool zero = !(there >> t & 1) || lsum == 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = Elem<T>::from_f32(!valid ? NAN : zero ? 0.f : as[0][i] / ls[0]);
+  for (int i = 0; i < 4; ++i) out[i] = Elem<T>::from_f32(zero ? 0.f : total[i] / lsum);
 }
 
-constexpr int64_t kGridTarget = 1024;
-constexpr int64_t kMostBlocks = 0xffffffff / 512;  // blocks of up to 512 threads: a launch has under 2^32 threads along x
+constexpr int64_t kMostSteps = 1 << 30;
 
 struct Plan {
-  int tiles;       // row tiles of 16 a wave
-  int waves;
-  int64_t row_blocks, chunks, wave_rows;
+  bool wide;
+  int tiles, waves;  // of tree_attn_kernel
+  int64_t keys, slot_rows, row_groups, groups, least;
+  bool split;
 };
+
 Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d, int dtype) {
-  const int64_t rows = h / hkv * t, keys = dtype == FERRITE_BF16 ? 32 : 16;
+  const bool half = dtype == FERRITE_BF16;
+  const int64_t rows = h / hkv * t;
   Plan p;
+  p.wide = half && rows > (d == 256 ? 32 : 64);
   p.tiles = rows <= 16 ? 1 : rows <= 32 || d > 128 ? 2 : 4;
-  p.row_blocks = cdiv(rows, 16 * p.tiles);
-  if (max_len <= 8 * 2 * keys) {
-    p.waves = 8;
-    p.chunks = 1;
-    p.wave_rows = cdiv(cdiv(max_len, 8), keys) * keys;
-    return p;
-  }
   p.waves = 4;
-  int64_t rows_of_chunk = 4 * keys;
-  while (rows_of_chunk < max_len && b * hkv * p.row_blocks * cdiv(max_len, rows_of_chunk) > kGridTarget) rows_of_chunk *= 2;
-  p.chunks = cdiv(max_len, rows_of_chunk);
-  p.wave_rows = rows_of_chunk / 4;
+  p.keys = p.wide ? (d == 256 ? 32 : 64) : half ? 32 : 16;
+  p.slot_rows = p.wide ? (d == 256 ? 128 : 256) : 16 * p.tiles;
+  p.row_groups = cdiv(rows, p.slot_rows);
+  const int64_t heads = b * hkv * p.row_groups, steps = cdiv(max_len, p.keys) + cdiv(t, p.keys);
+  // Workgroups that are resident together.
+  const int per_cu = p.wide ? 1 : p.tiles == 1 ? (d == 64 ? 3 : d == 128 ? 2 : 1) : p.tiles == 2 && d == 64 ? 2 : 1;
+  p.groups = 256 * per_cu;
+  p.least = p.wide ? 4 : (half || p.tiles == 1 ? 2 : 1) * p.waves;
+  p.split = heads < 4 * p.groups && steps > (p.wide ? 8 : 32);
+  if (!p.split) {
+    p.groups = heads;
+    if (!p.wide && p.tiles == 1 && d <= 128 && steps > 8) p.waves = 8;
+  } else {
+    p.groups = std::min(p.groups, cdiv(heads * steps, p.least));
+  }
   return p;
 }
 
-template <typename T, int D, int NT>
-int tree_launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  const int64_t blocks = cdiv(a.items, 8) * 8 * p.row_blocks;
-  if (blocks > kMostBlocks) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: too many heads");
-  if (p.waves == 8)
-    hipLaunchKernelGGL((tree_attn_kernel<T, D, NT, 8>), dim3((unsigned)blocks), dim3(512), 0, s, a);
-  else
-    hipLaunchKernelGGL((tree_attn_kernel<T, D, NT, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  if (p.chunks > 1) {
-    const int rc = check_launch("ferrite_tree_attention");
-    if (rc != FERRITE_OK) return rc;
-    const int64_t B = a.items / p.chunks / a.Hkv;
-    hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3((unsigned)cdiv(a.rows, 1024 / D), (unsigned)a.Hkv, (unsigned)B), dim3(256),
-                       0, s, a, (int)(4 * p.wave_rows));
-  }
+template <typename T, int D, int KEYS>
+int tree_finish(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  const int rc = check_launch("ferrite_tree_attention");
+  if (rc != FERRITE_OK || !p.split) return rc;
+  hipLaunchKernelGGL((tree_join_kernel<T, D, KEYS>), dim3((unsigned)cdiv(a.rows, 256 / D), (unsigned)a.Hkv, (unsigned)a.B), dim3(256),
+                     0, s, a, (int)p.slot_rows);
   return check_launch("ferrite_tree_attention");
+}
+
+template <typename T, int D, int NT, int W>
+int tree_launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  constexpr int bytes = kTreeLds<T, D, NT, W>;
+  if (bytes > (64 << 10)) {
+    const int rc = allow_lds(reinterpret_cast<const void*>(&tree_attn_kernel<T, D, NT, W>), bytes, s, "ferrite_tree_attention");
+    if (rc != FERRITE_OK) return rc;
+  }
+  hipLaunchKernelGGL((tree_attn_kernel<T, D, NT, W>), dim3((unsigned)p.groups), dim3(64 * W), bytes, s, a);
+  return tree_finish<T, D, Step<T, D>::KEYS>(a, p, s);
+}
+
+template <int D>
+int tree_wide_launch(const TreeArgs& a, const Plan& p, hipStream_t s) {
+  typedef WideShape<D> C;
+  const int rc = allow_lds(reinterpret_cast<const void*>(&tree_wide_kernel<D>), C::LDS, s, "ferrite_tree_attention");
+  if (rc != FERRITE_OK) return rc;
+  hipLaunchKernelGGL(tree_wide_kernel<D>, dim3((unsigned)p.groups), dim3(64 * C::W), C::LDS, s, a);
+  return tree_finish<bf16, D, C::KEYS>(a, p, s);
 }
 
 int check_tree(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d, int dtype) {
@@ -497,8 +885,13 @@ int check_tree(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, in
   if (b < 0 || hkv < 1 || b > 65535 || hkv > 65535 || h < hkv || h > 65535 || h % hkv)
     return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": need 0 <= b <= 65535 and up to 65535 query heads, a multiple of the key heads");
   if (t < 1 || t > kMaxNodes) return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": need 1 to 64 nodes");
-  if (max_len < 1 || max_len > 0x7fffffff / 512) return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": need 1 <= max_len < 2^22");
   if (d != 64 && d != 128 && d != 256) return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": head dim must be 64, 128 or 256");
+  if (max_len < 1 || max_len > kMostBytes / (d * (dtype == FERRITE_BF16 ? 2 : 4)))
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": need max_len >= 1, and a head's cache within 4 GiB less 128 KiB");
+  // Places on the line of steps are 32-bit numbers.
+  const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
+  if (b * hkv * p.row_groups > kMostSteps / 512 || b * hkv * p.row_groups * (cdiv(max_len, 16) + 4) > kMostSteps)
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": too many heads for caches of this length");
   return FERRITE_OK;
 }
 
@@ -510,7 +903,7 @@ extern "C" int64_t ferrite_internal_tree_attention_workspace(int64_t b, int64_t 
   using namespace ferrite;
   if (check_tree(b, h, hkv, t, max_len, d, dtype) != FERRITE_OK) return -1;
   const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
-  return p.chunks > 1 ? parts_bytes(b * hkv, p.chunks, h / hkv * t, d) : 0;
+  return p.split ? parts_bytes(2 * p.groups, p.slot_rows, d) : 0;
 }
 
 extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new, const void* v_new, void* k_cache,
@@ -528,28 +921,36 @@ extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new,
   bool aligned = a16(q) && a16(k_new) && a16(v_new) && a16(k_cache) && a16(v_cache) && a16(out);
   for (int i = 0; i < 9; ++i) aligned = aligned && strides[i] % (dtype == FERRITE_BF16 ? 8 : 4) == 0;
   if (!aligned) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: tensors and strides must be 16-byte aligned");
+  for (int i = 5; i < 9; i += 3)
+    if (strides[i] < 0 || (t - 1) * strides[i] * (dtype == FERRITE_BF16 ? 2 : 4) > (int64_t)kMostBytes - 1024)
+      return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: a head's new keys or values span 4 GiB");
   const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
-  TreeArgs a{q, k_new, v_new, k_cache, v_cache, pos, parents, out, nullptr, {}, {}, {}, b * hkv * p.chunks, (int)h, (int)hkv,
-             (int)(h / hkv), (int)t, (int)max_len, (int)(h / hkv * t), (int)p.chunks, (int)p.row_blocks, (int)p.wave_rows,
-             scale * kLog2e};
+  TreeArgs a{q, k_new, v_new, k_cache, v_cache, pos, parents, out, nullptr, {}, {}, {}, (int)b, (int)h, (int)hkv, (int)(h / hkv),
+             (int)t, (int)max_len, (int)(h / hkv * t), (int)p.row_groups, (int)p.groups, (int)p.least,
+             std::max(fabsf(scale) * kLog2e, 1e-37f),  // above 0, so that it times -inf is -inf
+             scale >= 0 ? 0u : dtype == FERRITE_BF16 ? 0x80008000u : 0x80000000u};
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = strides[i];
     a.ks[i] = strides[3 + i];
     a.vs[i] = strides[6 + i];
   }
-  if (p.chunks > 1) {
-    if (!workspace || !a16(workspace) || workspace_bytes < parts_bytes(b * hkv, p.chunks, a.rows, d))
+  if (p.split) {
+    if (!workspace || !a16(workspace) || workspace_bytes < parts_bytes(2 * p.groups, p.slot_rows, d))
       return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: workspace too small or unaligned");
     a.part = static_cast<char*>(workspace);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto tiles = [&](auto* e, auto D) {
     typedef std::remove_pointer_t<decltype(e)> T;
-    if (p.tiles == 1) return tree_launch<T, D.value, 1>(a, p, s);
-    if constexpr (D.value <= 128) {
-      if (p.tiles == 4) return tree_launch<T, D.value, 4>(a, p, s);
+    if constexpr (sizeof(T) == 2) {
+      if (p.wide) return tree_wide_launch<D.value>(a, p, s);
     }
-    return tree_launch<T, D.value, 2>(a, p, s);
+    if constexpr (D.value <= 128) {
+      if (p.waves == 8) return tree_launch<T, D.value, 1, 8>(a, p, s);
+      if (p.tiles == 4) return tree_launch<T, D.value, 4, 4>(a, p, s);
+    }
+    if (p.tiles == 1) return tree_launch<T, D.value, 1, 4>(a, p, s);
+    return tree_launch<T, D.value, 2, 4>(a, p, s);
   };
   auto dims = [&](auto* e) {
     if (d == 64) return tiles(e, std::integral_constant<int, 64>{});

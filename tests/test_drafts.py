@@ -244,7 +244,7 @@ def test_tree_abi_refusals():
 
     assert call(b=0) == 0
     for change, words in ((dict(dtype=3), "dtype"), (dict(b=-1), "65535"), (dict(h=3), "multiple"), (dict(hkv=0), "multiple"),
-                          (dict(t=0), "nodes"), (dict(t=65), "nodes"), (dict(n=0), "max_len"), (dict(n=1 << 22), "max_len"),
+                          (dict(t=0), "nodes"), (dict(t=65), "nodes"), (dict(n=0), "max_len"), (dict(n=1 << 25), "max_len"),
                           (dict(d=80), "head dim"), (dict(q=None), "null"), (dict(q=a + 8), "aligned"), (dict(), "workspace"),
                           (dict(st=(ctypes.c_int64 * 9)(*[68] * 9)), "aligned"),
                           (dict(b=65535, h=65535, hkv=65535, t=1, n=64), "too many heads")):
