@@ -540,16 +540,22 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 }
 
 // Many query rows (bf16): W waves of 32 rows each over the same keys, which go through LDS once for all of them. A stage of KEYS keys
-// and values is copied straight into LDS (three stages, two under way), 16-byte piece c of row r at place c ^ r of its
-// row, so that neither the reads of 32 rows' pieces (keys) nor the transposing ones (values) meet in a bank.
+// and values is copied straight into LDS (four stages, up to three under way), 16-byte pieces of a row
+// in an order of its own, so that neither the reads of 32 rows' pieces (keys) nor the transposing ones (values) meet in a bank.
 // S^T = K Q^T and O^T = V^T P^T in 32x32 tiles: a lane has 16 of a tile's 32 scores of one query.
+//
+// A step is two clusters, the softmax of its scores (VALU) and its product with V and the next step's with K (matrix units), each
+// behind a barrier, and the second half of the waves is one cluster behind the first: of a SIMD's two waves one is on the
+// VALU while the other is on the matrix units.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
   static constexpr int STAGE = 2 * KEYS * RB;                     // keys, then values
   static constexpr int COPIES = STAGE / 16 / (64 * W);            // per thread
-  static constexpr int LDS = std::max(3 * STAGE, ROWS * (D + 4) * 4);
-  static __device__ __forceinline__ int place(int row, int piece) { return row * RB + ((piece ^ row) & (PIECES - 1)) * 16; }
+  static constexpr int LDS = std::max(4 * STAGE, ROWS * (D + 4) * 4);
+  // Where in its row a piece lies, and which piece lies there.
+  static __device__ __forceinline__ int swapped(int row, int piece) { return (piece ^ ((row & 3) << 2 | (row >> 2 & 3))) & (PIECES - 1); }
+  static __device__ __forceinline__ int place(int row, int piece) { return row * RB + swapped(row, piece) * 16; }
 };
 
 template <int D>
@@ -573,24 +579,6 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
     const uint32_t kbytes = (uint32_t)a.ks[2] * 2, vbytes = (uint32_t)a.vs[2] * 2;
     const bool mine = row0 + wave * 32 < a.rows;  // whether this wave has rows; it copies in any case
 
-    // Step `s` into its stage; one past the last from past every range, so that the copies under way can be counted.
-    auto copy = [&](int s) {
-      const bool old = s < cached_steps;
-      const int from = (s - (old ? 0 : cached_steps)) * KEYS;
-      char* const stage = lds + (s - s0) % 3 * C::STAGE;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t step = old ? RB : half ? vbytes : kbytes;
-        const bf16* src = old ? static_cast<const bf16*>(half ? a.vc : a.kc) + base : half ? vn : kn;
-        const u32x4 rsrc = buffer_rsrc(src, old ? (uint32_t)cached * RB : (a.T - 1) * step + RB);
-#pragma unroll
-        for (int u = 0; u < C::COPIES / 2; ++u) {
-          const int piece = u * 64 * W + wave * 64 + lane, row = piece / C::PIECES;
-          const uint32_t off = (uint32_t)(from + row) * step + ((piece ^ row) & (C::PIECES - 1)) * 16;
-          dma16(rsrc, stage + half * KEYS * RB + (u * 64 * W + wave * 64) * 16, s < to ? off : kMostBytes);
-        }
-      }
-    };
     const int parent = a.parents[(int64_t)b * a.T + min(lane, a.T - 1)];
     // Query rows, as B operands: row r is node r % T of head h G + r / T; in place of rows past the last it is read again.
     bf16x8 q[D / 16];
@@ -618,89 +606,149 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         static_cast<u32x4*>(a.vc)[row] = reinterpret_cast<const u32x4*>(vn + t * a.vs[2])[c];
       }
     }
+    // Step `s` into its stage; one past the last from past every range, so that the copies under way can be counted.
+    auto copy = [&](int s) {
+      const bool old = s < cached_steps;
+      const int from = (s - (old ? 0 : cached_steps)) * KEYS;
+      char* const stage = lds + (s - s0) % 4 * C::STAGE;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t step = old ? RB : half ? vbytes : kbytes;
+        const bf16* src = old ? static_cast<const bf16*>(half ? a.vc : a.kc) + base : half ? vn : kn;
+        const u32x4 rsrc = buffer_rsrc(src, old ? (uint32_t)cached * RB : (a.T - 1) * step + RB);
+#pragma unroll
+        for (int u = 0; u < C::COPIES / 2; ++u) {
+          const int piece = (u * W + wave) * 64 + lane, row = piece / C::PIECES;
+          const uint32_t off = (uint32_t)(from + row) * step + C::swapped(row, piece) * 16;
+          // Absent nodes, whatever they hold, are zeros: their weight is 0.
+          const bool on = s < to && (old || (from + row < kMaxNodes && (there >> ((from + row) & 63) & 1)));
+          dma16(rsrc, stage + half * KEYS * RB + (u * W + wave) * 1024, on ? off : kMostBytes);
+        }
+      }
+    };
+    const bool leads = wave < W / 2;
     wait_vmem<0>();  // from here on the copies alone are counted
     copy(s0);
     copy(s0 + 1);
+    copy(s0 + 2);
+
+    // A lane's places in a stage: of its key row's pieces; of its values, which of 16 keys lie in rows 4 g .. and 8 + 4 g .. (a row's
+    // order of pieces is the same 16 rows on).
+    int koff[D / 16], voff[D / 32][2];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) koff[c] = C::place(q0, 2 * c + g);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi)
+        voff[j][hi] = KEYS * RB + C::place(8 * hi + 4 * g + (lane & 15) / 4, 4 * j + (lane >> 4 & 1) * 2 + (lane & 3) / 2) + (lane & 1) * 8;
 
     float m = -INFINITY, l = 0.f;
-    f32x16 o[D / 32];
+    f32x16 o[D / 32], x[NT];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
 
-    for (int s = s0; s < to; ++s) {
-      wait_vmem<C::COPIES>();
-      lds_barrier();  // this step's stage is there for all, and the one before is read
-      copy(s + 2);
-      char* const ks = lds + (s - s0) % 3 * C::STAGE;
-      char* const vs = ks + KEYS * RB;
-      const bool special = s >= whole_to, old = s < cached_steps;
-      const int first = old ? 0 : (s - cached_steps) * KEYS;  // first node
-      if (!old) {  // values of absent nodes, whatever they hold, as zeros: their weight is 0
-        for (int e = threadIdx.x; e < KEYS * C::PIECES; e += 64 * W) {
-          const int k = first + e / C::PIECES;
-          if (k >= kMaxNodes || !(there >> (k & 63) & 1)) *reinterpret_cast<u32x4*>(vs + e * 16) = u32x4{0, 0, 0, 0};
-        }
-        lds_barrier();
-      }
-      if (!mine) continue;
-      f32x16 x[NT];
+    auto scores = [&](int s) {
+      const char* ks = lds + (s - s0) % 4 * C::STAGE;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-          mma32(*reinterpret_cast<const bf16x8*>(ks + C::place(32 * t + q0, 2 * c + g)), q[c], x[t]);
-      }
-      if (special) {
-        const uint64_t sees = (old ? (1ull << (cached - s * KEYS)) - 1 : line >> first) >> (4 * g);
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma32(*reinterpret_cast<const bf16x8*>(ks + koff[c] + t * 32 * RB), q[c], x[t]);
+    };
+    // A wave copies step s + 3 when it begins the product of step s with V: all waves have left that of s - 1, whose stage it
+    // takes. Before the barrier at which the leading waves begin that product, every wave has waited for its copies of step
+    // s + 1: they when they leave the softmax of s, the others when they leave the product of s - 1.
+    wait_vmem<2 * C::COPIES>();
+    lds_barrier();
+    if (mine && s0 < to) scores(s0);
+    if (!leads) lds_barrier();
+    for (int s = s0; s < to; ++s) {
+      if (!leads) wait_vmem<C::COPIES>();
+      lds_barrier();
+      u32x4 pb[KEYS / 16];
+      if (mine) {
+        if (s >= whole_to) {  // not every row sees every key: bit k of `sees` is the step's key k
+          const bool old = s < cached_steps;
+          const uint64_t sees = (old ? (1ull << (cached - s * KEYS)) - 1 : line >> (s - cached_steps) * KEYS) >> (4 * g);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[t][i] = sees >> (32 * t + 8 * (i / 4) + i % 4) & 1 ? x[t][i] : -INFINITY;
+        }
+        float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[t][i] = sees >> (32 * t + 8 * (i / 4) + i % 4) & 1 ? x[t][i] : -INFINITY;
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
+        mx = fmaxf(m, lane32_max(mx) * a.c);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx > m)) {
+          const float f = __builtin_amdgcn_exp2f(m - ref);
+          l *= f;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[j][i] *= f;
+        }
+        m = mx;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], a.c, -ref));
+            l += x[t][i];
+          }
+        // 16 keys to an operand: a lane's weights are of keys 4 g .. and 8 + 4 g .., and so are its values.
+#pragma unroll
+        for (int c = 0; c < KEYS / 16; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pb[c][e] = pack_bf16(x[c / 2][c % 2 * 8 + 2 * e], x[c / 2][c % 2 * 8 + 2 * e + 1]);
       }
-      float mx = -INFINITY;
+      if (leads) wait_vmem<C::COPIES>();
+      lds_barrier();
+      copy(s + 3);
+      if (!mine) continue;
+      // The scores of the next step (behind the last one of zeros, for nothing), then O: reads from LDS are kept AHEAD products
+      // ahead of the one that they feed, in this order (a read's latency is some six products; left to itself the compiler has
+      // every product wait for its own read).
+      const char *ks = lds + (s + 1 - s0) % 4 * C::STAGE, *vs = lds + (s - s0) % 4 * C::STAGE;
+      constexpr int QK = NT * D / 16, ALL = QK + KEYS / 16 * D / 32, AHEAD = 8;
+      auto fetch = [&](int i) {
+        if (i < QK) return *reinterpret_cast<const bf16x8*>(ks + koff[i / NT] + i % NT * 32 * RB);
+        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+        const int c = (i - QK) / (D / 32), j = (i - QK) % (D / 32);
+        auto half = [&](int hi) {
+          return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              reinterpret_cast<lds_i16x4*>(reinterpret_cast<uintptr_t>(vs + voff[j][hi] + c * 16 * RB)));
+        };
+        const i16x4 lo = half(0), hi = half(1);
+        typedef short i16x8 __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(bf16x8, i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+      };
+      bf16x8 ring[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) ring[i] = fetch(i);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[t][i]);
-      mx = fmaxf(m, lane32_max(mx) * a.c);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      if (__any(mx > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - ref);
-        l *= f;
+        for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[j][i] *= f;
-      }
-      m = mx;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], a.c, -ref));
-          l += x[t][i];
-        }
-      // 16 keys at a time: a lane's weights are of keys 4 g .. and 8 + 4 g .., and so are its values.
-#pragma unroll
-      for (int c = 0; c < KEYS / 16; ++c) {
-        const f32x16& w = x[c / 2];
-        const int e = c % 2 * 8;
-        const u32x4 pb = {pack_bf16(w[e], w[e + 1]), pack_bf16(w[e + 2], w[e + 3]), pack_bf16(w[e + 4], w[e + 5]),
-                          pack_bf16(w[e + 6], w[e + 7])};
-        const int row = 16 * c + 4 * g + (lane & 15) / 4;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const int piece = 4 * j + (lane >> 4 & 1) * 2 + (lane & 3) / 2, in = (lane & 1) * 8;
-          const char* lo = vs + C::place(row, piece) + in;
-          const char* hi = vs + C::place(row + 8, piece) + in;
-          mma32(tr_frag(lo, (int)(hi - lo)), __builtin_bit_cast(bf16x8, pb), o[j]);
-        }
+      for (int i = 0; i < ALL; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < QK)
+          mma32(ring[i % AHEAD], q[i / NT], x[i % NT]);
+        else
+          mma32(ring[i % AHEAD], __builtin_bit_cast(bf16x8, pb[(i - QK) / (D / 32)]), o[(i - QK) % (D / 32)]);
+        if (i + AHEAD < ALL) ring[i % AHEAD] = fetch(i + AHEAD);
       }
     }
+    if (leads) lds_barrier();
 
     // O through LDS, rows whole, to the output or to this workgroup's slot.
     wait_vmem<0>();
@@ -737,20 +785,22 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         if (d == 0) parts.ml[i] = ml;
       }
     }
-    wait_vmem<0>();
     __syncthreads();
     at.pass(a, s1);
   }
 }
 
-// Joins what several workgroups have of a row: its pieces are dealt to LINES threads for every four elements, each adding
-// up eight at a time under a running maximum; then the lines in their order.
-template <typename T, int D, int KEYS>
+// Joins what several workgroups have of a row. The pieces of a row are dealt to LINES threads for every four elements, each adding
+// up N at a time under a running maximum; then the lines in their order. A workgroup takes kJoinRows rows, of one row group.
+template <int D, int LINES>
+constexpr int kJoinRows = LINES == 1 ? 16 : 1024 / D / LINES;
+template <typename T, int D, int KEYS, int LINES, int N>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_rows) {
-  constexpr int PER = D / 4, LINES = 4, ROWS = 256 / PER / LINES, N = 8;
+  constexpr int PER = D / 4, ROWS = 256 / PER / LINES;
   __shared__ __attribute__((aligned(16))) float red[LINES][ROWS][D + 4];  // D sums, m, l
-  const int b = blockIdx.z, h = blockIdx.y, block = (int)blockIdx.x * ROWS, lane = threadIdx.x & 63, per_seq = a.Hkv * a.row_groups;
-  const int d = threadIdx.x % PER * 4, row = threadIdx.x / PER % ROWS, part = threadIdx.x / PER / ROWS, r = block + row;
+  const int b = blockIdx.z, h = blockIdx.y, block = (int)blockIdx.x * kJoinRows<D, LINES>, lane = threadIdx.x & 63;
+  const int per_seq = a.Hkv * a.row_groups;
+  const int d = threadIdx.x % PER * 4, row = threadIdx.x / PER % ROWS, part = threadIdx.x / PER / ROWS;
   const int p = pos_of(a, b), parent = lane < a.T ? a.parents[(int64_t)b * a.T + lane] : -2;
   int sum = 0, before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -762,58 +812,67 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
   const int x0 = wave_total(before) * per_seq + (h * a.row_groups + block / slot_rows) * steps;
   const int w0 = x0 / share, used = (x0 + steps - 1) / share - w0 + 1;
   if (used == 1) return;  // one workgroup had it all
+  const uint64_t there = __ballot(ancestors(parent, lane) != 0);  // divided: the sequence has its place
   const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, slot_rows);
-  auto at = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 && x0 != w0 * share)) * slot_rows + r % slot_rows; };
-  float m = -INFINITY, l = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c = part; c < used; c += N * LINES) {
-    f32x2 ml[N];
-    f32x4 x[N];
+  const int to = min(block + kJoinRows<D, LINES>, a.rows);
+  for (int r0 = block; r0 < to; r0 += ROWS) {
+    const int r = min(r0 + row, to - 1);
+    auto at = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 && x0 != w0 * share)) * slot_rows + r % slot_rows; };
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int c = part; c < used; c += N * LINES) {
+      f32x2 ml[N];
+      f32x4 x[N];
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int64_t i = at(min(c + u * LINES, used - 1));
-      ml[u] = parts.ml[i];
-      x[u] = *reinterpret_cast<const f32x4*>(parts.acc + i * D + d);
+      for (int u = 0; u < N; ++u) {
+        const int64_t i = at(min(c + u * LINES, used - 1));
+        ml[u] = parts.ml[i];
+        x[u] = *reinterpret_cast<const f32x4*>(parts.acc + i * D + d);
+      }
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < N; ++u) mx = fmaxf(mx, ml[u][0]);
+      const float ref = mx == -INFINITY ? 0.f : mx, f = __builtin_amdgcn_exp2f(m - ref);
+      l *= f;
+      acc *= f;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const float w = c + u * LINES < used ? __builtin_amdgcn_exp2f(ml[u][0] - ref) : 0.f;
+        l += ml[u][1] * w;
+        acc += x[u] * w;
+      }
+      m = mx;
     }
-    float mx = m;
+    if constexpr (LINES > 1) {
+      *reinterpret_cast<f32x4*>(&red[part][row][d]) = acc;
+      if (d == 0) *reinterpret_cast<f32x2*>(&red[part][row][D]) = f32x2{m, l};
+      __syncthreads();
+      float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < N; ++u) mx = fmaxf(mx, ml[u][0]);
-    const float ref = mx == -INFINITY ? 0.f : mx, f = __builtin_amdgcn_exp2f(m - ref);
-    l *= f;
-    acc *= f;
+      for (int u = 0; u < LINES; ++u) mx = fmaxf(mx, red[u][row][D]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      l = 0.f;
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      if (c + u * LINES >= used) continue;
-      const float w = __builtin_amdgcn_exp2f(ml[u][0] - ref);
-      l += ml[u][1] * w;
-      acc += x[u] * w;
+      for (int u = 0; u < LINES; ++u) {
+        const float w = __builtin_amdgcn_exp2f(red[u][row][D] - ref);
+        l += red[u][row][D + 1] * w;
+        acc += *reinterpret_cast<const f32x4*>(&red[u][row][d]) * w;
+      }
+      __syncthreads();
     }
-    m = mx;
-  }
-  *reinterpret_cast<f32x4*>(&red[part][row][d]) = acc;
-  if (d == 0) {
-    red[part][row][D] = m;
-    red[part][row][D + 1] = l;
-  }
-  const uint64_t there = __ballot(ancestors(parent, lane) != 0);  // split: the sequence has its place
-  __syncthreads();
-  if (part != 0 || r >= a.rows) return;
-  float mx = -INFINITY, lsum = 0.f;
+    if (part != 0 || r0 + row >= to) continue;
+    const int gh = r / a.T, t = r - gh * a.T;
+    T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
+    const bool zero = !(there >> t & 1) || l == 0.f;
+    float y[4];
 #pragma unroll
-  for (int u = 0; u < LINES; ++u) mx = fmaxf(mx, red[u][row][D]);
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  f32x4 total = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int u = 0; u < LINES; ++u) {
-    const float w = __builtin_amdgcn_exp2f(red[u][row][D] - ref);
-    lsum += red[u][row][D + 1] * w;
-    total += *reinterpret_cast<const f32x4*>(&red[u][row][d]) * w;
+    for (int i = 0; i < 4; ++i) y[i] = zero ? 0.f : acc[i] / l;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+    else
+      *reinterpret_cast<f32x4*>(out) = f32x4{y[0], y[1], y[2], y[3]};
   }
-  const int gh = r / a.T, t = r - gh * a.T;
-  T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
-  const bool zero = !(there >> t & 1) || lsum == 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = Elem<T>::from_f32(zero ? 0.f : total[i] / lsum);
 }
 
 constexpr int64_t kMostSteps = 1 << 30;
@@ -854,8 +913,16 @@ template <typename T, int D, int KEYS>
 int tree_finish(const TreeArgs& a, const Plan& p, hipStream_t s) {
   const int rc = check_launch("ferrite_tree_attention");
   if (rc != FERRITE_OK || !p.split) return rc;
-  hipLaunchKernelGGL((tree_join_kernel<T, D, KEYS>), dim3((unsigned)cdiv(a.rows, 256 / D), (unsigned)a.Hkv, (unsigned)a.B), dim3(256),
-                     0, s, a, (int)p.slot_rows);
+  auto join = [&](auto lines, auto at_once) {
+    hipLaunchKernelGGL((tree_join_kernel<T, D, KEYS, lines.value, at_once.value>),
+                       dim3((unsigned)cdiv(a.rows, kJoinRows<D, lines.value>), (unsigned)a.Hkv, (unsigned)a.B), dim3(256), 0, s, a,
+                       (int)p.slot_rows);
+  };
+  // Few heads are cut into many pieces.
+  if (p.groups >= 8 * (int64_t)a.B * a.Hkv * a.row_groups)
+    join(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+  else
+    join(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
   return check_launch("ferrite_tree_attention");
 }
 
