@@ -179,56 +179,78 @@ template <int KEYS>
 __device__ __forceinline__ int steps_at(const TreeArgs& a, int b, int p) {
   return b >= a.B ? 0 : in_cache(a, p) ? (p + KEYS - 1) / KEYS + (a.T + KEYS - 1) / KEYS : 1;
 }
-__device__ __forceinline__ int wave_total(int x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, kWave);
-  return __builtin_amdgcn_readfirstlane(x);
+// The sums over the lanes up to each, and over all.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // rows of 16 lanes: from 1, 2, 4 and 8 lanes below
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  return x;
 }
-__device__ __forceinline__ int share_of(const TreeArgs& a, int total) {  // steps of a workgroup
-  return max((total + a.groups - 1) / a.groups, a.least);
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
+// Steps of a workgroup, and whether every (head, row group) takes whole shares of the line (the last one's end empty): so it is
+// where the workgroups suffice for that, and none then has a second one to begin.
+struct Shares {
+  int share;
+  bool apart;
+  // Of the first 64 sequences, a lane each: position, steps, and places on the line up to each (of one head and row group).
+  int p, steps, upto;
+  __device__ __forceinline__ int pieces(int n) const { return (n + share - 1) / share; }
+  __device__ __forceinline__ int span(int n) const { return apart ? pieces(n) * share : n; }
+};
+template <int KEYS>
+__device__ __forceinline__ Shares shares_of(const TreeArgs& a, int lane) {
+  const int per_seq = a.Hkv * a.row_groups;
+  Shares s;
+  s.p = pos_of(a, lane);
+  s.steps = steps_at<KEYS>(a, lane, s.p);
+  s.upto = wave_scan(s.steps);
+  int total = last_lane(s.upto);
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += last_lane(wave_scan(steps_at<KEYS>(a, b0 + lane, pos_of(a, b0 + lane))));
+  s.share = __builtin_amdgcn_readfirstlane(max((total * per_seq + a.groups - 1) / a.groups, a.least));
+  const int upto = wave_scan(s.pieces(s.steps));
+  int pieces = last_lane(upto);
+  for (int b0 = 64; b0 < a.B; b0 += 64)
+    pieces += last_lane(wave_scan(s.pieces(steps_at<KEYS>(a, b0 + lane, pos_of(a, b0 + lane)))));
+  s.apart = (int64_t)pieces * per_seq <= a.groups;
+  if (s.apart) s.upto = upto * s.share;
+  return s;
 }
 
-// Where a workgroup is on the line: steps [s0, ..) of the hr-th (head, row group) of sequence b, [cur, end) its own.
+// Where a workgroup is on the line: steps [s0, s1) of the hr-th (head, row group) of sequence b, [cur, end) its own.
 template <int KEYS>
 struct Cursor {
   int b, p, steps, hr, s0, cur, end;
+  Shares sh;
 
   // false: nothing to do.
   __device__ __forceinline__ bool start(const TreeArgs& a, int lane) {
     const int per_seq = a.Hkv * a.row_groups;
     int seq_at = 0;  // where on the line the sequence begins
+    sh = Shares{1, false, 0, 0, 0};
     if (a.part) {
-      int sum = 0, p0 = 0;
-      for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int x = pos_of(a, b0 + lane);
-        p0 = b0 ? p0 : x;
-        sum += steps_at<KEYS>(a, b0 + lane, x);
-      }
-      const int total = wave_total(sum) * per_seq, share = share_of(a, total);
-      if ((int64_t)blockIdx.x * share >= total) return false;
-      cur = (int)blockIdx.x * share;
-      end = min(cur + share, total);
-      int before = 0;
-      b = p = 0;
-      steps = 1;
-      for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int x = b0 ? pos_of(a, b0 + lane) : p0, mine = steps_at<KEYS>(a, b0 + lane, x);
-        int upto = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const int y = __shfl_up(upto, off, kWave);
-          upto += lane >= off ? y : 0;
-        }
+      sh = shares_of<KEYS>(a, lane);
+      cur = (int)blockIdx.x * sh.share;
+      end = cur + sh.share;
+      int before = 0, x = sh.p, mine = sh.steps, upto = sh.upto;
+      for (int b0 = 0;;) {
         const uint64_t past = __ballot((before + upto) * per_seq > cur);
         if (past) {
           const int at = __builtin_ctzll(past);
           b = b0 + at;
-          p = __shfl(x, at, kWave);
-          steps = __shfl(mine, at, kWave);
-          seq_at = (before + __shfl(upto, at, kWave) - steps) * per_seq;
+          p = __builtin_amdgcn_readlane(x, at);
+          steps = __builtin_amdgcn_readlane(mine, at);
+          seq_at = (before + __builtin_amdgcn_readlane(upto, at) - sh.span(steps)) * per_seq;
           break;
         }
-        before += __shfl(upto, 63, kWave);
+        before += last_lane(upto);
+        if ((b0 += 64) >= a.B) return false;
+        x = pos_of(a, b0 + lane);
+        mine = steps_at<KEYS>(a, b0 + lane, x);
+        upto = wave_scan(sh.span(mine));
       }
     } else {
       b = (int)(blockIdx.x / per_seq);
@@ -242,21 +264,24 @@ struct Cursor {
     steps = __builtin_amdgcn_readfirstlane(steps);
     cur = __builtin_amdgcn_readfirstlane(cur);
     end = __builtin_amdgcn_readfirstlane(end);
-    const int at = cur - __builtin_amdgcn_readfirstlane(seq_at);
-    hr = at / steps;
-    s0 = at - hr * steps;
+    const int at = cur - __builtin_amdgcn_readfirstlane(seq_at), span = __builtin_amdgcn_readfirstlane(sh.span(steps));
+    hr = __builtin_amdgcn_readfirstlane(at / span);
+    s0 = at - hr * span;
     return true;
   }
-  // Behind steps [s0, s1).
-  __device__ __forceinline__ void pass(const TreeArgs& a, int s1) {
-    cur += s1 - s0;
+  __device__ __forceinline__ int s1() const { return min(steps, s0 + end - cur); }
+  // To the next (head, row group); false: none left.
+  __device__ __forceinline__ bool next(const TreeArgs& a) {
+    cur += steps - s0;  // of shares that stand apart there is no next
+    if (sh.apart || cur >= end) return false;
     s0 = 0;
-    if (++hr == a.Hkv * a.row_groups && cur < end) {
+    if (++hr == a.Hkv * a.row_groups) {
       hr = 0;
-      ++b;
+      if (++b >= a.B) return false;
       p = __builtin_amdgcn_readfirstlane(pos_of(a, b));
       steps = steps_at<KEYS>(a, b, p);
     }
+    return true;
   }
 };
 
@@ -299,9 +324,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, q0 = lane & 15;
   Cursor<KEYS> at;
   if (!at.start(a, lane)) return;
-  for (int slot = 2 * (int)blockIdx.x; at.cur < at.end; slot = 2 * (int)blockIdx.x + 1) {  // what it shares comes first or last
-    const int b = at.b, p = at.p, s0 = at.s0, s1 = min(at.steps, s0 + at.end - at.cur);
-    const int h = at.hr / a.row_groups, row0 = (at.hr % a.row_groups) * ROWS;
+  int slot = 2 * (int)blockIdx.x;
+  do {
+    // readfirstlane: descriptors must be provably uniform, or every load becomes a loop over the lanes' distinct ones.
+    const int b = __builtin_amdgcn_readfirstlane(at.b), p = __builtin_amdgcn_readfirstlane(at.p);
+    const int s0 = __builtin_amdgcn_readfirstlane(at.s0), s1 = __builtin_amdgcn_readfirstlane(at.s1());
+    const int hr = __builtin_amdgcn_readfirstlane(at.hr), h = hr / a.row_groups, row0 = (hr - h * a.row_groups) * ROWS;
     const bool valid = in_cache(a, p);
     const int cached = valid ? p : 0, cached_steps = (cached + KEYS - 1) / KEYS;
 
@@ -535,8 +563,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
     }
     __syncthreads();
 
-    at.pass(a, s1);
-  }
+    slot = 2 * (int)blockIdx.x + 1;  // what it shares comes first or last
+  } while (at.next(a));
 }
 
 // Many query rows (bf16): W waves of 32 rows each over the same keys, which go through LDS once for all of them. A stage of KEYS keys
@@ -567,9 +595,12 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, q0 = lane & 31;
   Cursor<KEYS> at;
   if (!at.start(a, lane)) return;
-  for (int slot = 2 * (int)blockIdx.x; at.cur < at.end; slot = 2 * (int)blockIdx.x + 1) {
-    const int b = at.b, p = at.p, s0 = at.s0, s1 = min(at.steps, s0 + at.end - at.cur);
-    const int h = at.hr / a.row_groups, row0 = (at.hr % a.row_groups) * ROWS;
+  int slot = 2 * (int)blockIdx.x;
+  do {
+    // readfirstlane: descriptors must be provably uniform, or every load becomes a loop over the lanes' distinct ones.
+    const int b = __builtin_amdgcn_readfirstlane(at.b), p = __builtin_amdgcn_readfirstlane(at.p);
+    const int s0 = __builtin_amdgcn_readfirstlane(at.s0), s1 = __builtin_amdgcn_readfirstlane(at.s1());
+    const int hr = __builtin_amdgcn_readfirstlane(at.hr), h = hr / a.row_groups, row0 = (hr - h * a.row_groups) * ROWS;
     const bool valid = in_cache(a, p);
     const int cached = valid ? p : 0, cached_steps = (cached + KEYS - 1) / KEYS, whole_to = cached / KEYS;
     const int to = valid ? s1 : s0;
@@ -786,8 +817,8 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       }
     }
     __syncthreads();
-    at.pass(a, s1);
-  }
+    slot = 2 * (int)blockIdx.x + 1;  // what it shares comes first or last
+  } while (at.next(a));
 }
 
 // Joins what several workgroups have of a row. The pieces of a row are dealt to LINES threads for every four elements, each adding
@@ -802,14 +833,12 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
   const int per_seq = a.Hkv * a.row_groups;
   const int d = threadIdx.x % PER * 4, row = threadIdx.x / PER % ROWS, part = threadIdx.x / PER / ROWS;
   const int p = pos_of(a, b), parent = lane < a.T ? a.parents[(int64_t)b * a.T + lane] : -2;
-  int sum = 0, before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int mine = steps_at<KEYS>(a, b0 + lane, pos_of(a, b0 + lane));
-    sum += mine;
-    before += b0 + lane < b ? mine : 0;
-  }
-  const int share = share_of(a, wave_total(sum) * per_seq), steps = steps_at<KEYS>(a, b, p);
-  const int x0 = wave_total(before) * per_seq + (h * a.row_groups + block / slot_rows) * steps;
+  const Shares sh = shares_of<KEYS>(a, lane);
+  int before = 0;
+  for (int b0 = 0; b0 < b; b0 += 64)
+    before += last_lane(wave_scan(b0 + lane < b ? sh.span(steps_at<KEYS>(a, b0 + lane, b0 ? pos_of(a, b0 + lane) : sh.p)) : 0));
+  const int share = sh.share, steps = steps_at<KEYS>(a, b, p);
+  const int x0 = before * per_seq + (h * a.row_groups + block / slot_rows) * sh.span(steps);
   const int w0 = x0 / share, used = (x0 + steps - 1) / share - w0 + 1;
   if (used == 1) return;  // one workgroup had it all
   const uint64_t there = __ballot(ancestors(parent, lane) != 0);  // divided: the sequence has its place
