@@ -25,7 +25,7 @@ namespace {
 // lane groups of a wave take consecutive tokens and walk over the same heads, so that every
 // token's angles are read once for a chunk of heads, a wave's stores of one head are one
 // contiguous stretch of the output, and whether a head is of q, k or v is uniform.
-constexpr int kChunk = 4;  // heads per wave; their loads go out together
+constexpr int kChunk = 8;  // heads of a wave at most: one reading of the angles for all of them
 
 struct HeadsArgs {
   const void* qkv;
@@ -167,14 +167,32 @@ __device__ __forceinline__ void angles(const HeadsArgs& a, const Unit<T, V, INTE
   }
 }
 
+// V weights at index i, of w's type.
+template <int V>
+__device__ __forceinline__ void load_weights(const HeadsArgs& a, const void* w, int i, float* out) {
+  if (!a.w_bf16) {
+    load_floats<V>(static_cast<const float*>(w) + i, out);
+  } else if constexpr (V == 1) {
+    out[0] = (float)static_cast<const bf16*>(w)[i];
+  } else {
+    typedef bf16 __attribute__((ext_vector_type(V))) vec;
+    const vec x = *reinterpret_cast<const vec*>(static_cast<const bf16*>(w) + i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = (float)x[e];
+  }
+}
+// The weights of a lane's pairs.
 template <typename T, int V, bool INTER>
-__device__ __forceinline__ void weights(const HeadsArgs& a, const Unit<T, V, INTER>& u, const void* w, float* lo,
-                                        float* hi) {
+__device__ __forceinline__ void weights(const HeadsArgs& a, const Unit<T, V, INTER>& u, const void* w, float* lo, float* hi) {
+  float x[2][V] = {};
+  if (u.on) {
+    load_weights<V>(a, w, u.lo, x[0]);
+    load_weights<V>(a, w, u.hi, x[1]);
+  }
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int i = INTER ? u.lo + 2 * e : u.lo + e, j = INTER ? i + 1 : u.hi + e;
-    lo[e] = !u.on ? 0.f : a.w_bf16 ? (float)static_cast<const bf16*>(w)[i] : static_cast<const float*>(w)[i];
-    hi[e] = !u.on ? 0.f : a.w_bf16 ? (float)static_cast<const bf16*>(w)[j] : static_cast<const float*>(w)[j];
+    lo[e] = INTER && V > 1 ? x[2 * e / V][2 * e % V] : x[0][e];
+    hi[e] = INTER && V > 1 ? x[(2 * e + 1) / V][(2 * e + 1) % V] : x[1][e];
   }
 }
 
@@ -207,66 +225,53 @@ __global__ __launch_bounds__(256) void heads_rope_kernel(HeadsArgs a) {
   T* dst = static_cast<T*>(ch.kind == 0 ? a.q : ch.kind == 1 ? a.k : a.v) + (b * heads * a.S + s) * a.D;
   const int64_t head_step = (int64_t)a.S * a.D;
 
-  raw_t A[kChunk][N], B[kChunk][N];
+  float c[N][V], sn[N][V], wl[N][V], wh[N][V];
+  if (ch.kind < 2) {
+    const int p = a.pos ? (here ? a.pos[token] : 0) : s;
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    if (ch.from + i >= ch.to) break;
+    for (int n = 0; n < N; ++n) {
+      angles(a, u[n], p, c[n], sn[n]);
+      weights(a, u[n], ch.kind == 0 ? a.wq : a.wk, wl[n], wh[n]);
+    }
+  }
+  for (int h = ch.from; h < ch.to; ++h) {
+    raw_t A[N], B[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       if (!u[n].on) continue;
-      const T* p = src + (int64_t)(ch.from + i) * a.D;
-      A[i][n] = *reinterpret_cast<const raw_t*>(p + u[n].lo);
-      B[i][n] = *reinterpret_cast<const raw_t*>(p + u[n].hi);
+      const T* p = src + (int64_t)h * a.D;
+      A[n] = *reinterpret_cast<const raw_t*>(p + u[n].lo);
+      B[n] = *reinterpret_cast<const raw_t*>(p + u[n].hi);
     }
-  }
-  if (ch.kind == 2) {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      if (ch.from + i >= ch.to) break;
+    if (ch.kind < 2) {
+      float lo[N][V], hi[N][V], ss = 0.f;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         if (!u[n].on) continue;
-        T* o = dst + (ch.from + i) * head_step;
-        *reinterpret_cast<raw_t*>(o + u[n].lo) = A[i][n];
-        *reinterpret_cast<raw_t*>(o + u[n].hi) = B[i][n];
+        U::pairs(A[n], B[n], lo[n], hi[n]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) ss += lo[n][e] * lo[n][e] + hi[n][e] * hi[n][e];
+      }
+      const float r = rsqrtf(group_sum<L>(ss) / (float)a.D + a.eps);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (!u[n].on) continue;
+        float yl[V], yh[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float ul = lo[n][e] * r * wl[n][e], uh = hi[n][e] * r * wh[n][e];
+          yl[e] = ul * c[n][e] - uh * sn[n][e];
+          yh[e] = uh * c[n][e] + ul * sn[n][e];
+        }
+        U::vectors(yl, yh, A[n], B[n]);
       }
     }
-    return;
-  }
-  const int p = a.pos ? (here ? a.pos[token] : 0) : s;
-  float c[N][V], sn[N][V], wl[N][V], wh[N][V];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    angles(a, u[n], p, c[n], sn[n]);
-    weights(a, u[n], ch.kind == 0 ? a.wq : a.wk, wl[n], wh[n]);
-  }
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    if (ch.from + i >= ch.to) break;
-    float lo[N][V], hi[N][V], ss = 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       if (!u[n].on) continue;
-      U::pairs(A[i][n], B[i][n], lo[n], hi[n]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss += lo[n][e] * lo[n][e] + hi[n][e] * hi[n][e];
-    }
-    const float r = rsqrtf(group_sum<L>(ss) / (float)a.D + a.eps);
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if (!u[n].on) continue;
-      float yl[V], yh[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float ul = lo[n][e] * r * wl[n][e], uh = hi[n][e] * r * wh[n][e];
-        yl[e] = ul * c[n][e] - uh * sn[n][e];
-        yh[e] = uh * c[n][e] + ul * sn[n][e];
-      }
-      raw_t oa, ob;
-      U::vectors(yl, yh, oa, ob);
-      T* o = dst + (ch.from + i) * head_step;
-      *reinterpret_cast<raw_t*>(o + u[n].lo) = oa;
-      *reinterpret_cast<raw_t*>(o + u[n].hi) = ob;
+      T* o = dst + h * head_step;
+      *reinterpret_cast<raw_t*>(o + u[n].lo) = A[n];
+      *reinterpret_cast<raw_t*>(o + u[n].hi) = B[n];
     }
   }
 }
@@ -299,42 +304,36 @@ __global__ __launch_bounds__(256) void heads_rope_bwd_kernel(HeadsArgs a) {
     const T* src = static_cast<const T*>(a.qkv) + b * a.batch_stride + s * a.row_stride + (int64_t)base * a.D;
     const T* gsrc = grad + (b * heads * a.S + s) * a.D;
     T* dst = static_cast<T*>(a.dqkv) + token * width + (int64_t)base * a.D;
-    raw_t A[kChunk][N] = {}, B[kChunk][N] = {}, GA[kChunk][N] = {}, GB[kChunk][N] = {};
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      if (ch.from + i >= ch.to) break;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (!u[n].on || !here) continue;
-        const T* p = src + (int64_t)(ch.from + i) * a.D;
-        const T* g = gsrc + (ch.from + i) * head_step;
-        if (grad) {
-          GA[i][n] = *reinterpret_cast<const raw_t*>(g + u[n].lo);
-          GB[i][n] = *reinterpret_cast<const raw_t*>(g + u[n].hi);
-        }
-        if (ch.kind < 2) {
-          A[i][n] = *reinterpret_cast<const raw_t*>(p + u[n].lo);
-          B[i][n] = *reinterpret_cast<const raw_t*>(p + u[n].hi);
-        }
-      }
-    }
     float c[N][V], sn[N][V];
     if (ch.kind < 2) {
       const int p = a.pos ? (here ? a.pos[token] : 0) : s;
 #pragma unroll
       for (int n = 0; n < N; ++n) angles(a, u[n], p, c[n], sn[n]);
     }
+    for (int h = ch.from; h < ch.to; ++h) {
+      raw_t A[N] = {}, B[N] = {}, GA[N] = {}, GB[N] = {};
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      if (ch.from + i >= ch.to) break;
+      for (int n = 0; n < N; ++n) {
+        if (!u[n].on || !here) continue;
+        const T* p = src + (int64_t)h * a.D;
+        const T* g = gsrc + h * head_step;
+        if (grad) {
+          GA[n] = *reinterpret_cast<const raw_t*>(g + u[n].lo);
+          GB[n] = *reinterpret_cast<const raw_t*>(g + u[n].hi);
+        }
+        if (ch.kind < 2) {
+          A[n] = *reinterpret_cast<const raw_t*>(p + u[n].lo);
+          B[n] = *reinterpret_cast<const raw_t*>(p + u[n].hi);
+        }
+      }
       if (ch.kind < 2) {
         float lo[N][V], hi[N][V], ul[N][V], uh[N][V], ss = 0.f, st = 0.f;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
           if (!u[n].on || !here) continue;
           float gl[V], gh[V];
-          U::pairs(A[i][n], B[i][n], lo[n], hi[n]);
-          U::pairs(GA[i][n], GB[i][n], gl, gh);
+          U::pairs(A[n], B[n], lo[n], hi[n]);
+          U::pairs(GA[n], GB[n], gl, gh);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             ul[n][e] = gl[e] * c[n][e] + gh[e] * sn[n][e];
@@ -356,15 +355,15 @@ __global__ __launch_bounds__(256) void heads_rope_bwd_kernel(HeadsArgs a) {
             xl[e] = r * (ul[n][e] * wl[n][e] - lo[n][e] * t);
             xh[e] = r * (uh[n][e] * wh[n][e] - hi[n][e] * t);
           }
-          U::vectors(xl, xh, GA[i][n], GB[i][n]);
+          U::vectors(xl, xh, GA[n], GB[n]);
         }
       }
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         if (!u[n].on || !here) continue;
-        T* o = dst + (int64_t)(ch.from + i) * a.D;
-        *reinterpret_cast<raw_t*>(o + u[n].lo) = GA[i][n];
-        *reinterpret_cast<raw_t*>(o + u[n].hi) = GB[i][n];
+        T* o = dst + (int64_t)h * a.D;
+        *reinterpret_cast<raw_t*>(o + u[n].lo) = GA[n];
+        *reinterpret_cast<raw_t*>(o + u[n].hi) = GB[n];
       }
     }
   }
@@ -447,18 +446,26 @@ bool vectors_fit(const HeadsArgs& a, int esize) {
   const int v = 16 / esize;
   return a.D % (2 * v) == 0 && a.R % (2 * v) == 0 && a.row_stride % v == 0 && a.batch_stride % v == 0 &&
          aligned16(a.qkv) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.cos) && aligned16(a.sin) &&
-         aligned16(a.dqkv);
+         aligned16(a.dqkv) && aligned16(a.wq) && aligned16(a.wk);
 }
 
 int chunks_of(const HeadsArgs& a) { return (int)(cdiv(a.H, a.chunk) + 2 * cdiv(a.Hkv, a.chunk)); }
 
 // Tokens to a wave are at most 32; few tokens take a head per wave, so that their heads spread over the CUs.
-void set_chunk(HeadsArgs& a) { a.chunk = a.tokens * (a.H + 2 * a.Hkv) < 65536 ? 1 : kChunk; }
+// The heads of one kind are cut evenly.
+void set_chunk(HeadsArgs& a) {
+  const int most = a.tokens * (a.H + 2 * a.Hkv) < 65536 ? 1 : kChunk, heads = std::max(a.H, a.Hkv);
+  a.chunk = (int)cdiv(heads, cdiv(heads, (int64_t)most));
+}
 
-// Blocks along the tokens of the backward: four resident on a CU over all chunks, and no more than there are tokens for.
-int64_t bwd_blocks(int64_t tokens, int64_t chunks) {
-  const int64_t want = std::max<int64_t>(1, 1024 / chunks);
-  return std::max<int64_t>(1, std::min(want, cdiv(tokens, 8)));
+// Blocks along the tokens of the backward: some eight waves a SIMD over all chunks, their groups of tokens (4 waves of 64 / L
+// tokens) dealt evenly.
+int64_t most_blocks(int64_t tokens, int64_t chunks) {
+  return std::max<int64_t>(1, std::min<int64_t>(2048 / chunks, cdiv(tokens, (int64_t)4)));  // a wave takes a token or more
+}
+int64_t bwd_blocks(int64_t tokens, int64_t chunks, int per_block) {
+  const int64_t groups = cdiv(tokens, (int64_t)per_block);
+  return cdiv(groups, cdiv(groups, most_blocks(tokens, chunks)));
 }
 
 int check_heads(const char* name, int64_t b, int64_t s, int64_t h, int64_t hkv, int64_t d, int64_t rot, int64_t table,
@@ -517,7 +524,7 @@ extern "C" int64_t ferrite_internal_heads_rope_bwd_workspace(int64_t b, int64_t 
   a.Hkv = (int)hkv;
   set_chunk(a);
   const int64_t chunks = chunks_of(a), kept = cdiv(a.H, a.chunk) + cdiv(a.Hkv, a.chunk);
-  return kept * bwd_blocks(a.tokens, chunks) * d * (int64_t)sizeof(float);
+  return kept * most_blocks(a.tokens, chunks) * d * (int64_t)sizeof(float);
 }
 
 extern "C" int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64_t row_stride,
@@ -538,12 +545,14 @@ extern "C" int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_st
               const_cast<void*>(dv), dqkv, static_cast<float*>(workspace), b * s, (int)s, (int)h, (int)hkv, (int)d,
               (int)rot, (int)table, 0, eps, w_dtype == FERRITE_BF16};
   set_chunk(a);
-  const int64_t chunks = chunks_of(a), blocks = bwd_blocks(a.tokens, chunks);
+  const int64_t chunks = chunks_of(a);
+  int64_t blocks = 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.tokens) {
     auto launch = [&](auto* t, auto inter) {
       typedef std::remove_pointer_t<decltype(t)> T;
       return with_layout<T, inter.value>(vectors_fit(a, sizeof(T)), a.D, [&](auto V, auto L, auto N) {
+        blocks = bwd_blocks(a.tokens, chunks, 4 * (64 / L.value));
         hipLaunchKernelGGL((heads_rope_bwd_kernel<T, V.value, L.value, N.value, inter.value>),
                            dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0, st, a);
         return check_launch("ferrite_heads_rope_bwd");
@@ -554,9 +563,8 @@ extern "C" int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_st
                          : (interleaved ? launch((float*)nullptr, std::true_type{}) : launch((float*)nullptr, std::false_type{}));
     if (done != FERRITE_OK) return done;
   }
-  const int64_t rows = a.tokens ? blocks : 0;
   hipLaunchKernelGGL(heads_rope_dw_kernel, dim3((unsigned)cdiv(d, (int64_t)kDwCols), 2), dim3(1024), 0, st,
-                     static_cast<const float*>(workspace), dwq, dwk, rows * cdiv(h, (int64_t)a.chunk),
-                     rows * cdiv(hkv, (int64_t)a.chunk), (int)d, a.w_bf16);
+                     static_cast<const float*>(workspace), dwq, dwk, blocks * cdiv(h, (int64_t)a.chunk),
+                     blocks * cdiv(hkv, (int64_t)a.chunk), (int)d, a.w_bf16);
   return check_launch("ferrite_heads_rope_bwd");
 }
