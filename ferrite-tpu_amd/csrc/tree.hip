@@ -924,16 +924,23 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   p.slot_rows = p.wide ? (d == 256 ? 128 : 256) : 16 * p.tiles;
   p.row_groups = cdiv(rows, p.slot_rows);
   const int64_t heads = b * hkv * p.row_groups, steps = cdiv(max_len, p.keys) + cdiv(t, p.keys);
-  // Workgroups that are resident together.
+  // Workgroups that are resident together, and steps that one takes at least (one to a wave; with two to a wave one head of
+  // 1024 keys takes 15.3 us and not 13.4, f32 with 700 keys of 256 elements 34.9 and not 19.6).
   const int per_cu = p.wide ? 1 : p.tiles == 1 ? (d == 64 ? 3 : d == 128 ? 2 : 1) : p.tiles == 2 && d == 64 ? 2 : 1;
   p.groups = 256 * per_cu;
-  p.least = p.wide ? 4 : (half || p.tiles == 1 ? 2 : 1) * p.waves;
-  p.split = heads < 4 * p.groups && steps > (p.wide ? 8 : 32);
-  if (!p.split) {
-    p.groups = heads;
-    if (!p.wide && p.tiles == 1 && d <= 128 && steps > 8) p.waves = 8;
-  } else {
+  p.least = p.wide ? 2 : p.waves;
+  const bool eight = !p.wide && p.tiles == 1 && d <= 128;
+  // Whole heads need no second kernel. Short ones, or many, lose less by uneven shares than that one costs: 256 heads of 1024
+  // keys of 128 elements take 23.2 us whole and 26.4 cut (f32 46.1 and 47.4), 512 of 64 elements 19.3 and 25.9; but 32 of
+  // 128 elements 18.5 whole and 11.3 cut, 128 of them 20.5 and 16.2, f32 64 of 512 keys 24.2 and 16.2.
+  p.split = heads < 4 * p.groups && steps > (p.wide ? 8 : heads >= 256 ? 128 : eight ? 32 : 16);
+  if (p.split) {
     p.groups = std::min(p.groups, cdiv(heads * steps, p.least));
+  } else {
+    p.groups = heads;
+    // Eight waves to a head while that brings more waves to a CU (4 heads of 512 keys: 10.6 us, with four waves 13.6); 1024
+    // heads of 512 keys fill it with four (32.2 us, with eight 45.6; f32 66.9 and 81.1).
+    if (eight && steps > 8 && heads < 512) p.waves = 8;
   }
   return p;
 }
