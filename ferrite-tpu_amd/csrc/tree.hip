@@ -59,6 +59,12 @@ constexpr int kTiles = sizeof(T) == 2 ? 2 : 1;
 // no memory.
 constexpr uint32_t kMostBytes = 0xfffe0000u;
 
+// A word of values, infinities and NaN as zeros.
+__device__ __forceinline__ uint32_t finite_of(uint32_t x, float) { return (x & 0x7f800000u) == 0x7f800000u ? 0 : x; }
+__device__ __forceinline__ uint32_t finite_of(uint32_t x, bf16) {
+  return ((x & 0x7f800000u) == 0x7f800000u ? 0 : x & 0xffff0000u) | ((x & 0x7f80u) == 0x7f80u ? 0 : x & 0xffffu);
+}
+
 template <typename T, int D>
 struct Step {
   static constexpr int NS = kTiles<T>, KEYS = 16 * NS, RB = D * (int)sizeof(T), KB = RB / 64, VD = RB / 64;
@@ -107,6 +113,24 @@ struct Step {
 #pragma unroll
         for (int w = 0; w < VD; ++w) v[4 * n + i][w] &= keep;
       }
+  }
+  // Whether any value is infinite or NaN; those as zeros.
+  __device__ __forceinline__ bool not_finite() const {
+    uint32_t most[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4 * NS; ++i)
+#pragma unroll
+      for (int w = 0; w < VD; ++w) {
+        most[0] = max(most[0], v[i][w] & 0x7fffffffu);
+        if (sizeof(T) == 2) most[1] = max(most[1], v[i][w] << 16 & 0x7fffffffu);
+      }
+    return max(most[0], most[1]) >= 0x7f800000u;
+  }
+  __device__ __forceinline__ void drop_not_finite() {
+#pragma unroll
+    for (int i = 0; i < 4 * NS; ++i)
+#pragma unroll
+      for (int w = 0; w < VD; ++w) v[i][w] = finite_of(v[i][w], T{});
   }
 };
 
@@ -285,6 +309,22 @@ struct Cursor {
   }
 };
 
+// A node's value that is infinite or NaN counts for the rows that see it and for no other, but the products would have it times a
+// weight of 0 for those: it is left out there, and here is what such values of the nodes from .. to - 1 add to elements
+// d .. d + 3 of node t, which is there: along its line of parents.
+template <typename T>
+__device__ __forceinline__ f32x4 not_finite_of(const TreeArgs& a, int b, const T* vn, int t, int from, int to, int d) {
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int s = t; s >= from; s = a.parents[(int64_t)b * a.T + s])
+    if (s < to)
+      for (int i = 0; i < 4; ++i) {
+        const float v = (float)vn[s * a.vs[2] + d + i];
+        x[i] += __builtin_isfinite(v) ? 0.f : v;
+      }
+  return x;
+}
+
 // Slots of `rows` rows: (m, l) of each, then the unnormalised outputs.
 struct Parts {
   f32x2* ml;   // [slots, rows]
@@ -392,6 +432,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
     if (QL) __syncthreads();
 
     float m[NT], l[NT];
+    int odd_values = 0;  // whether nodes' values that are not finite were left out
     f32x4 o[NT][VE];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -423,7 +464,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
       if (at >= whole_to) {  // not every row sees every key: bit k of `sees` is the step's key k
         const bool old = at < cached_steps;
         const int first = old ? 0 : (at - cached_steps) * KEYS;
-        if (!old) st.drop_absent((uint32_t)(there >> first), lane);
+        if (!old) {
+          st.drop_absent((uint32_t)(there >> first), lane);
+          if (__any(st.not_finite())) {
+            st.drop_not_finite();
+            odd_values = 1;
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint64_t mine = __shfl((unsigned long long)line, node[n], kWave) >> first;
@@ -527,7 +574,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
           *reinterpret_cast<f32x4*>(&red[row * (D + 4) + g * (D / 4) + i * VE + j]) =
               f32x4{o[n][j][i], o[n][j + 1][i], o[n][j + 2][i], o[n][j + 3][i]};
     }
+    if (lane == 0) reinterpret_cast<int*>(red)[wave * ROWS * (D + 4) + D] = odd_values;
     __syncthreads();
+    odd_values = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) odd_values |= reinterpret_cast<const int*>(red)[w * ROWS * (D + 4) + D];
     const bool whole = s0 == 0 && s1 == at.steps;
     const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, ROWS);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * W) {
@@ -544,6 +595,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
         lsum += red_l[r + w * ROWS] * f;
         sum += *reinterpret_cast<const f32x4*>(&red[(r + w * ROWS) * (D + 4) + d]) * f;
       }
+      if (odd_values && there >> (row0 + r) % a.T & 1)
+        sum += not_finite_of(a, b, vn, (row0 + r) % a.T, (max(s0, cached_steps) - cached_steps) * KEYS, (s1 - cached_steps) * KEYS, d);
       if (whole) {
         const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
         T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
@@ -674,6 +727,25 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       for (int hi = 0; hi < 2; ++hi)
         voff[j][hi] = KEYS * RB + C::place(8 * hi + 4 * g + (lane & 15) / 4, 4 * j + (lane >> 4 & 1) * 2 + (lane & 3) / 2) + (lane & 1) * 8;
 
+    int odd_values = 0;  // whether nodes' values that are not finite were left out
+    // Of a step of nodes a wave reads the values that it copied (it has waited for them), and makes those zeros.
+    auto clean = [&](int s) {
+      if (s < cached_steps || s >= to) return;
+      char* const values = lds + (s - s0) % 4 * C::STAGE + KEYS * RB + wave * 1024 + lane * 16;
+#pragma unroll
+      for (int u = 0; u < C::COPIES / 2; ++u) {
+        u32x4& at = *reinterpret_cast<u32x4*>(values + u * W * 1024);
+        const u32x4 is = at;
+        u32x4 fin;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fin[e] = finite_of(is[e], bf16{});
+        if (fin[0] != is[0] || fin[1] != is[1] || fin[2] != is[2] || fin[3] != is[3]) {
+          at = fin;
+          odd_values = 1;
+        }
+      }
+    };
+
     float m = -INFINITY, l = 0.f;
     f32x16 o[D / 32], x[NT];
 #pragma unroll
@@ -696,11 +768,15 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
     // takes. Before the barrier at which the leading waves begin that product, every wave has waited for its copies of step
     // s + 1: they when they leave the softmax of s, the others when they leave the product of s - 1.
     wait_vmem<2 * C::COPIES>();
+    clean(s0);
     lds_barrier();
     if (mine && s0 < to) scores(s0);
     if (!leads) lds_barrier();
     for (int s = s0; s < to; ++s) {
-      if (!leads) wait_vmem<C::COPIES>();
+      if (!leads) {
+        wait_vmem<C::COPIES>();
+        clean(s + 1);
+      }
       lds_barrier();
       u32x4 pb[KEYS / 16];
       if (mine) {
@@ -741,7 +817,10 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
 #pragma unroll
           for (int e = 0; e < 4; ++e) pb[c][e] = pack_bf16(x[c / 2][c % 2 * 8 + 2 * e], x[c / 2][c % 2 * 8 + 2 * e + 1]);
       }
-      if (leads) wait_vmem<C::COPIES>();
+      if (leads) {
+        wait_vmem<C::COPIES>();
+        clean(s + 1);
+      }
       lds_barrier();
       copy(s + 3);
       if (!mine) continue;
@@ -793,15 +872,22 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         for (int i = 0; i < 16; i += 4)
           *reinterpret_cast<f32x4*>(&red[row * (D + 4) + 32 * j + 2 * i + 4 * g]) = f32x4{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
       if (g == 0) *reinterpret_cast<f32x2*>(&red[row * (D + 4) + D]) = f32x2{m, lt};
+      odd_values = __any(odd_values);
+      if (lane == 0) reinterpret_cast<int*>(red)[wave * 32 * (D + 4) + D + 2] = odd_values;
     }
     __syncthreads();
+    odd_values = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) odd_values |= reinterpret_cast<const int*>(red)[w * 32 * (D + 4) + D + 2];
     const bool whole = s0 == 0 && s1 == at.steps;
     const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, ROWS);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * W) {
       const int r = e / (D / 4), d = e % (D / 4) * 4;  // row r of the row group
       if (row0 + r >= a.rows) break;
-      const f32x4 sum = *reinterpret_cast<const f32x4*>(&red[r * (D + 4) + d]);
+      f32x4 sum = *reinterpret_cast<const f32x4*>(&red[r * (D + 4) + d]);
       const f32x2 ml = *reinterpret_cast<const f32x2*>(&red[r * (D + 4) + D]);
+      if (odd_values && there >> (row0 + r) % a.T & 1)
+        sum += not_finite_of(a, b, vn, (row0 + r) % a.T, (max(s0, cached_steps) - cached_steps) * KEYS, (s1 - cached_steps) * KEYS, d);
       if (whole) {
         const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
         bf16* out = static_cast<bf16*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
@@ -866,9 +952,11 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
       acc *= f;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        const float w = c + u * LINES < used ? __builtin_amdgcn_exp2f(ml[u][0] - ref) : 0.f;
-        l += ml[u][1] * w;
-        acc += x[u] * w;
+        const bool on = c + u * LINES < used;  // else the last piece again, whose values need not be finite
+        const float w = __builtin_amdgcn_exp2f(ml[u][0] - ref);
+        l += on ? ml[u][1] * w : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += on ? x[u][e] * w : 0.f;
       }
       m = mx;
     }

@@ -24,7 +24,8 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, pos, parents, *, scale: fl
 
     Node t of a sequence hangs on node ``parents[b, t]`` < t, or on the committed tokens (-1). It sees the cache's rows
     0 .. pos - 1, its ancestors and itself. A node with any other parent, or that hangs on such a node, is absent (the
-    padding of a smaller tree): nothing is written for it, nobody sees it and its output is zero. A sequence whose
+    padding of a smaller tree): nothing is written for it, nobody sees it and its output is zero. What a node does not see does not touch its output, NaN and infinities
+    included. A sequence whose
     rows pos .. pos + T - 1 do not lie in the cache writes nothing and yields NaN. Scores and softmax are f32."""
     if q.ndim != 4 or k_new.ndim != 4 or v_new.shape != k_new.shape or k_new.shape[0] != q.shape[0] \
             or k_new.shape[2:] != q.shape[2:] or k_new.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k_new.shape[1]:
@@ -81,9 +82,10 @@ def tree_attention_reference(q, k_new, v_new, k_cache, v_cache, pos, parents, *,
         k_cache[i, :, p + there] = k_new[i][:, there]
         v_cache[i, :, p + there] = v_new[i][:, there]
         out[i] = 0
-        keys = torch.cat([k_cache[i, :, :p], k_new[i][:, there]], 1).to(work).repeat_interleave(h // hkv, 0)
-        values = torch.cat([v_cache[i, :, :p], v_new[i][:, there]], 1).to(work).repeat_interleave(h // hkv, 0)
-        hidden = ~torch.cat([torch.ones(len(there), p, dtype=torch.bool, device=q.device), sees[there][:, there]], 1)
-        s = torch.matmul(q[i][:, there].to(work), keys.transpose(1, 2).contiguous()) * scale
-        out[i][:, there] = torch.matmul(torch.softmax(s.masked_fill(hidden, float("-inf")), -1), values).to(q.dtype)
+        for t in there.tolist():
+            rows = torch.cat([torch.arange(p, device=q.device), p + sees[t].nonzero()[:, 0]])
+            keys = k_cache[i][:, rows].to(work).repeat_interleave(h // hkv, 0)
+            values = v_cache[i][:, rows].to(work).repeat_interleave(h // hkv, 0)
+            s = (keys * q[i][:, t, None].to(work)).sum(-1) * scale
+            out[i][:, t] = (torch.softmax(s, -1)[..., None] * values).sum(1).to(q.dtype)
     return out

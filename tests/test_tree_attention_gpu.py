@@ -119,6 +119,33 @@ def test_unseen_values_do_not_matter(dev):
             assert torch.equal(tree_attention(q, a, c, k, v, p, parents.to(dev)), clean)
 
 
+@pytest.mark.parametrize("b,h,hkv,t,length,d,dtype,pos", [
+    (2, 2, 2, 9, 80, 64, BF16, [70, 0]), (2, 4, 2, 20, 3000, 128, BF16, [2900, 64]), (1, 6, 2, 18, 900, 256, BF16, [800]),
+    (2, 8, 2, 40, 200, 128, BF16, [160, 31]), (1, 3, 1, 64, 2000, 64, BF16, [1900]), (1, 2, 1, 40, 700, 256, BF16, [650]),
+    (2, 4, 2, 20, 700, 128, F32, [600, 3]), (1, 2, 2, 7, 60, 256, F32, [40])])
+def test_what_a_branch_does_not_see_does_not_touch_it(dev, b, h, hkv, t, length, d, dtype, pos):
+    """NaN and infinities in keys and values of a node that is there: rows that do not see it keep their bits; those
+    that do are what the sums over the nodes they see are."""
+    q, kn, vn, kc, vc = _inputs(dev, b, h, hkv, t, length, d, dtype, seed=t)
+    parents = torch.where(torch.arange(t) > 1, torch.arange(t) - 2, -1).int().expand(b, t).contiguous()  # two branches
+    clean = _check(dev, q, kn, vn, kc, vc, pos, parents)
+    k, v = kn.clone(), vn.clone()
+    v[:, 0, t // 2, 5], v[:, 0, t // 2 + 2, 5], v[:, -1, t - 1, 9] = float("inf"), -float("inf"), float("nan")
+    v[:, 0, t // 2, 8] = -float("inf")
+    k[:, -1, t // 2 + 1, 3] = float("nan")
+    p, par = torch.tensor(pos, dtype=torch.int32, device=dev), parents.to(dev)
+    dbl = [x.double() for x in (q, k, v, kc, vc)]
+    ref = tree_attention_reference(*dbl, p, par)
+    out = tree_attention(q, k, v, kc, vc, p, par)
+    assert torch.equal(kc.double().nan_to_num(7), dbl[3].nan_to_num(7)) and torch.equal(vc.double().nan_to_num(7), dbl[4].nan_to_num(7))
+    assert torch.equal(torch.isnan(out), torch.isnan(ref))
+    assert torch.equal(out == float("inf"), ref == float("inf")) and torch.equal(out == -float("inf"), ref == -float("inf"))
+    near = (out.double() - ref).abs() <= (4.8e-5 if dtype == F32 else 2.0**-8 * (ref.abs() + 5.5))
+    assert bool((near | ~torch.isfinite(ref)).all()) and not bool(torch.isfinite(ref).all())
+    other = (torch.arange(t) - t // 2) % 2 == 1  # the branch whose only bad node is a key of the last head and a value of it
+    assert torch.equal(out[:, : h // hkv][:, :, other], clean[:, : h // hkv][:, :, other]) or hkv == 1
+
+
 def test_large_scores(dev):
     """Scores of some hundreds: one key takes all the weight; rows whose keys are at -inf see only the others."""
     for dtype in (BF16, F32):
