@@ -85,6 +85,29 @@ def test_matches_64_bits(dev, b, h, hkv, t, length, d, dtype, pos):
     _check(dev, *x, pos, trees(b, t, 2, absent=0.3), scale=0.3 / d**0.5)
 
 
+@pytest.mark.parametrize("b,h,hkv,t,length,d,dtype", [
+    (70, 2, 2, 3, 1200, 64, F32),      # cut, more than 64 sequences
+    (200, 8, 4, 2, 2100, 64, F32),     # cut, more heads than workgroups
+    (130, 4, 2, 5, 600, 128, BF16),    # whole
+    (70, 3, 1, 30, 800, 64, BF16),     # 90 rows over shared keys: cut
+    (80, 6, 2, 60, 300, 128, BF16),    # whole
+    (66, 2, 1, 20, 500, 256, BF16)])
+def test_many_sequences(dev, b, h, hkv, t, length, d, dtype):
+    x = _inputs(dev, b, h, hkv, t, length, d, dtype, seed=b)
+    pos = torch.randint(0, length - t + 1, (b,), generator=torch.Generator().manual_seed(b))
+    pos[1], pos[b // 2], pos[b - 1], pos[65] = 0, -1, length - t, length
+    _check(dev, *x, pos.tolist(), trees(b, t, 1, absent=0.1))
+
+
+@pytest.mark.parametrize("h,hkv,t,length,d,dtype", [
+    (2, 2, 7, 400, 128, BF16), (4, 1, 40, 300, 64, BF16), (5, 1, 52, 1500, 128, BF16), (1, 1, 64, 400, 256, BF16),
+    (3, 1, 9, 500, 128, F32)])
+def test_scales_of_any_sign(dev, h, hkv, t, length, d, dtype):
+    x = _inputs(dev, 2, h, hkv, t, length, d, dtype, seed=t)
+    for scale in (-0.7 / d**0.5, 0.0, -0.0):
+        _check(dev, *x, [length - t, 40], trees(2, t, 1), scale=scale)
+
+
 def test_chains_stars_and_forests(dev):
     """A chain, children of one node, roots only, the deepest branch, everything absent; 64 nodes and fewer."""
     for t in (64, 20):
