@@ -36,6 +36,7 @@ struct TreeArgs {
   int B, H, Hkv, G, T, L, rows;  // rows = G T
   int row_groups;                // workgroups' row blocks per head
   int groups, least;             // workgroups that share the work, and steps of one at least
+  int begin;                     // what beginning a (head, row group) costs, in steps
   float c;                       // |scale| log2(e)
   uint32_t flip;                 // sign bits to flip in q (a negative scale)
 };
@@ -194,9 +195,9 @@ __device__ __forceinline__ float sum16(float x) {
 }
 
 // The work is a line of steps: sequence by sequence, (head, row group) by (head, row group), the steps of its cached keys and
-// of its nodes (one step for a sequence that has no place in the cache). It is cut evenly over the workgroups, so each
-// has at most one (head, row group) that it shares with workgroups before it and one with workgroups
-// behind it; their states go to its two slots of the workspace.
+// of its nodes (one step for a sequence that has no place in the cache), and in front of them places without work, as many
+// as it costs to begin. It is cut evenly over the workgroups, so each has at most one (head, row group) that it shares with
+// workgroups before it and one with workgroups behind it; their states go to its two slots of the workspace.
 __device__ __forceinline__ int pos_of(const TreeArgs& a, int b) { return a.pos[min(b, a.B - 1)]; }
 __device__ __forceinline__ bool in_cache(const TreeArgs& a, int p) { return p >= 0 && p <= a.L - a.T; }
 template <int KEYS>
@@ -218,12 +219,12 @@ __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readla
 // Steps of a workgroup, and whether every (head, row group) takes whole shares of the line (the last one's end empty): so it is
 // where the workgroups suffice for that, and none then has a second one to begin.
 struct Shares {
-  int share;
+  int share, begin;
   bool apart;
   // Of the first 64 sequences, a lane each: position, steps, and places on the line up to each (of one head and row group).
   int p, steps, upto;
   __device__ __forceinline__ int pieces(int n) const { return (n + share - 1) / share; }
-  __device__ __forceinline__ int span(int n) const { return apart ? pieces(n) * share : n; }
+  __device__ __forceinline__ int span(int n) const { return n == 0 ? 0 : apart ? pieces(n) * share : n + begin; }
 };
 template <int KEYS>
 __device__ __forceinline__ Shares shares_of(const TreeArgs& a, int lane) {
@@ -240,7 +241,14 @@ __device__ __forceinline__ Shares shares_of(const TreeArgs& a, int lane) {
   for (int b0 = 64; b0 < a.B; b0 += 64)
     pieces += last_lane(wave_scan(s.pieces(steps_at<KEYS>(a, b0 + lane, pos_of(a, b0 + lane)))));
   s.apart = (int64_t)pieces * per_seq <= a.groups;
-  if (s.apart) s.upto = upto * s.share;
+  if (s.apart) {
+    s.begin = 0;
+    s.upto = upto * s.share;
+  } else {
+    s.begin = a.begin;
+    s.upto += min(lane + 1, a.B) * a.begin;
+    s.share = __builtin_amdgcn_readfirstlane(max(((total + a.B * a.begin) * per_seq + a.groups - 1) / a.groups, a.least));
+  }
   return s;
 }
 
@@ -254,7 +262,7 @@ struct Cursor {
   __device__ __forceinline__ bool start(const TreeArgs& a, int lane) {
     const int per_seq = a.Hkv * a.row_groups;
     int seq_at = 0;  // where on the line the sequence begins
-    sh = Shares{1, false, 0, 0, 0};
+    sh = Shares{1, 0, false, 0, 0, 0};
     if (a.part) {
       sh = shares_of<KEYS>(a, lane);
       cur = (int)blockIdx.x * sh.share;
@@ -290,13 +298,17 @@ struct Cursor {
     end = __builtin_amdgcn_readfirstlane(end);
     const int at = cur - __builtin_amdgcn_readfirstlane(seq_at), span = __builtin_amdgcn_readfirstlane(sh.span(steps));
     hr = __builtin_amdgcn_readfirstlane(at / span);
-    s0 = at - hr * span;
-    return true;
+    s0 = at - hr * span - sh.begin;
+    if (s0 < 0) {
+      cur -= s0;
+      s0 = 0;
+    }
+    return cur < end;
   }
   __device__ __forceinline__ int s1() const { return min(steps, s0 + end - cur); }
   // To the next (head, row group); false: none left.
   __device__ __forceinline__ bool next(const TreeArgs& a) {
-    cur += steps - s0;  // of shares that stand apart there is no next
+    cur += steps - s0 + sh.begin;  // of shares that stand apart there is no next
     if (sh.apart || cur >= end) return false;
     s0 = 0;
     if (++hr == a.Hkv * a.row_groups) {
@@ -325,7 +337,7 @@ __device__ __forceinline__ f32x4 not_finite_of(const TreeArgs& a, int b, const T
   return x;
 }
 
-// Slots of `rows` rows: (m, l) of each, then the unnormalised outputs.
+// Slots of `rows` rows, two to a workgroup, the second for a first piece of a (head, row group): (m, l) of each, then the unnormalised outputs.
 struct Parts {
   f32x2* ml;   // [slots, rows]
   float* acc;  // [slots, rows, D]
@@ -350,6 +362,31 @@ template <typename T, int D, int NT, int W>
 constexpr int kTreeLds = std::max(kQueriesInLds<T, D, NT> ? NT * (D * (int)sizeof(T) / 64) * 1024 : 0,
                                   W * NT * 16 * (D + 4 + 2) * 4);
 
+// The nodes' rows of the cache, from element `at` of it, by the workgroup that has the first step of nodes of the head's first
+// rows: behind the steps, when those rows are in the L2, where all other waits are over.
+template <typename T, int D, int W>
+__device__ __forceinline__ void write_nodes(const TreeArgs& a, const T* kn, const T* vn, int64_t at, uint64_t there) {
+  constexpr int VEC = D * (int)sizeof(T) / 16, N = 4;
+  u32x4* const kc = reinterpret_cast<u32x4*>(static_cast<T*>(a.kc) + at);
+  u32x4* const vc = reinterpret_cast<u32x4*>(static_cast<T*>(a.vc) + at);
+  for (int e0 = threadIdx.x; e0 < a.T * VEC; e0 += N * 64 * W) {
+    u32x4 xk[N], xv[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int e = min(e0 + u * 64 * W, a.T * VEC - 1);
+      xk[u] = reinterpret_cast<const u32x4*>(kn + e / VEC * a.ks[2])[e % VEC];
+      xv[u] = reinterpret_cast<const u32x4*>(vn + e / VEC * a.vs[2])[e % VEC];
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int e = e0 + u * 64 * W;
+      if (e >= a.T * VEC || !(there >> (e / VEC) & 1)) continue;
+      kc[e] = xk[u];
+      vc[e] = xv[u];
+    }
+  }
+}
+
 // A row group of 16 NT rows, its steps dealt to W waves.
 template <typename T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
@@ -364,7 +401,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, q0 = lane & 15;
   Cursor<KEYS> at;
   if (!at.start(a, lane)) return;
-  int slot = 2 * (int)blockIdx.x;
   do {
     // readfirstlane: descriptors must be provably uniform, or every load becomes a loop over the lanes' distinct ones.
     const int b = __builtin_amdgcn_readfirstlane(at.b), p = __builtin_amdgcn_readfirstlane(at.p);
@@ -533,27 +569,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
       }
     }
 
-    // The nodes' rows of the cache, by the workgroup that has the first step of nodes of the head's first rows.
-    if (drafts && s0 <= cached_steps && row0 == 0) {
-      constexpr int VEC = S::RB / 16, N = 4;
-      for (int e0 = threadIdx.x; e0 < a.T * VEC; e0 += N * 64 * W) {
-        u32x4 xk[N], xv[N];
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-          const int e = min(e0 + u * 64 * W, a.T * VEC - 1);
-          xk[u] = reinterpret_cast<const u32x4*>(kn + e / VEC * a.ks[2])[e % VEC];
-          xv[u] = reinterpret_cast<const u32x4*>(vn + e / VEC * a.vs[2])[e % VEC];
-        }
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-          const int e = e0 + u * 64 * W;
-          if (e >= a.T * VEC || !(there >> (e / VEC) & 1)) continue;
-          const int64_t row = (base + (int64_t)p * D) / (16 / (int)sizeof(T)) + e;
-          static_cast<u32x4*>(a.kc)[row] = xk[u];
-          static_cast<u32x4*>(a.vc)[row] = xv[u];
-        }
-      }
-    }
+    if (drafts && s0 <= cached_steps && row0 == 0) write_nodes<T, D, W>(a, kn, vn, base + (int64_t)p * D, there);
 
     // The waves' states through LDS: weights 2^(m_w - max), then the sums over the waves of a row block in their order, to the
     // output or to this workgroup's slot.
@@ -609,14 +625,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
         else
           *reinterpret_cast<f32x4*>(out) = f32x4{y[0], y[1], y[2], y[3]};
       } else {
-        const int64_t i = (int64_t)slot * ROWS + r;
+        const int64_t i = (2 * (int64_t)blockIdx.x + (s0 == 0)) * ROWS + r;
         *reinterpret_cast<f32x4*>(parts.acc + i * D + d) = sum;
         if (d == 0) parts.ml[i] = f32x2{mx, lsum};
       }
     }
     __syncthreads();
 
-    slot = 2 * (int)blockIdx.x + 1;  // what it shares comes first or last
   } while (at.next(a));
 }
 
@@ -648,7 +663,6 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, q0 = lane & 31;
   Cursor<KEYS> at;
   if (!at.start(a, lane)) return;
-  int slot = 2 * (int)blockIdx.x;
   do {
     // readfirstlane: descriptors must be provably uniform, or every load becomes a loop over the lanes' distinct ones.
     const int b = __builtin_amdgcn_readfirstlane(at.b), p = __builtin_amdgcn_readfirstlane(at.p);
@@ -679,16 +693,6 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       line = ancestors(lane < a.T ? parent : -2, lane);
       there = __ballot(line != 0);
       line = __shfl((unsigned long long)line, node, kWave);
-    }
-    // The nodes' rows of the cache, by the workgroup that has the first step of nodes of the head's first rows.
-    if (drafts && s0 <= cached_steps && row0 == 0) {
-      for (int e = threadIdx.x; e < a.T * C::PIECES; e += 64 * W) {
-        const int t = e / C::PIECES, c = e % C::PIECES;
-        if (!(there >> t & 1)) continue;
-        const int64_t row = (base + (int64_t)p * D) / 8 + e;
-        static_cast<u32x4*>(a.kc)[row] = reinterpret_cast<const u32x4*>(kn + t * a.ks[2])[c];
-        static_cast<u32x4*>(a.vc)[row] = reinterpret_cast<const u32x4*>(vn + t * a.vs[2])[c];
-      }
     }
     // Step `s` into its stage; one past the last from past every range, so that the copies under way can be counted.
     auto copy = [&](int s) {
@@ -879,6 +883,7 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
     odd_values = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) odd_values |= reinterpret_cast<const int*>(red)[w * 32 * (D + 4) + D + 2];
+    if (drafts && s0 <= cached_steps && row0 == 0) write_nodes<bf16, D, W>(a, kn, vn, base + (int64_t)p * D, there);
     const bool whole = s0 == 0 && s1 == at.steps;
     const Parts parts = parts_of(a.part, 2 * (int64_t)a.groups, ROWS);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * W) {
@@ -897,13 +902,12 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         for (int i = 0; i < 4; ++i) y[i] = !valid ? NAN : zero ? 0.f : sum[i] / ml[1];
         *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
       } else {
-        const int64_t i = (int64_t)slot * ROWS + r;
+        const int64_t i = (2 * (int64_t)blockIdx.x + (s0 == 0)) * ROWS + r;
         *reinterpret_cast<f32x4*>(parts.acc + i * D + d) = sum;
         if (d == 0) parts.ml[i] = ml;
       }
     }
     __syncthreads();
-    slot = 2 * (int)blockIdx.x + 1;  // what it shares comes first or last
   } while (at.next(a));
 }
 
@@ -924,7 +928,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
   for (int b0 = 0; b0 < b; b0 += 64)
     before += last_lane(wave_scan(b0 + lane < b ? sh.span(steps_at<KEYS>(a, b0 + lane, b0 ? pos_of(a, b0 + lane) : sh.p)) : 0));
   const int share = sh.share, steps = steps_at<KEYS>(a, b, p);
-  const int x0 = before * per_seq + (h * a.row_groups + block / slot_rows) * sh.span(steps);
+  const int x0 = before * per_seq + (h * a.row_groups + block / slot_rows) * sh.span(steps) + sh.begin;
   const int w0 = x0 / share, used = (x0 + steps - 1) / share - w0 + 1;
   if (used == 1) return;  // one workgroup had it all
   const uint64_t there = __ballot(ancestors(parent, lane) != 0);  // divided: the sequence has its place
@@ -932,7 +936,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
   const int to = min(block + kJoinRows<D, LINES>, a.rows);
   for (int r0 = block; r0 < to; r0 += ROWS) {
     const int r = min(r0 + row, to - 1);
-    auto at = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 && x0 != w0 * share)) * slot_rows + r % slot_rows; };
+    auto at = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0)) * slot_rows + r % slot_rows; };
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int c = part; c < used; c += N * LINES) {
@@ -997,7 +1001,7 @@ constexpr int64_t kMostSteps = 1 << 30;
 struct Plan {
   bool wide;
   int tiles, waves;  // of tree_attn_kernel
-  int64_t keys, slot_rows, row_groups, groups, least;
+  int64_t keys, slot_rows, row_groups, groups, least, begin;
   bool split;
 };
 
@@ -1017,6 +1021,10 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   const int per_cu = p.wide ? 1 : p.tiles == 1 ? (d == 64 ? 3 : d == 128 ? 2 : 1) : p.tiles == 2 && d == 64 ? 2 : 1;
   p.groups = 256 * per_cu;
   p.least = p.wide ? 2 : p.waves;
+  // A wide head takes some 12 us to begin and to store, and a step 1.9 (16 sequences of 1008 to 4032 keys, 8 heads each, 256
+  // rows: 77 us; with 0 it takes 90, with 4 or 8 80); else it is about a step of each wave (eight heads of 1024 keys 12.3 us and
+  // 14.3 with 0, f32, four nodes of four heads to each of 16 heads 33.4 and 44.3, and none slower).
+  p.begin = p.wide ? 6 : p.waves;
   const bool eight = !p.wide && p.tiles == 1 && d <= 128;
   // Whole heads need no second kernel. Short ones, or many, lose less by uneven shares than that one costs: 256 heads of 1024
   // keys of 128 elements take 23.2 us whole and 26.4 cut (f32 46.1 and 47.4), 512 of 64 elements 19.3 and 25.9; but 32 of
@@ -1081,7 +1089,7 @@ int check_tree(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, in
     return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": need max_len >= 1, and a head's cache within 4 GiB less 128 KiB");
   // Places on the line of steps are 32-bit numbers.
   const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
-  if (b * hkv * p.row_groups > kMostSteps / 512 || b * hkv * p.row_groups * (cdiv(max_len, 16) + 4) > kMostSteps)
+  if (b * hkv * p.row_groups > kMostSteps / 512 || b * hkv * p.row_groups * (cdiv(max_len, 16) + 64) > kMostSteps)
     return fail(FERRITE_ERR_INVALID_ARGUMENT, n + ": too many heads for caches of this length");
   return FERRITE_OK;
 }
@@ -1117,7 +1125,7 @@ extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new,
       return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: a head's new keys or values span 4 GiB");
   const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
   TreeArgs a{q, k_new, v_new, k_cache, v_cache, pos, parents, out, nullptr, {}, {}, {}, (int)b, (int)h, (int)hkv, (int)(h / hkv),
-             (int)t, (int)max_len, (int)(h / hkv * t), (int)p.row_groups, (int)p.groups, (int)p.least,
+             (int)t, (int)max_len, (int)(h / hkv * t), (int)p.row_groups, (int)p.groups, (int)p.least, (int)p.begin,
              std::max(fabsf(scale) * kLog2e, 1e-37f),  // above 0, so that it times -inf is -inf
              scale >= 0 ? 0u : dtype == FERRITE_BF16 ? 0x80008000u : 0x80000000u};
   for (int i = 0; i < 3; ++i) {
