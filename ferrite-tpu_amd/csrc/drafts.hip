@@ -34,51 +34,63 @@ __device__ __forceinline__ int64_t index_of(uint64_t key) { return 0xffffffffu -
 template <typename T>
 __device__ __forceinline__ float elem_of(const u32x4& raw, int e) {
   if constexpr (sizeof(T) == 2)
-    return (float)__builtin_bit_cast(bf16x8, raw)[e];
+    return __uint_as_float(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
   else
     return __builtin_bit_cast(f32x4, raw)[e];
 }
 
-// The largest key of x[from, to) that thread t of n threads sees. Vectors of 16 bytes between the first and the
-// last 16-byte boundary; every value of a thread comes later than its last one.
-template <typename T>
-__device__ __forceinline__ uint64_t best_of(const T* x, int64_t from, int64_t to, int t, int n) {
-  constexpr int V = 16 / sizeof(T), BATCH = 4;
-  uint32_t best = 0;
-  int64_t at = from;
-  auto one = [&](int64_t i) {
-    const uint32_t o = order_of(Elem<T>::to_f32(x[i]));
-    if (o > best) {
-      best = o;
-      at = i;
-    }
-  };
-  const int64_t lead = ((16 - (reinterpret_cast<uintptr_t>(x + from) & 15)) & 15) / sizeof(T);
-  const int64_t first = min(from + lead, to), vecs = (to - first) / V;
-  if (from + t < first) one(from + t);
-  const u32x4* v = reinterpret_cast<const u32x4*>(x + first);
-  auto many = [&](const u32x4& raw, int64_t i) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const uint32_t o = order_of(elem_of<T>(raw, e));
-      if (o > best) {
-        best = o;
-        at = first + i * V + e;
-      }
-    }
-  };
-  int64_t i = t;
-  for (; i + (BATCH - 1) * n < vecs; i += BATCH * n) {
+// The largest key of vectors t, t + n, .. of v (element 0 is x[first]), BATCH under way. Past the end the last one is read again:
+// loads behind branches of their own would be waited for one by one. Numbers are compared as they are (three operations a
+// value; orders take ten, which the reads of long rows do not hide): NaN, for which no comparison holds, is looked for
+// alongside, and a thread that has one goes over its values again.
+template <typename T, int BATCH>
+__device__ __forceinline__ uint64_t best_vector(const u32x4* v, int64_t first, int64_t vecs, int t, int n) {
+  constexpr int V = 16 / sizeof(T);
+  if (t >= vecs) return 0;
+  float best = -INFINITY;
+  int64_t at = first + (int64_t)t * V;
+  bool nan = false;
+  for (int64_t i = t; i < vecs; i += BATCH * n) {
     u32x4 raw[BATCH];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) raw[u] = __builtin_nontemporal_load(v + i + u * n);
+    for (int u = 0; u < BATCH; ++u) raw[u] = __builtin_nontemporal_load(v + min(i + u * n, vecs - 1));
+    int found = -1;  // of equal ones the first: a thread's values come in order
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) many(raw[u], i + u * n);
+    for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x = elem_of<T>(raw[u], e);
+        nan |= x != x;
+        if (x > best) {
+          best = x;
+          found = u * V + e;
+        }
+      }
+    if (found >= 0) at = first + min(i + found / V * n, vecs - 1) * V + found % V;
   }
-  for (; i < vecs; i += n) many(__builtin_nontemporal_load(v + i), i);
-  const int64_t tail = first + vecs * V + t;
-  if (tail < to) one(tail);
-  return key_of(best, at);
+  uint64_t k = key_of(order_of(best), at);
+  if (nan)
+    for (int64_t i = t; i < vecs; i += n) {
+      const u32x4 raw = v[i];
+#pragma unroll
+      for (int e = 0; e < V; ++e) k = max(k, key_of(order_of(elem_of<T>(raw, e)), first + i * V + e));
+    }
+  return k;
+}
+
+// The largest key of x[from, to), not empty, that thread t of n threads sees: vectors of 16 bytes between the first and the last
+// 16-byte boundary, and an element before and behind them, whose loads go out first.
+template <typename T>
+__device__ __forceinline__ uint64_t best_of(const T* x, int64_t from, int64_t to, int t, int n) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t lead = ((16 - (reinterpret_cast<uintptr_t>(x + from) & 15)) & 15) / sizeof(T);
+  const int64_t first = min(from + lead, to), vecs = (to - first) / V, tail = first + vecs * V + t;
+  const float head_x = Elem<T>::to_f32(x[min(from + t, to - 1)]), tail_x = Elem<T>::to_f32(x[min(tail, to - 1)]);
+  const u32x4* v = reinterpret_cast<const u32x4*>(x + first);
+  uint64_t k = vecs <= n ? best_vector<T, 1>(v, first, vecs, t, n) : best_vector<T, 4>(v, first, vecs, t, n);
+  if (from + t < first) k = max(k, key_of(order_of(head_x), from + t));
+  if (tail < to) k = max(k, key_of(order_of(tail_x), tail));
+  return k;
 }
 
 __device__ __forceinline__ uint64_t wave_best(uint64_t k) {
@@ -166,12 +178,17 @@ __global__ __launch_bounds__(1024) void accept_walk_kernel(const uint64_t* __res
   if (threadIdx.x < 64) walk(target, tokens, parents, path, count, following, b, t);
 }
 
-// A row of up to kShortRow values is read by one wave of its sequence's workgroup; longer ones are cut into pieces
-// over the chip.
-constexpr int64_t kShortRow = 2048, kPiece = 4096;
+// Whether one workgroup walks a sequence's rows, a wave to each, or they are cut into pieces over the chip and walked by a second
+// kernel. One: 8 rows of 4096 floats 6.6 us and not 9.4, of 8192 bf16 7.6 and not 9.3; 32 rows (two to a wave) of 2048 floats
+// 6.5 and 10.1; 64 of 1024 8.0 and 10.3 (bf16 12.1 and 10.5). Two: 32 rows of 4096 9.1 us and not 10.7, 64 of 2048 10.3 and
+// 10.6 (bf16 10.5 and 13.2), of 4096 9.3 and 20.8.
+bool short_rows(int64_t t, int64_t v) { return v <= (t <= 16 ? 8192 : 4096 / cdiv(t, 16)); }
+// Pieces of a row: small ones, so that the chip stays full to the end (16 sequences of up to 32 rows of 50257 floats:
+// 14.1 us, 5.5 TB/s with the launch; pieces of 8192 14.7, of 16384 17.0), but no more than 8192 workgroups of them.
+constexpr int64_t kPiece = 4096;
 int64_t piece_of(int64_t rows, int64_t v) {
   int64_t piece = kPiece;
-  while (piece < v && rows * cdiv(v, piece) > 4096) piece *= 2;
+  while (piece < v && rows * cdiv(v, piece) > 8192) piece *= 2;
   return piece;
 }
 
@@ -221,7 +238,7 @@ __global__ __launch_bounds__(256) void compact_kernel(U* __restrict__ k_cache, U
 extern "C" int64_t ferrite_internal_accept_drafts_workspace(int64_t b, int64_t t, int64_t v) {
   using namespace ferrite;
   if (b < 0 || t < 1 || t > kMaxNodes || v < 1 || v > 0x7fffffff || b > 65535 / t) return -1;
-  return v <= kShortRow ? 0 : b * t * cdiv(v, piece_of(b * t, v)) * (int64_t)sizeof(uint64_t);
+  return short_rows(t, v) ? 0 : b * t * cdiv(v, piece_of(b * t, v)) * (int64_t)sizeof(uint64_t);
 }
 
 extern "C" int ferrite_internal_accept_drafts(const void* logits, const int64_t* tokens, const int32_t* parents,
