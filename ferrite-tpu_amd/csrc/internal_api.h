@@ -104,7 +104,10 @@ int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64
  * and its output is zero. Where pos[b] < 0 or pos[b] + T > max_len nothing is written and the sequence's outputs are NaN. q [B, H, T, D],
  * k_new and v_new [B, Hkv, T, D] with dense last dimensions and the nine element strides (sequence, head, node of
  * each; whole 16 bytes); out [B, T, H, D], dense. H is a multiple of Hkv. The workspace, 16-byte aligned, has
- * ferrite_internal_tree_attention_workspace(...) bytes (-1: sizes out of range); its content need not survive the call.
+ * ferrite_internal_tree_attention_workspace(...) bytes (-1: sizes out of range); its content need not survive the call. A head's
+ * cached keys, and its nodes' rows with what lies between them, take at most 4 GiB less 128 KiB. A node's values that are not
+ * finite reach only the rows that see it. How the sums are parted depends on the sizes and positions of the whole batch, so a
+ * sequence's last bits may differ from batch to batch; for the same call they are the same.
  */
 int64_t ferrite_internal_tree_attention_workspace(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d,
                                                   int dtype);

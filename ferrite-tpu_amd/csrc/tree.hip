@@ -136,6 +136,8 @@ struct Step {
 };
 
 // O^T += V^T P^T; o[j] row i stands for element i D / 16 + j.
+// The weights are rounded to bf16 for the bf16 product (half a step, 2^-9 of each, errors apart from one another; m and l, and what
+// is summed to l, stay f32): with f32 values the products would run at a sixteenth of the rate.
 template <int D>
 __device__ __forceinline__ void add_pv(const Step<bf16, D>& st, const f32x4 (&p)[2], f32x4 (&o)[D / 16]) {
   const u32x4 b = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
@@ -387,7 +389,10 @@ __device__ __forceinline__ void write_nodes(const TreeArgs& a, const T* kn, cons
   }
 }
 
-// A row group of 16 NT rows, its steps dealt to W waves.
+// A row group of 16 NT rows, its steps dealt to W waves. Long caches: bound by HBM (8 sequences of 5 to 8 thousand keys, 32 heads of
+// 128, 4 nodes, bf16: 103 us, 6.5 TB/s; two steps of 16 KB are under way in each of 8 waves a CU). Short ones: by the
+// chain of round trips (position, parents and rows, keys, LDS, store): 4 heads of 512 keys 10.5 us. f32 rows past 16: by the f32
+// matrix rate beside the loads (3 sequences of 3000 keys, 39 rows: 12.4 us).
 template <typename T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
   typedef Step<T, D> S;
@@ -642,7 +647,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 //
 // A step is two clusters, the softmax of its scores (VALU) and its product with V and the next step's with K (matrix units), each
 // behind a barrier, and the second half of the waves is one cluster behind the first: of a SIMD's two waves one is on the
-// VALU while the other is on the matrix units.
+// VALU while the other is on the matrix units. Bound by LDS: a step's keys and values are read by all eight waves, 256 KB at
+// 128 bytes a clock and more for the transposing reads, some 3500 of its 4400 cycles (1.9 us); the products take 2000. 64 rows to a
+// wave would halve that and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of 1008 to 4032
+// keys, 8 key heads of 128, 256 rows each: 75 us, 34 GFLOP of nodes that are there in 54 of products.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
@@ -1009,7 +1017,10 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   const bool half = dtype == FERRITE_BF16;
   const int64_t rows = h / hkv * t;
   Plan p;
-  p.wide = half && rows > (d == 256 ? 32 : 64);
+  // Many rows share keys and values through LDS: 8 sequences of 4096 keys, 4 key heads of 128, 48 rows each 25.8 us and not 27.5,
+  // 64 rows 26.7 and 29.9, 96 rows 30.3 and 43.2; of 64 elements 64 rows 19.4 and 18.3, 96 rows 21.1 and 24.8; of 256
+  // elements 24 and 32 rows 36.6 and 37.7 against 32.9 and 35.0, 48 rows 41.6 and 52.8.
+  p.wide = half && rows > (d == 64 ? 64 : 32);
   p.tiles = rows <= 16 ? 1 : rows <= 32 || d > 128 ? 2 : 4;
   p.waves = 4;
   p.keys = p.wide ? (d == 256 ? 32 : 64) : half ? 32 : 16;
@@ -1050,8 +1061,11 @@ int tree_finish(const TreeArgs& a, const Plan& p, hipStream_t s) {
                        dim3((unsigned)cdiv(a.rows, kJoinRows<D, lines.value>), (unsigned)a.Hkv, (unsigned)a.B), dim3(256), 0, s, a,
                        (int)p.slot_rows);
   };
-  // Few heads are cut into many pieces.
-  if (p.groups >= 8 * (int64_t)a.B * a.Hkv * a.row_groups)
+  // Few heads are cut into many pieces, and four lines add up a row's: one head of 64 rows, 8192 keys 20.2 us and not 34.3, eight of
+  // 8 rows, 4096 keys 12.9 and 15.1; of many rows there are lines enough (32 heads of 96 rows 30.3 us and 29.0, of 128 rows 32.6
+  // and 30.2).
+  const int64_t heads = (int64_t)a.B * a.Hkv;
+  if (p.groups >= 8 * heads * a.row_groups && heads * a.rows <= 2048)
     join(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
   else
     join(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
@@ -1146,6 +1160,8 @@ extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new,
     }
     if constexpr (D.value <= 128) {
       if (p.waves == 8) return tree_launch<T, D.value, 1, 8>(a, p, s);
+    }
+    if constexpr (D.value == 64 || (D.value == 128 && sizeof(T) == 4)) {
       if (p.tiles == 4) return tree_launch<T, D.value, 4, 4>(a, p, s);
     }
     if (p.tiles == 1) return tree_launch<T, D.value, 1, 4>(a, p, s);
