@@ -650,7 +650,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 // VALU while the other is on the matrix units. Bound by LDS: a step's keys and values are read by all eight waves, 256 KB at
 // 128 bytes a clock and more for the transposing reads, some 3500 of its 4400 cycles (1.9 us); the products take 2000. 64 rows to a
 // wave would halve that and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of 1008 to 4032
-// keys, 8 key heads of 128, 256 rows each: 75 us, 34 GFLOP of nodes that are there in 54 of products.
+// keys, 8 key heads of 128, 256 rows each: 74 us, 34 GFLOP of nodes that are there in 54 of products.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
@@ -790,6 +790,7 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         clean(s + 1);
       }
       lds_barrier();
+      __builtin_amdgcn_s_setprio(0);
       u32x4 pb[KEYS / 16];
       if (mine) {
         if (s >= whole_to) {  // not every row sees every key: bit k of `sees` is the step's key k
@@ -838,9 +839,9 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       if (!mine) continue;
       // The scores of the next step (behind the last one of zeros, for nothing), then O: reads from LDS are kept AHEAD products
       // ahead of the one that they feed, in this order (a read's latency is some six products; left to itself the compiler has
-      // every product wait for its own read).
+      // every product wait for its own read). The kernel's fastest run takes 70.4 us with 4 and 6, 72.2 with 8, 76 with 10.
       const char *ks = lds + (s + 1 - s0) % 4 * C::STAGE, *vs = lds + (s - s0) % 4 * C::STAGE;
-      constexpr int QK = NT * D / 16, ALL = QK + KEYS / 16 * D / 32, AHEAD = 8;
+      constexpr int QK = NT * D / 16, ALL = QK + KEYS / 16 * D / 32, AHEAD = 6;
       auto fetch = [&](int i) {
         if (i < QK) return *reinterpret_cast<const bf16x8*>(ks + koff[i / NT] + i % NT * 32 * RB);
         typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
@@ -853,6 +854,7 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
         typedef short i16x8 __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(bf16x8, i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
       };
+      __builtin_amdgcn_s_setprio(1);  // before the SIMD's other wave, whose softmax waits for no one
       bf16x8 ring[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) ring[i] = fetch(i);
