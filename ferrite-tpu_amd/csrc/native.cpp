@@ -53,6 +53,25 @@ bool records(std::initializer_list<const Tensor*> inputs) {
     if (t->requires_grad()) return true;
   return false;
 }
+// A leaf's gradient is added up on the stream where the graph that first took the leaf was made, for as long as that graph lives. While
+// it is a stream outside the current capture, a backward pass captured here would run work there and end the process:
+// refused where the pass would begin.
+void refuse_leaves_of_other_graphs(std::initializer_list<const Tensor*> inputs, const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : inputs) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (!stream || stream->id() == c10::hip::getCurrentHIPStream(t->device().index()).id()) continue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (stream->id() != 0 &&
+        hipStreamIsCapturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *stream).stream(), &status) == hipSuccess &&
+        status == hipStreamCaptureStatusActive)
+      continue;
+    throw std::runtime_error(std::string(what) + ": a graph made outside this capture still holds one of its leaves; "
+                             "drop that graph's outputs before capturing a pass that records a backward");
+  }
+}
 // Rows of a [..., last] tensor.
 int64_t rows_of(const Tensor& t) {
   if (t.dim() < 1 || t.size(-1) == 0) throw std::runtime_error("ferrite's kernels need a non-empty last dimension");
@@ -326,8 +345,9 @@ std::tuple<Tensor, Tensor, Tensor> qk_norm_rope(const Tensor& qkv0, const Tensor
   Tensor pos;
   if (pos0) pos = pos0->expand({qkv.size(0), qkv.size(1)}).contiguous();
   const HeadsOptions o{h, hkv, eps, interleaved, pos};
-  const auto out =
-      records({&qkv, &wq, &wk}) ? HeadsFn::apply(qkv, wq, wk, cos, sin, o) : heads_forward(qkv, wq, wk, cos, sin, o);
+  const bool record = records({&qkv, &wq, &wk});
+  if (record) refuse_leaves_of_other_graphs({&qkv0, &wq0, &wk0}, "ferrite_qk_norm_rope");
+  const auto out = record ? HeadsFn::apply(qkv, wq, wk, cos, sin, o) : heads_forward(qkv, wq, wk, cos, sin, o);
   return {out[0], out[1], out[2]};
 }
 

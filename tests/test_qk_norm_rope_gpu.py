@@ -249,6 +249,48 @@ def test_streams_and_graph(dev):
     graph.reset()
 
 
+@pytest.mark.parametrize("rows", [16, 32])
+def test_capture_refuses_leaves_that_an_eager_graph_holds(dev, rows):
+    """While an eager graph of the leaves lives, no pass that records a backward begins in a capture; once it is dropped,
+    one that takes the leaves twice does, and its backward() replays as it runs. Of 16 rows the tables are too short for
+    some of the second call's positions: NaN in their gradients and the weights'."""
+    qkv, wq, wk, cos, sin = _inputs(dev, 2, 16, 4, 4, 64, 64, F32, rows=rows)
+    leaves = [t.requires_grad_() for t in (qkv, wq, wk)]
+    for t in leaves:
+        t.grad = torch.zeros_like(t)
+
+    def step():
+        for t in leaves:
+            t.grad.zero_()
+        outs = [o for p in places for o in qk_norm_rope(*leaves, cos, sin, n_head=4, positions=p)]
+        torch.autograd.backward(outs, grads)
+
+    grads = [torch.randn(2, 4, 16, 64, device=dev) for _ in range(6)]
+    places = [torch.arange(16, dtype=torch.int32, device=dev), torch.arange(16, dtype=torch.int32, device=dev) + 7]
+    step()
+    want = [t.grad.clone() for t in leaves]
+    assert bool(torch.isnan(want[1]).any()) == (rows == 16) and not bool(torch.isnan(want[0]).all())
+    alive = qk_norm_rope(*leaves, cos, sin, n_head=4)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(graph):
+            qk_norm_rope(*leaves, cos, sin, n_head=4)
+    with torch.no_grad():
+        assert torch.equal(qk_norm_rope(*leaves, cos, sin, n_head=4)[0], alive[0])
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        for t in leaves:
+            t.grad.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t.grad.nan_to_num(7), w.nan_to_num(7)) for t, w in zip(leaves, want))
+    graph.reset()
+
+
 def test_feeds_attention_like_split_heads(dev):
     """With unit weights' norm undone the heads are split_heads'; and the outputs go straight into flash attention."""
     qkv, wq, wk, cos, sin = _inputs(dev, 2, 128, 4, 4, 64, 64, BF16)
