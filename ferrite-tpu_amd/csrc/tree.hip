@@ -647,10 +647,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 //
 // A step is two clusters, the softmax of its scores (VALU) and its product with V and the next step's with K (matrix units), each
 // behind a barrier, and the second half of the waves is one cluster behind the first: of a SIMD's two waves one is on the
-// VALU while the other is on the matrix units. Bound by LDS: a step's keys and values are read by all eight waves, 256 KB at
-// 128 bytes a clock and more for the transposing reads, some 3500 of its 4400 cycles (1.9 us); the products take 2000. 64 rows to a
-// wave would halve that and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of 1008 to 4032
-// keys, 8 key heads of 128, 256 rows each: 74 us, 34 GFLOP of nodes that are there in 54 of products.
+// VALU while the other is on the matrix units. Bound by LDS: a step's keys and values are read by all eight waves, 128 KB of
+// each, at 128 bytes a clock and the transposing reads at 64: some 3100 of a step's 4300 cycles (1.8 us); the products take 2000.
+// 64 rows to a wave would halve that and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of 1008
+// to 4032 keys, 8 key heads of 128, 256 rows each: 73 us, 34 GFLOP of nodes that are there in 54 of products.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
@@ -1042,6 +1042,7 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   // Whole heads need no second kernel. Short ones, or many, lose less by uneven shares than that one costs: 256 heads of 1024
   // keys of 128 elements take 23.2 us whole and 26.4 cut (f32 46.1 and 47.4), 512 of 64 elements 19.3 and 25.9; but 32 of
   // 128 elements 18.5 whole and 11.3 cut, 128 of them 20.5 and 16.2, f32 64 of 512 keys 24.2 and 16.2.
+  // More heads than fill the chip four times are whole too: 2048 heads of 4096 keys 625 us, cut 668; of 8192 1218 and 1284.
   p.split = heads < 4 * p.groups && steps > (p.wide ? 8 : heads >= 256 ? 128 : eight ? 32 : 16);
   if (p.split) {
     p.groups = std::min(p.groups, cdiv(heads * steps, p.least));
