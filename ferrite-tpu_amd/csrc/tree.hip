@@ -136,7 +136,7 @@ struct Step {
 };
 
 // O^T += V^T P^T; o[j] row i stands for element i D / 16 + j.
-// The weights are rounded to bf16 for the bf16 product (half a step, 2^-9 of each, errors apart from one another; m and l, and what
+// The weights are rounded to bf16 for the bf16 product (at most 2^-8 of each, errors apart from one another; m and l, and what
 // is summed to l, stay f32): with f32 values the products would run at a sixteenth of the rate.
 template <int D>
 __device__ __forceinline__ void add_pv(const Step<bf16, D>& st, const f32x4 (&p)[2], f32x4 (&o)[D / 16]) {
@@ -389,10 +389,10 @@ __device__ __forceinline__ void write_nodes(const TreeArgs& a, const T* kn, cons
   }
 }
 
-// A row group of 16 NT rows, its steps dealt to W waves. Long caches: bound by HBM (8 sequences of 5 to 8 thousand keys, 32 heads of
+// A row group of 16 NT rows, its steps dealt to W waves. Long caches: bound by HBM (8 sequences of 2047 to 8188 keys, 32 heads of
 // 128, 4 nodes, bf16: 103 us, 6.5 TB/s; two steps of 16 KB are under way in each of 8 waves a CU). Short ones: by the
 // chain of round trips (position, parents and rows, keys, LDS, store): 4 heads of 512 keys 10.5 us. f32 rows past 16: by the f32
-// matrix rate beside the loads (3 sequences of 3000 keys, 39 rows: 12.4 us).
+// matrix rate beside the loads (sequences of 747, 1868 and 2988 keys, 39 rows: 12.4 us).
 template <typename T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
   typedef Step<T, D> S;
