@@ -391,8 +391,8 @@ __device__ __forceinline__ void write_nodes(const TreeArgs& a, const T* kn, cons
 
 // A row group of 16 NT rows, its steps dealt to W waves. Long caches: bound by HBM (8 sequences of 2047 to 8188 keys, 32 heads of
 // 128, 4 nodes, bf16: 103 us, 6.5 TB/s; two steps of 16 KB are under way in each of 8 waves a CU). Short ones: by the
-// chain of round trips (position, parents and rows, keys, LDS, store): 4 heads of 512 keys 10.5 us. f32 rows past 16: by the f32
-// matrix rate beside the loads (sequences of 747, 1868 and 2988 keys, 39 rows: 12.4 us).
+// chain of round trips (position, parents and rows, keys, LDS, store): 4 heads of 512 keys 10.5 us, and f32 (a wave has
+// a step or two) 39 rows for each of 2 heads of 64 over 747, 1868 and 2988 keys 12.4 us.
 template <typename T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
   typedef Step<T, D> S;
