@@ -135,20 +135,38 @@ struct Step {
   }
 };
 
+// Two weights as bf16 pairs that together are within 2^-16 of each: `high`, the bits of a float below the weight cut to bf16, and
+// the rest of the weight (exact in f32), rounded. A weight's one rounding to bf16 would be off by up to 2^-8, and keys of one score
+// would all be off by the same, while l sums the weights as they are. `high` is less than the weight, so the rest is 0 for a weight of 0
+// alone, and an infinite value times both stays what it is times the weight.
+struct WeightPair {
+  uint32_t high, rest;
+};
+__device__ __forceinline__ WeightPair split_weights(float a, float b) {
+  const uint32_t x = __builtin_elementwise_sub_sat(__float_as_uint(a), 1u), y = __builtin_elementwise_sub_sat(__float_as_uint(b), 1u);
+  return {__builtin_amdgcn_perm(y, x, 0x07060302u),
+          pack_bf16(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u))};
+}
+
 // O^T += V^T P^T; o[j] row i stands for element i D / 16 + j.
-// The weights are rounded to bf16 for the bf16 product (at most 2^-8 of each, errors apart from one another; m and l, and what
-// is summed to l, stay f32): with f32 values the products would run at a sixteenth of the rate.
+// bf16 values: two bf16 products, of the weights' high parts and of their rests (f32 ones run at a sixteenth of the rate).
 template <int D>
 __device__ __forceinline__ void add_pv(const Step<bf16, D>& st, const f32x4 (&p)[2], f32x4 (&o)[D / 16]) {
-  const u32x4 b = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
-                   pack_bf16(p[1][2], p[1][3])};
+  u32x4 high, rest;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const WeightPair x = split_weights(p[w / 2][w % 2 * 2], p[w / 2][w % 2 * 2 + 1]);
+    high[w] = x.high;
+    rest[w] = x.rest;
+  }
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) {
     u32x4 a;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
       a[w] = __builtin_amdgcn_perm(st.v[2 * w + 1][j / 2], st.v[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-    o[j] = mfma16(a, b, o[j], bf16{});
+    o[j] = mfma16(a, high, o[j], bf16{});
+    o[j] = mfma16(a, rest, o[j], bf16{});
   }
 }
 template <int D>
@@ -647,10 +665,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 //
 // A step is two clusters, the softmax of its scores (VALU) and its product with V and the next step's with K (matrix units), each
 // behind a barrier, and the second half of the waves is one cluster behind the first: of a SIMD's two waves one is on the
-// VALU while the other is on the matrix units. Bound by LDS: a step's keys and values are read by all eight waves, 128 KB of
-// each, at 128 bytes a clock and the transposing reads at 64: some 3100 of a step's 4300 cycles (1.8 us); the products take 2000.
-// 64 rows to a wave would halve that and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of 1008
-// to 4032 keys, 8 key heads of 128, 256 rows each: 73 us, 34 GFLOP of nodes that are there in 54 of products.
+// VALU while the other is on the matrix units. Bound by LDS and the matrix units, neither of which is fed without a pause: a step's
+// keys and values are read by all eight waves, 128 KB of each, at 128 bytes a clock and the transposing reads at 64, some 3100 of a
+// step's 5000 cycles (2.1 us); the products take 3000, 1000 of them those of the weights' rests (without these the kernel takes
+// 72 us). 64 rows to a wave would halve the reads and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of
+// 1008 to 4032 keys, 8 key heads of 128, 256 rows each: 84 us, 34 GFLOP of nodes that are there in 81 of products.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
@@ -791,7 +810,7 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       }
       lds_barrier();
       __builtin_amdgcn_s_setprio(0);
-      u32x4 pb[KEYS / 16];
+      u32x4 high[KEYS / 16], rest[KEYS / 16];  // the weights' two parts
       if (mine) {
         if (s >= whole_to) {  // not every row sees every key: bit k of `sees` is the step's key k
           const bool old = s < cached_steps;
@@ -828,7 +847,11 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
 #pragma unroll
         for (int c = 0; c < KEYS / 16; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) pb[c][e] = pack_bf16(x[c / 2][c % 2 * 8 + 2 * e], x[c / 2][c % 2 * 8 + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) {
+            const WeightPair w = split_weights(x[c / 2][c % 2 * 8 + 2 * e], x[c / 2][c % 2 * 8 + 2 * e + 1]);
+            high[c][e] = w.high;
+            rest[c][e] = w.rest;
+          }
       }
       if (leads) {
         wait_vmem<C::COPIES>();
@@ -837,15 +860,15 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       lds_barrier();
       copy(s + 3);
       if (!mine) continue;
-      // The scores of the next step (behind the last one of zeros, for nothing), then O: reads from LDS are kept AHEAD products
-      // ahead of the one that they feed, in this order (a read's latency is some six products; left to itself the compiler has
-      // every product wait for its own read). The kernel's fastest run takes 70.4 us with 4 and 6, 72.2 with 8, 76 with 10.
+      // O, then the scores of the next step (behind the last one of zeros, for nothing), so that the weights are gone when those
+      // arrive: reads from LDS are kept AHEAD operands ahead of the one that they feed, in this order (a read's latency is some six
+      // products; left to itself the compiler has every product wait for its own read).
       const char *ks = lds + (s + 1 - s0) % 4 * C::STAGE, *vs = lds + (s - s0) % 4 * C::STAGE;
-      constexpr int QK = NT * D / 16, ALL = QK + KEYS / 16 * D / 32, AHEAD = 6;
+      constexpr int PV = KEYS / 16 * D / 32, ALL = PV + NT * D / 16, AHEAD = 5;
       auto fetch = [&](int i) {
-        if (i < QK) return *reinterpret_cast<const bf16x8*>(ks + koff[i / NT] + i % NT * 32 * RB);
+        if (i >= PV) return *reinterpret_cast<const bf16x8*>(ks + koff[(i - PV) / NT] + (i - PV) % NT * 32 * RB);
         typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-        const int c = (i - QK) / (D / 32), j = (i - QK) % (D / 32);
+        const int c = i / (D / 32), j = i % (D / 32);
         auto half = [&](int hi) {
           return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               reinterpret_cast<lds_i16x4*>(reinterpret_cast<uintptr_t>(vs + voff[j][hi] + c * 16 * RB)));
@@ -859,16 +882,20 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) ring[i] = fetch(i);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
-#pragma unroll
       for (int i = 0; i < ALL; ++i) {
         __builtin_amdgcn_sched_barrier(0);
-        if (i < QK)
-          mma32(ring[i % AHEAD], q[i / NT], x[i % NT]);
-        else
-          mma32(ring[i % AHEAD], __builtin_bit_cast(bf16x8, pb[(i - QK) / (D / 32)]), o[(i - QK) % (D / 32)]);
+        if (i < PV) {
+          const int c = i / (D / 32), j = i % (D / 32);
+          mma32(ring[i % AHEAD], __builtin_bit_cast(bf16x8, high[c]), o[j]);
+          mma32(ring[i % AHEAD], __builtin_bit_cast(bf16x8, rest[c]), o[j]);
+        } else {
+          const int c = (i - PV) / NT, t = (i - PV) % NT;
+          if (c == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
+          }
+          mma32(ring[i % AHEAD], q[c], x[t]);
+        }
         if (i + AHEAD < ALL) ring[i % AHEAD] = fetch(i + AHEAD);
       }
     }

@@ -10,6 +10,8 @@ their norms (independent errors) under 1e-6 of the result's. bf16: the weights a
 errors: 2^-8 * sqrt(sum p^2 v^2) <= 2^-8 max|v| / 1), and the output by half a step of itself; together 2^-8 (|out| + 5
 sqrt(sum p^2)) with sum p^2 <= 1: relative to the norm 2^-8 * sqrt(2)."""
 
+import math
+
 import pytest
 import torch
 
@@ -285,3 +287,65 @@ def test_accepted_rows_make_the_cache_of_plain_decoding(dev):
             assert float((e - out[i:i + 1, :, node]).abs().max()) <= 4.8e-5
         rows = int(pos[i] + count[i])
         assert torch.equal(kc[i, :, :rows], k0[i, :, :rows]) and torch.equal(vc[i, :, :rows], v0[i, :, :rows])
+
+
+def _half_step(x):
+    """Half the distance of bf16 values at |x|."""
+    return torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0**-126))) - 8)
+
+
+# bf16 kernels by rows: 16, 32 and 64 of a wave, and the ones that share keys through LDS; each head in one workgroup and cut.
+BF16_ROWS = [(b, h, hkv, t, length, d)
+             for d, rows in ((64, ((2, 2, 8), (3, 1, 7), (4, 1, 13), (4, 1, 40))), (128, ((1, 1, 1), (2, 2, 8), (4, 1, 8), (5, 1, 13), (8, 1, 40))),
+                             (256, ((2, 2, 8), (4, 1, 8), (4, 1, 17))))
+             for h, hkv, t in rows for b, length in ((2, 200), (2, 3000))]
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d", BF16_ROWS)
+def test_weights_of_bf16_values_sum_to_one(dev, b, h, hkv, t, length, d):
+    """One value for all keys and nodes: every output is that value, whatever the weights. Those are summed in f32 (n terms, n 2^-24
+    <= 2^-12 with n <= 3000) and lie within 2^-16 of themselves in the product: together under 2^-9, half a step of any value.
+    First all keys but one have a weight of 0.5 (1 + 0.97 * 2^-8), which one rounding to bf16 takes down by nearly 2^-8."""
+    q, kn, vn, kc, vc = _inputs(dev, b, h, hkv, t, length, d, BF16, seed=t)
+    value = vc[:, :, :1].clone()
+    pos, parents = torch.tensor([length - t, length // 2], dtype=torch.int32, device=dev), trees(b, t, 1).to(dev)
+    want = value.repeat_interleave(h // hkv, 1).expand(b, h, t, d)
+    one, minus = torch.zeros_like(q), torch.zeros_like(kc)
+    one[..., 0], minus[..., 0] = 1, -1
+    minus[:, :, 3] = 0
+    for qs, ks, news, scale in ((one, minus, minus[:, :, 4:4 + t], -math.log(0.5 * (1 + 0.97 * 2.0**-8))), (q, kc, kn, None)):
+        out = tree_attention(qs, news, value.expand_as(vn), ks.clone(), value.expand_as(vc).contiguous(), pos, parents, scale=scale)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d", BF16_ROWS)
+def test_bf16_outputs_are_rounded_once(dev, b, h, hkv, t, length, d):
+    """The distance from the sums in 64 bits is the output's half step, beside it 2^-16 of the weights' values (up to 5.5) and the f32
+    sums' 4.8e-5. With few keys, whose outputs are of order one, that is under a tenth of most half steps."""
+    for pos in ([length - t, length // 2], [9, 0]):
+        q, kn, vn, kc, vc = _inputs(dev, b, h, hkv, t, length, d, BF16, seed=t + 1)
+        p, parents = torch.tensor(pos, dtype=torch.int32, device=dev), trees(b, t, 2)
+        ref = tree_attention_reference(*(x.double() for x in (q, kn, vn, kc, vc)), p, parents.to(dev))
+        if t == 1 and h == hkv:
+            one = lambda x: x[:, :, 0]
+            e = decode_attention(one(q), one(kn), one(vn), kc.clone(), vc.clone(), p)
+            assert bool(((e.double() - one(ref)).abs() <= _half_step(one(ref)) * 1.001 + 5.5 * 2.0**-16 + 4.8e-5).all())
+        out = tree_attention(q, kn, vn, kc, vc, p, parents.to(dev))
+        assert bool(((out.double() - ref).abs() <= _half_step(ref) * 1.001 + 5.5 * 2.0**-16 + 4.8e-5).all())
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d", BF16_ROWS)
+def test_infinite_values_of_the_cache(dev, b, h, hkv, t, length, d):
+    """Infinities and NaN in cached values, which every row sees: infinite in that element, NaN where two signs or a NaN meet."""
+    q, kn, vn, kc, vc = _inputs(dev, b, h, hkv, t, length, d, BF16, seed=t + 2)
+    inf = float("inf")
+    for row, element, bad in ((5, 3, inf), (40, 7, -inf), (60, 9, float("nan")), (33, 11, inf), (2, 11, -inf), (7, 20, inf), (61, 20, inf)):
+        vc[:, :, row, element] = bad
+    p, parents = torch.tensor([length - t, length // 2], dtype=torch.int32, device=dev), trees(b, t, 3).to(dev)
+    ref = tree_attention_reference(*(x.double() for x in (q, kn, vn, kc, vc)), p, parents)
+    out = tree_attention(q, kn, vn, kc, vc, p, parents)
+    assert bool((ref[..., 3] == inf).all()) and bool((ref[..., 7] == -inf).all()) and bool(torch.isnan(ref[..., [9, 11]]).all())
+    assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(out.isinf(), ref.isinf())
+    assert torch.equal(out == inf, ref == inf)
+    near = (out.double() - ref).abs() <= _half_step(ref) * 1.001 + 5.5 * 2.0**-16 + 4.8e-5
+    assert bool((near | ~torch.isfinite(ref)).all())
