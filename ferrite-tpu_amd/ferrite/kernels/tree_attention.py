@@ -83,10 +83,10 @@ def tree_attention_reference(q, k_new, v_new, k_cache, v_cache, pos, parents, *,
         k_cache[i, :, p + there] = k_new[i][:, there]
         v_cache[i, :, p + there] = v_new[i][:, there]
         out[i] = 0
-        for t in there.tolist():
-            rows = torch.cat([torch.arange(p, device=q.device), p + sees[t].nonzero()[:, 0]])
+        for node in there.tolist():
+            rows = torch.cat([torch.arange(p, device=q.device), p + sees[node].nonzero()[:, 0]])
             keys = k_cache[i][:, rows].to(work).repeat_interleave(h // hkv, 0)
             values = v_cache[i][:, rows].to(work).repeat_interleave(h // hkv, 0)
-            s = (keys * q[i][:, t, None].to(work)).sum(-1) * scale
-            out[i][:, t] = (torch.softmax(s, -1)[..., None] * values).sum(1).to(q.dtype)
+            s = (keys * q[i][:, node, None].to(work)).sum(-1) * scale
+            out[i][:, node] = (torch.softmax(s, -1)[..., None] * values).sum(1).to(q.dtype)
     return out

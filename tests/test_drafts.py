@@ -272,3 +272,21 @@ def test_tree_reference_is_attention_along_each_branch():
     assert not out[0, :, 4].any()
     assert torch.equal(kc[0, 0, 6:10], kn[0, 0, :4]) and torch.equal(kc[0, 0, 10:], k0[0, 0, 10:])
     assert ancestors(parents)[0].int().tolist() == [[1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 0, 1, 0, 0], [1, 0, 1, 1, 0], [0] * 5]
+
+
+@pytest.mark.parametrize("t,pos", [(1, [0, 16]), (4, [2, 13]), (4, [2, 15]), (3, [0, 14, 13, -1, 16])])
+def test_tree_reference_checks_every_sequence_against_the_whole_tree(t, pos):
+    """A sequence whose rows pos .. pos + T - 1 do not lie in the cache is NaN and writes nothing, whatever nodes the one before it
+    has."""
+    g = torch.Generator().manual_seed(1)
+    mk = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    b, length = len(pos), 16
+    q, kn, vn, kc, vc = mk(b, 2, t, 64), mk(b, 1, t, 64), mk(b, 1, t, 64), mk(b, 1, length, 64), mk(b, 1, length, 64)
+    parents = (torch.arange(t) - 1).int().expand(b, t).clone()
+    parents[0, 1:] = -2  # the first sequence has one node
+    k0, v0 = kc.clone(), vc.clone()
+    out = tree_attention_reference(q, kn, vn, kc, vc, torch.tensor(pos), parents)
+    for i, p in enumerate(pos):
+        inside = 0 <= p <= length - t
+        assert bool(torch.isnan(out[i]).any()) == (not inside)
+        assert torch.equal(kc[i], k0[i]) != inside and torch.equal(vc[i], v0[i]) != inside

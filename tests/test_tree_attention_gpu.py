@@ -349,3 +349,14 @@ def test_infinite_values_of_the_cache(dev, b, h, hkv, t, length, d):
     assert torch.equal(out == inf, ref == inf)
     near = (out.double() - ref).abs() <= _half_step(ref) * 1.001 + 5.5 * 2.0**-16 + 4.8e-5
     assert bool((near | ~torch.isfinite(ref)).all())
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d,dtype", [
+    (130, 512, 1, 1, 6300, 64, F32),   # 512 rows a sequence: 1040 row groups
+    (96, 32, 32, 2, 600, 64, F32)])    # 3072 heads
+def test_many_whole_heads_of_unequal_lengths(dev, b, h, hkv, t, length, d, dtype):
+    """More heads than fill the chip, each in one workgroup: short, empty, misplaced and full sequences side by side."""
+    x = _inputs(dev, b, h, hkv, t, length, d, dtype, seed=b)
+    pos = torch.randint(0, length - t + 1, (b,), generator=torch.Generator().manual_seed(b)) // 8
+    pos[1], pos[b // 2 - 1], pos[b - 1], pos[65], pos[7] = 0, -1, length - t, length, length - t
+    _check(dev, *x, pos.tolist(), trees(b, t, 1, absent=0.1))
