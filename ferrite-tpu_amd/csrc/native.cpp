@@ -53,6 +53,13 @@ bool records(std::initializer_list<const Tensor*> inputs) {
     if (t->requires_grad()) return true;
   return false;
 }
+// Whether a forward-mode tangent belongs to one of `inputs` (grad mode or not): such a call goes to the autograd function too, which
+// has none to give and says so.
+bool has_tangent(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
+}
 // A leaf's gradient is added up on the stream where the graph that first took the leaf was made, for as long as that graph lives. While
 // it is a stream outside the current capture, a backward pass captured here would run work there and end the process:
 // refused where the pass would begin.
@@ -347,7 +354,8 @@ std::tuple<Tensor, Tensor, Tensor> qk_norm_rope(const Tensor& qkv0, const Tensor
   const HeadsOptions o{h, hkv, eps, interleaved, pos};
   const bool record = records({&qkv, &wq, &wk});
   if (record) refuse_leaves_of_other_graphs({&qkv0, &wq0, &wk0}, "ferrite_qk_norm_rope");
-  const auto out = record ? HeadsFn::apply(qkv, wq, wk, cos, sin, o) : heads_forward(qkv, wq, wk, cos, sin, o);
+  const auto out = record || has_tangent({&qkv, &wq, &wk, &cos, &sin}) ? HeadsFn::apply(qkv, wq, wk, cos, sin, o)
+                                                                       : heads_forward(qkv, wq, wk, cos, sin, o);
   return {out[0], out[1], out[2]};
 }
 

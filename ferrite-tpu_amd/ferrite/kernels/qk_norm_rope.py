@@ -69,7 +69,8 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, *, n_head: int, n_kv_head: i
     in f32, rounded once. A position outside the tables gives NaN in its q and k rows. Head dims: even, up to 512.
 
     Differentiable in qkv and the weights, whose gradients are summed in f32 in a fixed order. A captured call that records
-    a backward raises RuntimeError while a graph made outside the capture holds one of these as a leaf."""
+    a backward raises RuntimeError while a graph made outside the capture holds one of these as a leaf, and so does any call with a
+    forward-mode tangent."""
     n_kv_head = n_head if n_kv_head is None else n_kv_head
     _check(qkv, q_weight, k_weight, cos, sin, n_head, n_kv_head, positions)
     _hip.dtype_code(qkv.dtype)

@@ -308,3 +308,21 @@ def test_feeds_attention_like_split_heads(dev):
     want = torch.autograd.grad(ro, ref, g.float())[0]
     o, ro = o.detach(), ro.detach()
     assert float((o.float() - ro).norm() / ro.norm()) <= 1e-2 and float((got.float() - want).norm() / want.norm()) <= 2e-2
+
+
+def test_forward_mode_is_refused(dev):
+    """There is no rule for tangents: a dual input raises, in whatever place and grad mode, as flash_attention does."""
+    import torch.autograd.forward_ad as fwd
+
+    inputs = list(_inputs(dev, 2, 5, 2, 1, 64, 32, F32))
+    plain = qk_norm_rope(*inputs, n_head=2, n_kv_head=1)
+    with fwd.dual_level():
+        for i in range(5):
+            for mode in (torch.no_grad, torch.enable_grad):
+                dual = [fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(inputs)]
+                with mode(), pytest.raises(RuntimeError, match="jvp"):
+                    qk_norm_rope(*dual, n_head=2, n_kv_head=1)
+        heads = torch.randn(1, 2, 128, 64, device=dev)
+        with pytest.raises(RuntimeError, match="jvp"):
+            flash_attention(fwd.make_dual(heads, torch.ones_like(heads)), heads, heads)
+        assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(*inputs, n_head=2, n_kv_head=1), plain))
