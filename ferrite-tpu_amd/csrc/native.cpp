@@ -653,17 +653,23 @@ Tensor tree_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, cons
   return out.transpose(1, 2);
 }
 
+// As many sequences to a call of the kernels as their 65535 nodes hold; the calls share the workspace, one behind the other.
 std::tuple<Tensor, Tensor, Tensor> accept_drafts(const Tensor& logits0, const Tensor& tokens0, const Tensor& parents0) {
   const Tensor logits = logits0.contiguous(), tokens = tokens0.to(at::kLong).contiguous(),
                parents = parents0.contiguous();
-  const int64_t b = logits.size(0), t = logits.size(1), v = logits.size(2);
+  const int64_t b = logits.size(0), t = logits.size(1), v = logits.size(2), most = std::min(b, 65535 / t);
   Tensor path = at::empty({b, t}, parents.options()), count = at::empty({b}, parents.options()),
          following = at::empty({b}, tokens.options());
-  const Tensor ws = bytes_on(ferrite_internal_accept_drafts_workspace(b, t, v), logits);
-  check(ferrite_internal_accept_drafts(ptr(logits), (const int64_t*)ptr(tokens), (const int32_t*)ptr(parents),
-                                       (int32_t*)ptr(path), (int32_t*)ptr(count), (int64_t*)ptr(following), b, t, v,
-                                       code(logits), ptr(ws), size_of(ws), stream_of(logits)),
-        "ferrite_accept_drafts");
+  const Tensor ws = bytes_on(ferrite_internal_accept_drafts_workspace(most, t, v), logits);
+  for (int64_t from = 0; from < b; from += most) {
+    const int64_t n = std::min(most, b - from);
+    check(ferrite_internal_accept_drafts(static_cast<char*>(ptr(logits)) + from * t * v * logits.element_size(),
+                                         (const int64_t*)ptr(tokens) + from * t, (const int32_t*)ptr(parents) + from * t,
+                                         (int32_t*)ptr(path) + from * t, (int32_t*)ptr(count) + from,
+                                         (int64_t*)ptr(following) + from, n, t, v, code(logits), ptr(ws), size_of(ws),
+                                         stream_of(logits)),
+          "ferrite_accept_drafts");
+  }
   return {path, count, following};
 }
 

@@ -186,3 +186,10 @@ def test_streams_and_graph(dev, v):
         compact_cache_reference(kr, vr, pos.cpu(), *want[:2])
         assert torch.equal(k.cpu(), kr) and torch.equal(vv.cpu(), vr)
     graph.reset()
+
+
+@pytest.mark.parametrize("b,t,v", [(1030, 64, 7), (1030, 64, 1100), (70001, 1, 5)])
+def test_accept_more_nodes_than_one_launch_takes(dev, b, t, v):
+    """Over 65535 nodes in all, walked by one workgroup a sequence and cut into pieces."""
+    logits, tokens, parents = _drafts(dev, b, t, v, BF16 if v > 1000 else F32, seed=b)
+    _check(dev, logits, tokens, parents)
