@@ -195,6 +195,12 @@ class DeviceGuard {
 // names the entry point).
 int allow_lds(const void* kernel, int bytes, hipStream_t s, const char* what);
 
+// Whether [p, p + np) and [q, q + nq) have a byte in common.
+inline bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
+  const char *a = static_cast<const char*>(p), *b = static_cast<const char*>(q);
+  return a < b + nq && b < a + np;
+}
+
 inline bool valid_dtype(int dt) { return dt == FERRITE_F32 || dt == FERRITE_BF16; }
 inline const char* dtype_name(int dt) { return dt == FERRITE_F32 ? "f32" : dt == FERRITE_BF16 ? "bf16" : "?"; }
 

@@ -294,6 +294,9 @@ extern "C" int ferrite_internal_compact_cache(void* k_cache, void* v_cache, cons
   const bool vec = bytes % 16 == 0 && ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0;
   const int64_t cols = vec ? bytes / 16 : d, blocks = cdiv(2 * layers * h * cols, 256);
   if (blocks > 0xffffffff / 256) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_compact_cache: too many heads");
+  const int64_t all = std::min(layers * b * h, ((int64_t)1 << 62) / (max_len * bytes)) * max_len * bytes;
+  if (overlap(k_cache, all, v_cache, all))  // a row could be read behind the other cache's write of it
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_compact_cache: the caches overlap");
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto* unit) {
     typedef std::remove_pointer_t<decltype(unit)> U;

@@ -107,7 +107,8 @@ int ferrite_internal_heads_rope_bwd(const void* qkv, int64_t batch_stride, int64
  * ferrite_internal_tree_attention_workspace(...) bytes (-1: sizes out of range); its content need not survive the call. A head's
  * cached keys, and its nodes' rows with what lies between them, take at most 4 GiB less 128 KiB. A node's values that are not
  * finite reach only the rows that see it. How the sums are parted depends on the sizes and positions of the whole batch, so a
- * sequence's last bits may differ from batch to batch; for the same call they are the same.
+ * sequence's last bits may differ from batch to batch; for the same call they are the same. The caches must not overlap each
+ * other or what lies from the first to the last element of q, k_new or v_new.
  */
 int64_t ferrite_internal_tree_attention_workspace(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int64_t d,
                                                   int dtype);
@@ -130,7 +131,8 @@ int ferrite_internal_accept_drafts(const void* logits, const int64_t* tokens, co
 
 /*
  * Rows pos[b] + path[b, i] of the caches [layers, B, H, max_len, D] to pos[b] + i, i < count[b], in place; a path ends
- * at the first entry that is not larger than the one before (or negative) or whose row lies outside the cache. 1 <= T <= 64.
+ * at the first entry that is not larger than the one before (or negative) or whose row lies outside the cache. 1 <= T <= 64. The caches
+ * must not overlap.
  */
 int ferrite_internal_compact_cache(void* k_cache, void* v_cache, const int32_t* pos, const int32_t* path,
                                    const int32_t* count, int64_t layers, int64_t b, int64_t h, int64_t max_len, int64_t d,

@@ -1167,6 +1167,15 @@ extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new,
   for (int i = 5; i < 9; i += 3)
     if (strides[i] < 0 || (t - 1) * strides[i] * (dtype == FERRITE_BF16 ? 2 : 4) > (int64_t)kMostBytes - 1024)
       return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: a head's new keys or values span 4 GiB");
+  // Nodes' rows are written while other workgroups read the inputs.
+  const int64_t size = dtype == FERRITE_BF16 ? 2 : 4, cache = b * hkv * max_len * d * size;
+  bool apart = !overlap(k_cache, cache, v_cache, cache);
+  const void* inputs[3] = {q, k_new, v_new};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t* st = strides + 3 * i;
+    const int64_t span = ((b - 1) * st[0] + ((i ? hkv : h) - 1) * st[1] + (t - 1) * st[2] + d) * size;
+    apart = apart && !overlap(inputs[i], span, k_cache, cache) && !overlap(inputs[i], span, v_cache, cache);
+  }
   const Plan p = plan_for(b, h, hkv, t, max_len, d, dtype);
   TreeArgs a{q, k_new, v_new, k_cache, v_cache, pos, parents, out, nullptr, {}, {}, {}, (int)b, (int)h, (int)hkv, (int)(h / hkv),
              (int)t, (int)max_len, (int)(h / hkv * t), (int)p.row_groups, (int)p.groups, (int)p.least, (int)p.begin,
@@ -1182,6 +1191,8 @@ extern "C" int ferrite_internal_tree_attention(const void* q, const void* k_new,
       return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: workspace too small or unaligned");
     a.part = static_cast<char*>(workspace);
   }
+  if (!apart)
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_tree_attention: the caches overlap each other or q, k_new or v_new");
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto tiles = [&](auto* e, auto D) {
     typedef std::remove_pointer_t<decltype(e)> T;

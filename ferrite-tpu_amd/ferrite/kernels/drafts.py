@@ -49,7 +49,7 @@ def compact_cache(k_cache, v_cache, pos, path, count) -> None:
 
     A path goes up (path[b, i] > path[b, i - 1], from 0), as :func:`accept_drafts` gives it, so all rows move as if each were read
     before any was written. It ends at the first entry that does not, or whose row lies outside the cache; rows
-    behind it stay as they are."""
+    behind it stay as they are. Caches that overlap raise RuntimeError. Layers, B and H are at most 65535."""
     if k_cache.ndim not in (4, 5) or v_cache.shape != k_cache.shape:
         raise ValueError(f"expected caches [B, H, max_len, D] or [layers, B, H, max_len, D] of one shape; got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")

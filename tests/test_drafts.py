@@ -290,3 +290,28 @@ def test_tree_reference_checks_every_sequence_against_the_whole_tree(t, pos):
         inside = 0 <= p <= length - t
         assert bool(torch.isnan(out[i]).any()) == (not inside)
         assert torch.equal(kc[i], k0[i]) != inside and torch.equal(vc[i], v0[i]) != inside
+
+
+def test_overlapping_caches_are_refused():
+    """By address, before any launch: caches that share a byte, and inputs that reach into one."""
+    import ctypes
+
+    lib = _hip.lib()
+    k = 1 << 30
+    compact = lambda v: lib.ferrite_internal_compact_cache(k, v, 4096, 4096, 4096, 3, 2, 4, 100, 64, 8, _hip.BF16, None)
+    size = 3 * 2 * 4 * 100 * 64 * 2
+    for v in (k, k + size - 16, k - size + 16, k + 2):
+        assert compact(v) == 1 and "overlap" in _hip.last_error(), v
+    b, h, hkv, t, n, d = 2, 4, 2, 3, 128, 64
+    size, far = b * hkv * n * d * 2, 1 << 34
+    dense = [v for heads in (h, hkv, hkv) for v in (heads * t * d, t * d, d)]
+
+    def tree(q=far, kn=far + (1 << 20), vn=far + (2 << 20), vc=far << 1, st=dense):
+        return lib.ferrite_internal_tree_attention(q, kn, vn, k, vc, 4096, 4096, 1 << 40, (ctypes.c_int64 * 9)(*st), b, h, hkv, t, n, d,
+                                                   _hip.BF16, 0.1, None, 0, None)
+
+    rows, q_rows = b * hkv * t * d * 2, b * h * t * d * 2
+    for change in (dict(vc=k), dict(vc=k + size - 16), dict(vc=k - size + 16), dict(q=k), dict(q=k + size - 16), dict(q=k - q_rows + 16),
+                   dict(kn=k + 512), dict(kn=k - rows + 16), dict(vn=k), dict(vn=(far << 1) + size - 16), dict(kn=(far << 1)),
+                   dict(kn=k - 4096 + rows, st=[*dense[:3], 2048, t * d, d, *dense[6:]])):  # a view's last sequence
+        assert tree(**change) == 1 and "overlap" in _hip.last_error(), change

@@ -193,3 +193,19 @@ def test_accept_more_nodes_than_one_launch_takes(dev, b, t, v):
     """Over 65535 nodes in all, walked by one workgroup a sequence and cut into pieces."""
     logits, tokens, parents = _drafts(dev, b, t, v, BF16 if v > 1000 else F32, seed=b)
     _check(dev, logits, tokens, parents)
+
+
+def test_caches_beside_each_other(dev):
+    """Caches that end where the other begins are two; one for both, or shifted by a row, is refused and left as it is."""
+    both = torch.randn(2, 2, 3, 16, 8, device=dev)
+    want = [c.cpu() for c in both]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    args = ints([3, 9]), ints([[0, 2, 5], [1, 2, 6]]), ints([3, 2])
+    compact_cache_reference(*want, *(a.cpu() for a in args))
+    compact_cache(both[0], both[1], *args)
+    assert all(torch.equal(c.cpu(), w) for c, w in zip(both, want))
+    flat = both.flatten()
+    for k, v in ((both[0], both[0]), (both[1], flat[8 * 16 * 6 - 8:-8].view(2, 3, 16, 8))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            compact_cache(k, v, *args)
+    assert all(torch.equal(c.cpu(), w) for c, w in zip(both, want))

@@ -360,3 +360,21 @@ def test_many_whole_heads_of_unequal_lengths(dev, b, h, hkv, t, length, d, dtype
     pos = torch.randint(0, length - t + 1, (b,), generator=torch.Generator().manual_seed(b)) // 8
     pos[1], pos[b // 2 - 1], pos[b - 1], pos[65], pos[7] = 0, -1, length - t, length, length - t
     _check(dev, *x, pos.tolist(), trees(b, t, 1, absent=0.1))
+
+
+def test_caches_beside_each_other(dev):
+    """Two halves of one allocation are two caches; one for both, or nodes that are rows of one, are refused and nothing is written."""
+    b, h, t, length, d = 2, 2, 5, 200, 64
+    for dtype in (BF16, F32):
+        q, kn, vn, kc, vc = _inputs(dev, b, h, h, t, length, d, dtype)
+        both = torch.stack([kc, vc])
+        pos, parents = torch.tensor([20, 100], dtype=torch.int32, device=dev), trees(b, t, 1).to(dev)
+        want = tree_attention(q, kn, vn, kc, vc, pos, parents)
+        assert torch.equal(tree_attention(q, kn, vn, both[0], both[1], pos, parents), want)
+        assert torch.equal(both, torch.stack([kc, vc]))
+        rows = both[0][:, :, 20:20 + t]
+        for args in ((q, kn, vn, both[0], both[0]), (q, rows, vn, both[0], both[1]), (q, kn, rows, both[0], both[1]),
+                     (rows, kn, vn, both[0], both[1]), (q, kn, both[1][:, :, :t], both[0], both[1])):
+            with pytest.raises(RuntimeError, match="overlap"):
+                tree_attention(*args, pos, parents)
+        assert torch.equal(both, torch.stack([kc, vc]))
