@@ -639,7 +639,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
       if (whole) {
         const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
         T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
-        const bool zero = !(there >> t & 1) || lsum == 0.f;
+        const bool zero = !(there >> t & 1);
         float y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = !valid ? NAN : zero ? 0.f : sum[i] / lsum;
@@ -933,7 +933,7 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       if (whole) {
         const int gh = (row0 + r) / a.T, t = row0 + r - gh * a.T;
         bf16* out = static_cast<bf16*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
-        const bool zero = !(there >> t & 1) || ml[1] == 0.f;
+        const bool zero = !(there >> t & 1);
         float y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = !valid ? NAN : zero ? 0.f : sum[i] / ml[1];
@@ -1022,7 +1022,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int slot_row
     if (part != 0 || r0 + row >= to) continue;
     const int gh = r / a.T, t = r - gh * a.T;
     T* out = static_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.H + h * a.G + gh) * D + d;
-    const bool zero = !(there >> t & 1) || l == 0.f;
+    const bool zero = !(there >> t & 1);
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = zero ? 0.f : acc[i] / l;

@@ -378,3 +378,27 @@ def test_caches_beside_each_other(dev):
             with pytest.raises(RuntimeError, match="overlap"):
                 tree_attention(*args, pos, parents)
         assert torch.equal(both, torch.stack([kc, vc]))
+
+
+@pytest.mark.parametrize("h,hkv,t,length,d,dtype", [
+    (2, 2, 7, 200, 64, BF16), (2, 2, 7, 3000, 128, BF16), (4, 2, 20, 300, 128, BF16), (4, 2, 40, 3000, 64, BF16), (4, 2, 13, 200, 256, BF16),
+    (4, 2, 9, 200, 64, F32), (4, 2, 9, 3000, 128, F32), (4, 2, 33, 900, 64, F32)])
+def test_rows_whose_scores_are_all_minus_infinity(dev, h, hkv, t, length, d, dtype):
+    """The quotient of two zeros, as a softmax of such scores and decode_attention have it: NaN in the rows of that key head, and where
+    one key is left its value. Absent nodes stay zero."""
+    q, kn, vn, kc, vc = _inputs(dev, 2, h, hkv, t, length, d, dtype, seed=t)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    kc[:, 0, :, 0], kn[:, 0, :, 0] = -float("inf"), -float("inf")
+    kc[1, 0, 33, 0] = 1
+    pos, parents = torch.tensor([length - t, length // 2], dtype=torch.int32, device=dev), trees(2, t, 1)
+    parents[:, 2] = -2
+    there = ancestors(parents).diagonal(dim1=1, dim2=2).to(dev)[:, None, :, None]
+    ref = tree_attention_reference(*(x.double() for x in (q, kn, vn, kc, vc)), pos, parents.to(dev))
+    out = tree_attention(q, kn, vn, kc.clone(), vc.clone(), pos, parents.to(dev))
+    g = h // hkv
+    assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(torch.isnan(out[0, :g]), there[0].expand_as(out[0, :g]))
+    assert torch.equal(out[1, :g], torch.where(there[1], vc[1, 0, 33], torch.zeros_like(vc[1, 0, 33])).expand_as(out[1, :g]))
+    assert not bool(torch.isnan(out[:, g:]).any()) and not bool(torch.where(there, 0, out).any())
+    e = decode_attention(q[:, :, 0], *(x[:, :, 0].repeat_interleave(g, 1) for x in (kn, vn)),
+                         *(x.repeat_interleave(g, 1) for x in (kc, vc)), pos)
+    assert torch.equal(torch.isnan(e), torch.isnan(out[:, :, 0]))
