@@ -326,3 +326,26 @@ def test_forward_mode_is_refused(dev):
         with pytest.raises(RuntimeError, match="jvp"):
             flash_attention(fwd.make_dual(heads, torch.ones_like(heads)), heads, heads)
         assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(*inputs, n_head=2, n_kv_head=1), plain))
+
+
+# Sizes of training and prefill: up to eight heads to a wave (from 196608 heads on, 13 + 5 + 5 of them 7, 6 and 5 at a time), and more
+# groups of tokens than the backward has blocks, so that each goes over several of them, the last round not full. A weight's gradient: a
+# lane adds up to 7 heads of each of 5 groups of tokens, then come at most 4, 4, 17 and 6 additions: 66 of the 128 allowed.
+@pytest.mark.parametrize("b,s,h,hkv,d,rot,dtype,inter", [
+    (3, 2851, 13, 5, 64, 64, BF16, False),   # 16 tokens to a wave
+    (3, 2851, 13, 5, 128, 64, BF16, True),
+    (1, 8551, 13, 5, 40, 24, F32, False),
+    (3, 2851, 13, 5, 130, 130, BF16, False),  # by elements, a token to a wave: five rounds
+    (1, 2049, 13, 5, 130, 52, F32, True),     # the same with two heads to a wave
+    (1, 4099, 3, 1, 512, 512, F32, False),    # vectors, a token to a wave, one head
+    (2, 8200, 8, 2, 512, 256, BF16, False)])  # two tokens to a wave
+def test_training_sizes(dev, b, s, h, hkv, d, rot, dtype, inter):
+    test_forward_and_gradients(dev, b, s, h, hkv, d, rot, dtype, inter)
+
+
+# Lanes to a head, and pairs in halves or side by side, that the cases above leave out.
+@pytest.mark.parametrize("d,rot,dtype,inter", [
+    (32, 16, BF16, False), (256, 128, BF16, True), (80, 40, BF16, True), (130, 4, BF16, True), (24, 16, F32, False), (16, 8, F32, True),
+    (64, 64, F32, True), (256, 128, F32, False), (200, 200, F32, True), (512, 256, F32, True)])
+def test_layouts(dev, d, rot, dtype, inter):
+    test_forward_and_gradients(dev, 2, 75, 3, 2, d, rot, dtype, inter)
