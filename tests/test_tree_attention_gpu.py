@@ -402,3 +402,32 @@ def test_rows_whose_scores_are_all_minus_infinity(dev, h, hkv, t, length, d, dty
     e = decode_attention(q[:, :, 0], *(x[:, :, 0].repeat_interleave(g, 1) for x in (kn, vn)),
                          *(x.repeat_interleave(g, 1) for x in (kc, vc)), pos)
     assert torch.equal(torch.isnan(e), torch.isnan(out[:, :, 0]))
+
+
+# Two and four row tiles to a wave: heads whole (up to 16 steps), cut among few, and cut among many, whose pieces one line of the join
+# adds up; and the narrowest rows over caches of many heads.
+TILES = [(2, h, hkv, t, length, d, dtype)
+         for d, dtype in ((64, BF16), (128, BF16), (256, BF16), (64, F32), (128, F32), (256, F32))
+         for h, hkv, t in ((1, 1, 17), (6, 2, 8), (4, 1, 8)) for length in (230, 3000)]
+TILES += [(2, h, hkv, t, length, 64, dtype) for dtype in (BF16, F32) for h, hkv, t in ((3, 1, 11), (8, 2, 13), (1, 1, 64))
+          for length in (240, 1500)]
+TILES += [(8, 32, 32, 4, 4200, 128, BF16), (8, 32, 32, 9, 4300, 64, BF16), (8, 96, 32, 8, 4200, 128, BF16), (8, 64, 32, 9, 4200, 256, BF16),
+          (8, 128, 32, 13, 4200, 64, BF16), (8, 64, 32, 10, 2100, 128, F32),
+          (16, 16, 4, 24, 1500, 128, BF16)]  # 96 rows over shared keys
+
+
+@pytest.mark.parametrize("b,h,hkv,t,length,d,dtype", TILES)
+def test_row_tiles(dev, b, h, hkv, t, length, d, dtype):
+    x = _inputs(dev, b, h, hkv, t, length, d, dtype, seed=h * t + d)
+    pos = [length - t - i * (length // 9) for i in range(b)]
+    pos[1] = 31
+    _check(dev, *x, pos, trees(b, t, 1))
+    if b == 2:
+        _check(dev, *x, pos[::-1], trees(b, t, 2, absent=0.3), scale=-0.3 / d**0.5)
+
+
+@pytest.mark.parametrize("h,hkv,t,length,d,dtype", [
+    (4, 2, 8, 230, 128, BF16), (6, 2, 8, 3000, 128, BF16), (8, 2, 8, 3000, 128, BF16), (4, 2, 9, 200, 256, BF16), (8, 2, 8, 3000, 256, BF16),
+    (8, 2, 12, 1500, 64, BF16), (6, 2, 8, 3000, 64, F32), (6, 2, 8, 200, 256, F32)])
+def test_branches_stay_apart_in_row_tiles(dev, h, hkv, t, length, d, dtype):
+    test_what_a_branch_does_not_see_does_not_touch_it(dev, 2, h, hkv, t, length, d, dtype, [length - t, 40])
