@@ -134,3 +134,89 @@ def test_drafted_steps_decode_like_single_tokens(dev, t):
         if t > 4:
             assert sum(len(x) - len(s) for x, s in zip(got, starts)) > b * steps  # drafts were taken
         graph.reset()
+
+
+@pytest.mark.parametrize("h,hkv,t,d,length", [
+    (4, 2, 8, 64, 300), (4, 4, 6, 128, 2500), (8, 2, 8, 128, 900), (8, 2, 24, 128, 1200), (4, 1, 40, 256, 700), (16, 2, 60, 64, 500)])
+def test_bf16_steps_are_their_operators(dev, h, hkv, t, d, length):
+    """Steps in bf16, with few rows a key head and with many that share keys, in turn plain and replayed: every operator's outputs are
+    what its definition gives in 64 bits for the inputs that it had in that step. The heads are off by half a bf16 step and 20 * 2^-24
+    of a pair's size (under 2 * 16), the attention by half a step, 2^-16 of the values (up to 5.5) and 4.8e-5; tokens, paths and
+    cached rows are equal."""
+    from ferrite.kernels.drafts import accept_drafts_reference, compact_cache_reference
+    from ferrite.kernels.tree_attention import tree_attention_reference
+
+    from tests.test_drafts_gpu import trees
+
+    g = torch.Generator().manual_seed(t)
+    b, c, bf = 3, h * d, torch.bfloat16
+    mk = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(dev, bf)
+    layers = [(mk(c, (h + 2 * hkv) * d, scale=c**-0.5), mk(d, scale=0.1) + 1, mk(d, scale=0.1) + 1, mk(c, c, scale=c**-0.5))
+              for _ in range(2)]
+    head, x0 = mk(c, 71, scale=c**-0.5), mk(b, t, c)
+    cos, sin = rope_tables(length, d, device=dev)
+    kc, vc = mk(2, b, hkv, length, d), mk(2, b, hkv, length, d)
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
+    pos, tokens, parents, depths = ints(b), ints(b, t), ints(b, t), ints(b, t)
+
+    def step():
+        x, seen = x0, []
+        for layer, (wqkv, wq, wk, wo) in enumerate(layers):
+            qkv = x @ wqkv
+            q, k, v = qk_norm_rope(qkv, wq, wk, cos, sin, n_head=h, n_kv_head=hkv, positions=pos[:, None] + depths)
+            a = tree_attention(q, k, v, kc[layer], vc[layer], pos, parents)
+            x = x + a.transpose(1, 2).reshape(b, t, c) @ wo
+            seen.append((qkv, q, k, v, a))
+        logits = x @ head
+        kept = accept_drafts(logits, tokens, parents)
+        compact_cache(kc, vc, pos, kept[0], kept[1])
+        return seen, logits, kept
+
+    def draw(seed):
+        up = trees(b, t, seed, absent=0.1)
+        up[:, 0] = -1
+        deep = torch.zeros(b, t, dtype=torch.int32)
+        for i in range(1, t):
+            deep[:, i] = torch.where((up[:, i] >= 0) & (up[:, i] < i), deep.gather(1, up[:, i:i + 1].clamp(0, t - 1).long())[:, 0] + 1, 0)
+        parents.copy_(up)
+        depths.copy_(deep)
+        pos.copy_(torch.tensor([length - t - seed, 40 + seed, length // 2]))
+        x0.copy_(mk(b, t, c))
+
+    half = lambda r: torch.exp2(torch.floor(torch.log2(r.abs().clamp(min=2.0**-126))) - 8) * 1.001
+    with torch.no_grad():
+        draw(0)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        taken = 0
+        for seed in range(1, 5):
+            draw(seed)
+            held = kc.clone(), vc.clone()
+            wanted = step()[1].float().argmax(-1)  # the drafts do not feed the step: most of them hold what it wants
+            hit = (torch.rand(b, t, generator=g) < 0.7).to(dev)
+            tokens.copy_(torch.where(hit, wanted.gather(1, parents.clamp(0, t - 1).long()), 70 - wanted))
+            for c0, c1 in zip((kc, vc), held):
+                c0.copy_(c1)
+            if seed % 2:
+                graph.replay()
+                seen, logits, kept = outs
+            else:
+                seen, logits, kept = step()
+            k64, v64 = (x.double() for x in held)
+            for layer, ((qkv, q, k, v, a), (_, wq, wk, _)) in enumerate(zip(seen, layers)):
+                ref = qk_norm_rope_reference(*(x.double() for x in (qkv, wq, wk, cos, sin)), n_head=h, n_kv_head=hkv,
+                                             positions=pos[:, None] + depths)
+                for x, r in zip((q, k, v), ref):
+                    assert bool(((x.double() - r).abs() <= half(r) + 20 * 2.0**-24 * 32).all())
+                r = tree_attention_reference(*(x.double() for x in (q, k, v)), k64[layer], v64[layer], pos, parents)
+                assert bool(((a.double() - r).abs() <= half(r) + 5.5 * 2.0**-16 + 4.8e-5).all())
+            want = accept_drafts_reference(logits.float().cpu(), tokens.cpu(), parents.cpu())
+            assert all(torch.equal(x.cpu(), y) for x, y in zip(kept, want))
+            compact_cache_reference(k64, v64, pos, kept[0], kept[1])
+            assert torch.equal(kc.double(), k64) and torch.equal(vc.double(), v64)
+            taken += int(kept[1].sum()) - b
+        assert taken > 4
+        graph.reset()
