@@ -458,9 +458,10 @@ bool vectors_fit(const HeadsArgs& a, int esize) {
 
 int chunks_of(const HeadsArgs& a) { return (int)(cdiv(a.H, a.chunk) + 2 * cdiv(a.Hkv, a.chunk)); }
 
-// Tokens to a wave are at most 32; with few tokens a wave takes a head or two, so that the heads spread over the CUs. Forward in us
-// with 1, 2 and kChunk heads: 512 tokens of 36 heads of 64 3.8, 4.4, 6.4, 2048 of them 5.9, 6.2, 8.4, 4096 8.7, 8.4, 9.4; 8191 of
-// 48 heads of 128 47.9, 43.4, 38.8. The heads of one kind are cut evenly.
+// Tokens to a wave are at most 32; with few tokens a wave takes a head or two, so that the heads spread over the CUs. The forward
+// kernel's us with 1, 2 and kChunk heads, in turn with the backward, whose data is in the caches: 512 tokens of 36 heads of 64 3.8, 4.4,
+// 6.7, 2048 of them 6.0, 6.2, 8.4, 4096 8.7, 8.4, 9.4; 8191 of 48 heads of 128 46.8, 42.4, 39.0 (34.2 with no backward between). The
+// heads of one kind are cut evenly.
 void set_chunk(HeadsArgs& a) {
   const int64_t all = a.tokens * (a.H + 2 * a.Hkv);
   const int most = all < 32768 ? 1 : all < 196608 ? 2 : kChunk, heads = std::max(a.H, a.Hkv);

@@ -343,7 +343,8 @@ struct Cursor {
 
 // A node's value that is infinite or NaN counts for the rows that see it and for no other, but the products would have it times a
 // weight of 0 for those: it is left out there, and here is what such values of the nodes from .. to - 1 add to elements
-// d .. d + 3 of node t, which is there: along its line of parents.
+// d .. d + 3 of node t, which is there: along its line of parents. (Their weights, above 0, change nothing of that; one of a score of
+// -inf counts as above 0 too.)
 template <typename T>
 __device__ __forceinline__ f32x4 not_finite_of(const TreeArgs& a, int b, const T* vn, int t, int from, int to, int d) {
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -408,9 +409,11 @@ __device__ __forceinline__ void write_nodes(const TreeArgs& a, const T* kn, cons
 }
 
 // A row group of 16 NT rows, its steps dealt to W waves. Long caches: bound by HBM (8 sequences of 2047 to 8188 keys, 32 heads of
-// 128, 4 nodes, bf16: 103 us, 6.5 TB/s; two steps of 16 KB are under way in each of 8 waves a CU). Short ones: by the
-// chain of round trips (position, parents and rows, keys, LDS, store): 4 heads of 512 keys 10.5 us, and f32 (a wave has
-// a step or two) 39 rows for each of 2 heads of 64 over 747, 1868 and 2988 keys 12.4 us.
+// 128, 4 nodes, bf16: 104 us, 6.5 TB/s; two steps of 16 KB are under way in each of 8 waves a CU). Short ones: by what follows one
+// another in a wave with two or three steps. 4 heads of 512 keys of 128, bf16: 10.9 us, of them from inside 9.5: 0.5 to find the place,
+// 2.4 until the queries and ancestors are there, 4.7 for the steps (the first one's keys and values are on their way since the place
+// is known), 0.7 for the nodes' rows, 1.2 through LDS and out. f32, 39 rows for each of 2 heads of 64 over 747, 1868 and 2988 keys:
+// 12.7 us, of them 1.1, 3.5, 3.2, 0.1 and 1.9 (and the join).
 template <typename T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, D, NT>, kWavesPerSimd<T, D, NT>))) void tree_attn_kernel(TreeArgs a) {
   typedef Step<T, D> S;
@@ -665,11 +668,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kWavesPe
 //
 // A step is two clusters, the softmax of its scores (VALU) and its product with V and the next step's with K (matrix units), each
 // behind a barrier, and the second half of the waves is one cluster behind the first: of a SIMD's two waves one is on the
-// VALU while the other is on the matrix units. Bound by LDS and the matrix units, neither of which is fed without a pause: a step's
-// keys and values are read by all eight waves, 128 KB of each, at 128 bytes a clock and the transposing reads at 64, some 3100 of a
-// step's 5000 cycles (2.1 us); the products take 3000, 1000 of them those of the weights' rests (without these the kernel takes
-// 72 us). 64 rows to a wave would halve the reads and leave one wave to a SIMD, and nothing to set against its softmax. 16 sequences of
-// 1008 to 4032 keys, 8 key heads of 128, 256 rows each: 84 us, 34 GFLOP of nodes that are there in 81 of products.
+// VALU while the other is on the matrix units. Bound by LDS and the matrix units, neither of which is fed without a pause: of a
+// step's 2.9 us (256 heads of 1088 to 4160 keys) the reads of keys and values by all eight waves, 128 KB of each, at 128 bytes a clock
+// and the transposing ones at 64, take 3100 cycles, 1.3 us, and the products 3000, 1000 of them those of the weights' rests
+// (without these a step takes 2.3 us). 64 rows to a wave would halve the reads and leave one wave to a SIMD, and nothing to set against
+// its softmax. 16 sequences of 1008 to 4032 keys, 8 key heads of 128, 256 rows each: 84 us (without the rests 72), 34 GFLOP of nodes
+// that are there in 81 of products.
 template <int D>
 struct WideShape {
   static constexpr int W = D == 256 ? 4 : 8, KEYS = D == 256 ? 32 : 64, RB = 2 * D, PIECES = RB / 16, ROWS = 32 * W;
@@ -862,7 +866,8 @@ __global__ __launch_bounds__(64 * WideShape<D>::W) void tree_wide_kernel(TreeArg
       if (!mine) continue;
       // O, then the scores of the next step (behind the last one of zeros, for nothing), so that the weights are gone when those
       // arrive: reads from LDS are kept AHEAD operands ahead of the one that they feed, in this order (a read's latency is some six
-      // products; left to itself the compiler has every product wait for its own read).
+      // products; left to itself the compiler has every product wait for its own read). 4 and 5 are alike, 6 takes five registers more than
+      // there are at head dim 128 (the kernel's fastest run 86 us and 84).
       const char *ks = lds + (s + 1 - s0) % 4 * C::STAGE, *vs = lds + (s - s0) % 4 * C::STAGE;
       constexpr int PV = KEYS / 16 * D / 32, ALL = PV + NT * D / 16, AHEAD = 5;
       auto fetch = [&](int i) {
@@ -1046,9 +1051,11 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   const bool half = dtype == FERRITE_BF16;
   const int64_t rows = h / hkv * t;
   Plan p;
-  // Many rows share keys and values through LDS: 8 sequences of 4096 keys, 4 key heads of 128, 48 rows each 25.8 us and not 27.5,
-  // 64 rows 26.7 and 29.9, 96 rows 30.3 and 43.2; of 64 elements 64 rows 19.4 and 18.3, 96 rows 21.1 and 24.8; of 256
-  // elements 24 and 32 rows 36.6 and 37.7 against 32.9 and 35.0, 48 rows 41.6 and 52.8.
+  // Many rows share keys and values through LDS (the call's us so, and with 32 rows to a wave, 64 of 64 elements): 8 sequences of 4096
+  // keys, 4 key heads of 128 elements, 32 rows each 26.6 and 20.6, 48 rows 27.7 and 29.4, 64 rows 28.5 and 30.7, 96 rows 30.8 and
+  // 36.5, 128 rows 32.0 and 41.9; of 64 elements 64 rows 21.4 and 19.3, 96 rows 22.4 and 26.6; of 256 elements 24 and 32 rows 39.7 and
+  // 40.7 against 33.5 and 35.3, 48 rows 45.1 and 53.5, 64 rows 47.9 and 56.2. Few heads lose by it: 64 rows of one sequence's 4 heads
+  // over 2048 keys 19.9 and 15.5.
   p.wide = half && rows > (d == 64 ? 64 : 32);
   p.tiles = rows <= 16 ? 1 : rows <= 32 || d > 128 ? 2 : 4;
   p.waves = 4;
@@ -1061,9 +1068,10 @@ Plan plan_for(int64_t b, int64_t h, int64_t hkv, int64_t t, int64_t max_len, int
   const int per_cu = p.wide ? 1 : p.tiles == 1 ? (d == 64 ? 3 : d == 128 ? 2 : 1) : p.tiles == 2 && d == 64 ? 2 : 1;
   p.groups = 256 * per_cu;
   p.least = p.wide ? 2 : p.waves;
-  // A wide head takes some 12 us to begin and to store, and a step 1.9 (16 sequences of 1008 to 4032 keys, 8 heads each, 256
-  // rows: 77 us; with 0 it takes 90, with 4 or 8 80); else it is about a step of each wave (eight heads of 1024 keys 12.3 us and
-  // 14.3 with 0, f32, four nodes of four heads to each of 16 heads 33.4 and 44.3, and none slower).
+  // A wide head takes some 12 us to begin and to store, and a step 2.9 (16 sequences of 1008 to 4032 keys, 8 heads each, 256
+  // rows, the kernel's fastest run: 85 us; with 0 it takes 101, with 4 85, with 8 87); else it is about a step of each wave (eight heads
+  // of 1024 keys 12.3 us and 14.3 with 0, f32, 32 nodes of four heads to each of 16 key heads of 1024 keys 33.4 and 44.3, and none
+  // slower).
   p.begin = p.wide ? 6 : p.waves;
   const bool eight = !p.wide && p.tiles == 1 && d <= 128;
   // Whole heads need no second kernel. Short ones, or many, lose less by uneven shares than that one costs: 256 heads of 1024
