@@ -75,7 +75,7 @@ CASES = [
     (2, 13, 2, 1, 2, 2, F32, False),
     (1, 21, 3, 1, 130, 130, BF16, False),  # by elements, over 128
     (1, 5, 1, 1, 258, 4, F32, False),
-    (9, 700, 7, 3, 64, 64, BF16, False),   # four heads to a wave
+    (9, 700, 7, 3, 64, 64, BF16, False),   # two heads to a wave
     (4, 701, 9, 5, 8, 8, F32, False),
 ]
 

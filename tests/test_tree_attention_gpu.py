@@ -63,9 +63,9 @@ CASES = [
     (3, 4, 4, 8, 512, 128, BF16, [504, 0, 31]),
     (3, 4, 2, 5, 512, 256, BF16, [507, 32, 33]),
     (2, 3, 1, 7, 700, 64, BF16, [693, 128]),          # 21 rows: two tiles
-    (2, 8, 2, 16, 1000, 128, BF16, [984, 511]),       # 64 rows: four tiles
-    (2, 8, 1, 13, 1000, 128, BF16, [512, 513]),       # 104 rows: two row blocks, the second short
-    (1, 16, 1, 64, 600, 64, BF16, [536]),             # 1024 rows
+    (2, 8, 2, 16, 1000, 128, BF16, [984, 511]),       # 64 rows: they share keys through LDS
+    (2, 8, 1, 13, 1000, 128, BF16, [512, 513]),       # 104 rows, of the 256 that share keys
+    (1, 16, 1, 64, 600, 64, BF16, [536]),             # 1024 rows: four row groups
     (2, 6, 1, 64, 900, 256, BF16, [836, 640]),
     (2, 32, 32, 4, 4100, 128, BF16, [4096, 1]),
     (9, 64, 64, 3, 2050, 64, BF16, [2047, 0, 1, 127, 128, 129, 1023, 1024, 2000]),
