@@ -33,7 +33,8 @@ def accept_drafts(logits, tokens, parents):
     token is the argmax of the node's logits (of equal logits the lowest token, NaN above all, as
     torch.argmax; of equal children the lowest node) until there is none: ``path`` are the ``count`` nodes visited, -1
     behind them, and ``next_token`` the argmax at the last, which no draft held. A node whose parent is not -1 or an earlier
-    node is absent: its logits are not read. Where node 0 is absent nothing is accepted: count 0, next_token -1."""
+    node is absent: its logits are not read. Where node 0 is absent nothing is accepted: count 0, next_token -1. Logits that are
+    not dense (a slice of a padded vocabulary) are copied first."""
     if logits.ndim != 3 or not 1 <= logits.shape[1] <= MAX_NODES or logits.shape[2] < 1:
         raise ValueError(f"expected logits as [B, T, V] with 1 to {MAX_NODES} nodes; got {tuple(logits.shape)}")
     _check_ints("tokens", tokens, logits.shape[:2], (torch.int64, torch.int32))

@@ -28,7 +28,7 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, pos, parents, *, scale: fl
     does not touch its output, NaN and infinities included. A sequence whose rows pos .. pos + T - 1 do not lie in the cache
     writes nothing and yields NaN. Scores and softmax are f32. There is no gradient (as for decode_attention). The caches
     must not overlap each other or the memory from the first element of q, k_new or v_new to its last: RuntimeError. B and H are
-    at most 65535."""
+    at most 65535. q, k_new and v_new are read as they lie where rows are dense and start at 16-byte boundaries, else copied first."""
     if q.ndim != 4 or k_new.ndim != 4 or v_new.shape != k_new.shape or k_new.shape[0] != q.shape[0] \
             or k_new.shape[2:] != q.shape[2:] or k_new.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k_new.shape[1]:
         raise ValueError(f"expected q as [B, H, T, D] and k_new, v_new as [B, Hkv, T, D] with H a multiple of Hkv; got "
