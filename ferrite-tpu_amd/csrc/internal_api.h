@@ -138,4 +138,20 @@ int ferrite_internal_compact_cache(void* k_cache, void* v_cache, const int32_t* 
                                    const int32_t* count, int64_t layers, int64_t b, int64_t h, int64_t max_len, int64_t d,
                                    int64_t t, int dtype, void* stream);
 
+/*
+ * Layer norm of rows of h = x + r (rounded to x's type and stored; h = x without r): y = (h - mean) rstd w + b. w and b (or
+ * null) [dim] of w_dtype. stats, or null, receives f32 (mean, rstd) of each row. 1 <= dim < 2^25; any alignment.
+ */
+int ferrite_internal_layernorm(const void* x, const void* r, const void* w, const void* b, void* h, void* y, float* stats,
+                               int64_t rows, int64_t dim, int x_dtype, int w_dtype, float eps, void* stream);
+/*
+ * Its gradients from dy, dd (h's own gradient, or null) and the forward's h and stats: dh, of x and r alike, and dw and db (or null), in
+ * w_dtype, summed in f32 in a fixed order. The workspace has ferrite_internal_layernorm_bwd_workspace(...) bytes (-1: sizes out of
+ * range); its content need not survive the call.
+ */
+int64_t ferrite_internal_layernorm_bwd_workspace(int64_t rows, int64_t dim);
+int ferrite_internal_layernorm_bwd(const void* h, const void* w, const void* dy, const void* dd, const float* stats, void* dh,
+                                   void* dw, void* db, int64_t rows, int64_t dim, int x_dtype, int w_dtype, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
 }  // extern "C"

@@ -170,6 +170,75 @@ std::tuple<Tensor, Tensor> add_rmsnorm(const Tensor& x, const Tensor& r, const T
 }
 
 // ---------------------------------------------------------------------------
+// Layer norm and residual add + layer norm
+// ---------------------------------------------------------------------------
+// A parameter of a function that records a backward, where it has that one.
+const Tensor& or_none(const std::optional<Tensor>& t) {
+  static const Tensor& none = *new Tensor;
+  return t ? *t : none;
+}
+std::optional<Tensor> dense(const std::optional<Tensor>& t) { return t ? std::optional<Tensor>(t->contiguous()) : t; }
+
+// (h, y) of dense tensors and, where `stats` asks for them, the rows' means and inverse deviations; h is x without a residual.
+std::tuple<Tensor, Tensor> layernorm_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, double eps,
+                                             Tensor* stats) {
+  const int64_t dim = x.size(-1), rows = rows_of(x);
+  Tensor h = r.defined() ? at::empty(x.sizes(), x.options()) : x, y = at::empty(x.sizes(), x.options());
+  if (stats) *stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
+  check(ferrite_internal_layernorm(ptr(x), ptr(r), ptr(w), ptr(b), r.defined() ? ptr(h) : nullptr, ptr(y),
+                                   stats ? (float*)ptr(*stats) : nullptr, rows, dim, code(x), code(w), (float)eps,
+                                   stream_of(x)),
+        "ferrite_layernorm");
+  return {h, y};
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b,
+                               const std::optional<Tensor>& r, double eps) {
+    Tensor stats;
+    auto [h, y] = layernorm_forward(x, w, or_none(b), or_none(r), eps, &stats);
+    ctx->save_for_backward({h, w, stats});
+    ctx->saved_data["b"] = b.has_value();
+    ctx->saved_data["r"] = r.has_value();
+    ctx->set_materialize_grads(false);
+    if (r) return {h, y};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gs) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &h = s[0], &w = s[1];
+    const bool has_b = ctx->saved_data["b"].toBool(), has_r = ctx->saved_data["r"].toBool();
+    const Tensor g = gs.back(), d = has_r ? gs[0] : Tensor();
+    const Tensor dy = g.defined() ? g.to(h.scalar_type()).contiguous() : at::zeros_like(h);
+    const Tensor dd = d.defined() ? d.to(h.scalar_type()).contiguous() : Tensor();
+    const int64_t dim = h.size(-1), rows = rows_of(h);
+    Tensor dh = at::empty(h.sizes(), h.options()), dw = at::empty(w.sizes(), w.options()),
+           db = has_b ? at::empty(w.sizes(), w.options()) : Tensor();
+    const Tensor ws = bytes_on(ferrite_internal_layernorm_bwd_workspace(rows, dim), h);
+    check(ferrite_internal_layernorm_bwd(ptr(h), ptr(w), ptr(dy), ptr(dd), (const float*)ptr(s[2]), ptr(dh), ptr(dw),
+                                         ptr(db), rows, dim, code(h), code(w), ptr(ws), ws.defined() ? ws.numel() : 0,
+                                         stream_of(h)),
+          "ferrite_layernorm_bwd");
+    return {dh, dw, db, has_r ? dh : Tensor(), Tensor()};
+  }
+};
+
+// y, or (h, y) with a residual.
+variable_list layernorm(const Tensor& x0, const Tensor& w0, const std::optional<Tensor>& b0, const std::optional<Tensor>& r0,
+                        double eps) {
+  const Tensor x = x0.contiguous(), w = w0.contiguous();
+  const auto b = dense(b0), r = dense(r0);
+  const Tensor &bt = or_none(b), &rt = or_none(r);
+  if (records({&x, &w, b ? &bt : &x, r ? &rt : &x}) || has_tangent({&x, &w, b ? &bt : &x, r ? &rt : &x})) {
+    refuse_leaves_of_other_graphs({&x0, &w0, b0 ? &*b0 : &x0, r0 ? &*r0 : &x0}, "ferrite_layernorm");
+    return LayerNormFn::apply(x, w, b, r, eps);
+  }
+  auto [h, y] = layernorm_forward(x, w, bt, rt, eps, nullptr);
+  if (r) return {h, y};
+  return {y};
+}
+
+// ---------------------------------------------------------------------------
 // Flash attention
 // ---------------------------------------------------------------------------
 // Workspaces of the long-context split kernels (partial states and per-pair counts), kept per
@@ -723,6 +792,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   typedef py::call_guard<py::gil_scoped_release> nogil;  // as ctypes calls do
   m.def("rmsnorm", &rmsnorm, nogil());
   m.def("add_rmsnorm", &add_rmsnorm, nogil());
+  m.def("layernorm", &layernorm, nogil());
   m.def("flash", &flash, nogil());
   m.def("flash_forward", &flash_forward, nogil());
   m.def("flash_backward", &flash_backward, nogil());

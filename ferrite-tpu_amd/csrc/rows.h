@@ -1,0 +1,101 @@
+// Rows of any width and alignment in vectors of eight elements, for kernels that hold a row in registers.
+//
+// Chunk c of a row of dim >= 8 elements holds elements 8 c .. 8 c + 7. The last one of a width that is no multiple of 8 holds
+// the row's last eight elements instead: the first `skip` of them belong to the chunk before as well, are left
+// out of sums, and are stored twice with the same value. So no element is loaded or stored by itself, and rows that start at
+// odd elements take the same 16-byte accesses (which this GPU makes at any address) as aligned ones.
+#pragma once
+
+#include "common.h"
+
+namespace ferrite {
+namespace {
+
+struct Chunk {
+  int at, skip;
+  bool on;
+};
+__device__ __forceinline__ Chunk chunk_of(int c, int dim) {
+  const int at = min(8 * c, dim - 8);
+  return {at, 8 * c - at, 8 * c < dim};
+}
+
+// Vectors that may start at any element.
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// Eight elements of T as they lie in memory. Each byte of a row is touched once: the accesses are non-temporal.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<bf16> {
+  bf16x8 v;
+  __device__ __forceinline__ void load(const bf16* p) { v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8_any*>(p)); }
+  __device__ __forceinline__ void load_cached(const bf16* p) { v = *reinterpret_cast<const bf16x8_any*>(p); }
+  __device__ __forceinline__ void zero() { v = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u}); }
+  __device__ __forceinline__ void store(bf16* p) const { __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p)); }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (bf16)x[e];
+  }
+};
+template <>
+struct Eight<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p));
+    b = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p + 4));
+  }
+  __device__ __forceinline__ void load_cached(const float* p) {
+    a = *reinterpret_cast<const f32x4_any*>(p);
+    b = *reinterpret_cast<const f32x4_any*>(p + 4);
+  }
+  __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ void store(float* p) const {
+    __builtin_nontemporal_store(a, reinterpret_cast<f32x4_any*>(p));
+    __builtin_nontemporal_store(b, reinterpret_cast<f32x4_any*>(p + 4));
+  }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = a[e];
+      o[4 + e] = b[e];
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    a = f32x4{x[0], x[1], x[2], x[3]};
+    b = f32x4{x[4], x[5], x[6], x[7]};
+  }
+};
+
+// Sum over a group of G threads (a wave, or a whole workgroup of G), in every one of its threads. Two sums share the waits.
+template <int G>
+__device__ __forceinline__ void rows_sum(float& x, float& y, float (*lds)[16]) {
+  x = wave_sum(x);
+  y = wave_sum(y);
+  if constexpr (G > 64) {
+    __syncthreads();  // the previous sums have been read
+    if ((threadIdx.x & 63) == 0) {
+      lds[0][threadIdx.x >> 6] = x;
+      lds[1][threadIdx.x >> 6] = y;
+    }
+    __syncthreads();
+    x = y = 0.f;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) {
+      x += lds[0][w];
+      y += lds[1][w];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace ferrite

@@ -160,6 +160,9 @@ INTERNAL: dict[str, tuple] = {
         _c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _c_i64, _vp],
     ),
+    "ferrite_internal_layernorm": (_c_int, [*[_vp] * 7, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _vp]),
+    "ferrite_internal_layernorm_bwd_workspace": (_c_i64, [_c_i64] * 2),
+    "ferrite_internal_layernorm_bwd": (_c_int, [*[_vp] * 8, _c_i64, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp]),
     "ferrite_internal_compact_cache": (_c_int, [_vp, _vp, _vp, _vp, _vp, *[_c_i64] * 6, _c_int, _vp]),
 }
 
