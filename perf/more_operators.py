@@ -36,9 +36,12 @@ def _library():
         pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ferrite-tpu_amd")
         if pkg not in sys.path:
             sys.path.insert(0, pkg)
-        from ferrite.kernels import clip, embedding, layernorm, matmul
+        from ferrite.kernels.clip import clip_grad_norm_
+        from ferrite.kernels.embedding import embedding
+        from ferrite.kernels.layernorm import layernorm
+        from ferrite.kernels.matmul import linear
 
-        _calls = (layernorm.layernorm, matmul.linear, embedding.embedding, clip.clip_grad_norm_)
+        _calls = (layernorm, linear, embedding, clip_grad_norm_)
     return _calls
 
 
