@@ -154,4 +154,54 @@ int ferrite_internal_layernorm_bwd(const void* h, const void* w, const void* dy,
                                    void* dw, void* db, int64_t rows, int64_t dim, int x_dtype, int w_dtype, void* workspace,
                                    int64_t workspace_bytes, void* stream);
 
+/*
+ * norm = sqrt(sum of all squares) of n tensors grads[i] of numel[i] elements of dtypes[i], added in 64 bits in a fixed order; where
+ * it is a finite float and most / (norm + 1e-6) < 1 every element is multiplied by that. grads, numel and dtypes are host arrays,
+ * read before the call returns. The tensors must not overlap; any alignment. The workspace, 8-byte aligned, has
+ * ferrite_internal_clip_workspace(n) bytes (-1: n out of range); its content need not survive the call.
+ */
+int64_t ferrite_internal_clip_workspace(int64_t n_tensors);
+int ferrite_internal_clip(int64_t n_tensors, void* const* grads, const int64_t* numel, const int32_t* dtypes, double most,
+                          float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * out[i] = scale table[tokens[i]] in f32, rounded once to out_dtype; table [vocab, dim]. A token outside the table gives NaN.
+ * rows < 2^30, vocab < 2^31 - 1, dim <= 64 * 65535; any alignment.
+ */
+int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* out, int64_t rows, int64_t dim, int64_t vocab,
+                               float scale, int table_dtype, int out_dtype, void* stream);
+/*
+ * Its gradient: dtable[t] = scale times the sum of dy's rows of token t, in f32 in a fixed order, zero where there is none. Tokens
+ * outside the table, and `padding` (-1: none), add nothing. The workspace, 16-byte aligned, has
+ * ferrite_internal_embedding_bwd_workspace(...) bytes (-1: sizes out of range); its content need not survive the call.
+ */
+int64_t ferrite_internal_embedding_bwd_workspace(int64_t rows, int64_t dim, int64_t vocab);
+int ferrite_internal_embedding_bwd(const int64_t* tokens, const void* dy, void* dtable, int64_t rows, int64_t dim,
+                                   int64_t vocab, int64_t padding, float scale, int dy_dtype, int table_dtype,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * out[M,N] = act(x[M,K] . w[K,N] + bias) + residual: x, residual, out and aux of `dtype`, w of `w_dtype` (that of x, or float with a
+ * bf16 x of up to 64 rows, rounded as it is read), bias [N] of bias_dtype. bias, residual and aux may be null; aux receives the
+ * pre-activation. residual may be neither out nor overlap it. The workspace, 16-byte aligned, has
+ * ferrite_internal_linear_workspace(...) bytes (-1: sizes out of range); its content need not survive the call.
+ */
+#define FERRITE_ACT_NONE 0
+#define FERRITE_ACT_RELU 1
+#define FERRITE_ACT_GELU 2 /* tanh form */
+#define FERRITE_ACT_SILU 3
+int64_t ferrite_internal_linear_workspace(const void* x, const void* w, const void* out, int64_t m, int64_t n, int64_t k,
+                                          int dtype, int w_dtype);
+int ferrite_internal_linear(const void* x, const void* w, const void* bias, const void* residual, void* out, void* aux,
+                            int64_t m, int64_t n, int64_t k, int dtype, int w_dtype, int bias_dtype, int act, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+/*
+ * du = dy act'(u) and db, the sums of du's rows before its rounding, in f32 in a fixed order: [rows, dim] of `dtype`, db [dim] of
+ * bias_dtype or null. Without u du is dy, and is not written. The workspace for db has ferrite_internal_act_grad_workspace(...)
+ * bytes (-1: sizes out of range).
+ */
+int64_t ferrite_internal_act_grad_workspace(int64_t rows, int64_t dim);
+int ferrite_internal_act_grad(const void* dy, const void* u, void* du, void* db, int64_t rows, int64_t dim, int act, int dtype,
+                              int bias_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 }  // extern "C"

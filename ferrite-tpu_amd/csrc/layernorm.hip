@@ -245,6 +245,8 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
     const TX* __restrict__ h, const TW* __restrict__ w, const TX* __restrict__ dy, const TX* __restrict__ dd,
     const float* __restrict__ stats, TX* __restrict__ dh, float* __restrict__ part, int64_t rows, int dim, float inv_dim) {
   constexpr int kGroups = G < 256 ? 256 / G : 1;
+  // The widest rows leave no registers for the next row and the weights (up to 180 spilled).
+  constexpr bool kAhead = G * VPL < 2048;
   extern __shared__ float red[];  // [kGroups][dim] where there is more than one group
   __shared__ float lds[2][16];
   const int t = threadIdx.x % G, grp = threadIdx.x / G;
@@ -253,7 +255,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     ch[i] = chunk_of(t + G * i, dim);
-    if (ch[i].on) load_params(w, ch[i].at, wv[i]);
+    if (kAhead && ch[i].on) load_params(w, ch[i].at, wv[i]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
   }
@@ -268,13 +270,14 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
       if (ch[i].on) {
         hr[i].load(h + off + ch[i].at);
         gr[i].load(dy + off + ch[i].at);
-        if constexpr (DIRECT) dr[i].load(dd + off + ch[i].at);
+        if constexpr (DIRECT && kAhead) dr[i].load(dd + off + ch[i].at);
       }
   };
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + grp;
-  if (row < rows) load(row);
+  if (kAhead && row < rows) load(row);
   for (; row < rows; row += step) {
+    if (!kAhead) load(row);
     const int64_t off = row * dim;
     float cv[VPL][8], gv[VPL][8], dv[VPL][8];
     float rest = 0.f, sg = 0.f, sgc = 0.f, none = 0.f;
@@ -284,13 +287,14 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
       if (ch[i].on) {
         hr[i].get(cv[i]);
         gr[i].get(gv[i]);
-        if constexpr (DIRECT) dr[i].get(dv[i]);
+        if constexpr (DIRECT && kAhead) dr[i].get(dv[i]);
       }
-    if (row + step < rows) load(row + step);  // the next row's, under way during this one's sums
+    if (kAhead && row + step < rows) load(row + step);  // the next row's, under way during this one's sums
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (ch[i].on)
+      if (ch[i].on) {
+        if (!kAhead) load_params(w, ch[i].at, wv[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           cv[i][e] -= m;
@@ -300,6 +304,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
           sg += g;
           sgc += g * cv[i][e];
         }
+      }
     rows_sum<G>(rest, sg, lds);
     rows_sum<G>(sgc, none, lds);
     rest *= inv_dim;
@@ -307,6 +312,13 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (ch[i].on) {
+        if constexpr (!kAhead) {
+          load_params(w, ch[i].at, wv[i]);
+          if constexpr (DIRECT) {
+            dr[i].load(dd + off + ch[i].at);
+            dr[i].get(dv[i]);
+          }
+        }
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -391,31 +403,6 @@ __global__ __launch_bounds__(256) void layernorm_bwd_cols_kernel(const TX* __res
   part[((int64_t)blockIdx.y * 2 + 1) * dim + col] = db;
 }
 
-// dw (blockIdx.y 0) and db (1) from the partial rows: 64 columns to a workgroup, whose 16 waves each add every 16th row in
-// turn; the waves' sums are added in their order.
-template <typename TW>
-__global__ __launch_bounds__(1024) void layernorm_bwd_join_kernel(const float* __restrict__ part, TW* __restrict__ dw,
-                                                                  TW* __restrict__ db, int parts, int64_t dim) {
-  __shared__ float red[16][64];
-  TW* const out = blockIdx.y ? db : dw;
-  if (!out) return;
-  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + c;
-  float acc = 0.f;
-  if (col < dim) {
-#pragma unroll 8
-    for (int p = wave; p < parts; p += 16) acc += part[((int64_t)p * 2 + blockIdx.y) * dim + col];
-  }
-  red[wave][c] = acc;
-  __syncthreads();
-  if (wave == 0 && col < dim) {
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) sum += red[k][c];
-    out[col] = Elem<TW>::from_f32(sum);
-  }
-}
-
 // Partial rows: at least four rows to a group of the backward, at most two workgroups per CU.
 int bwd_parts(int64_t rows, const NormPlan& plan) {
   const int64_t groups = plan.group == 64 ? 4 : 1;
@@ -439,8 +426,7 @@ int norm_bwd_launch(const TX* h, const TW* w, const TX* dy, const TX* dd, const 
     hipLaunchKernelGGL((layernorm_bwd_cols_kernel<TX>), dim3((unsigned)cdiv(dim, 256), (unsigned)parts), dim3(256), 0, stream,
                        h, dy, stats, part, rows, dim);
   }
-  hipLaunchKernelGGL((layernorm_bwd_join_kernel<TW>), dim3((unsigned)cdiv(dim, 64), 2), dim3(1024), 0, stream, part, dw, db,
-                     parts, dim);
+  join_parts(part, dw, db, 2, parts, dim, stream);
   return check_launch("ferrite_layernorm_bwd");
 }
 

@@ -25,6 +25,7 @@
 #include "common.h"
 #include "gelu.h"
 #include "internal_api.h"
+#include "linear.h"
 #include "skinny.h"
 #include "splitk.h"
 
@@ -599,6 +600,7 @@ struct RagArgs {
   int ldx, ldy;
   int64_t slab;
   int vec_out;
+  LinArgs lin;  // of kEpiLinear, ragged or not
 };
 
 // out[M,N] (or, with a K split, the f32 partial slab of K slice blockIdx.x / tiles)
@@ -620,7 +622,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void gemm_dma_kernel(const 
   typedef OperandTile<YT> YTl;
   static_assert(BM == 256 || (BM == 128 && !XT), "128-row tiles need a k-contiguous x");
   static_assert(SLOTS == 2 || (SLOTS == 3 && BM == 128), "three LDS stages fit 128-row tiles only");
-  static_assert(EPI == kEpiNone || sizeof(TO) == 2, "the GELU epilogues write bf16");
+  static_assert(EPI == kEpiNone || sizeof(TO) == 2, "the epilogues write bf16");
   static_assert(W == 8 || (W == 4 && BM == 256), "four waves own 128 x 128 each of a 256-row tile");
   // W = 8: wave w owns rows (w / 4) BM/2 .., columns (w % 4) 64 ..; W = 4: wave w owns
   // rows (w / 2) 128 .., columns (w % 2) 128 .. (one wave per SIMD, accumulators in AGPRs).
@@ -755,6 +757,76 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void gemm_dma_kernel(const 
     }
   }
   wait_vmem<0>();  // the empty loads past the slice have landed too
+
+  if constexpr (EPI == kEpiLinear) {
+    // The stores below, with the sums left in f32 until bias, activation and residual are in: a lane takes eight columns of a row,
+    // two 16-byte chunks of the staged group, and has their biases from the start. A row group's residuals are
+    // loaded before it is staged.
+    constexpr int kRow = YF * 32 * 4, kChunks = kRow / 16, kLanesRow = YF * 4, kRows = 64 / kLanesRow;
+    static_assert(W * 32 * kRow <= SLOTS * kStageBytes, "every wave's row group fits the stage ring");
+    lds_barrier();
+    char* const ep = smem + wave * (32 * kRow);
+    const int c8 = lane % kLanesRow, n = n0 + wn0 + 8 * c8, there = min(N - n, 8);  // columns of the eight
+    const bf16* const res = static_cast<const bf16*>(rag.lin.residual);
+    float bv[8];
+    bias_eight(rag.lin, n, there, bv);
+#pragma unroll
+    for (int i = 0; i < XF; ++i) {
+      const int mg = m0 + wm0 + 32 * i + lane / kLanesRow;  // the lane's first row
+      Eight<bf16> rv[32 / kRows];
+      if (res && there == 8) {
+#pragma unroll
+        for (int rr = 0; rr < 32 / kRows; ++rr)
+          if (mg + rr * kRows < M) rv[rr].load(res + (int64_t)(mg + rr * kRows) * N + n);
+      }
+#pragma unroll
+      for (int j = 0; j < YF; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int ch = 8 * j + 2 * q + g;
+          *reinterpret_cast<f32x4*>(ep + l32 * kRow + ((ch ^ (l32 & (kChunks - 1))) * 16)) =
+              f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+        }
+#pragma unroll
+      for (int rr = 0; rr < 32 / kRows; ++rr) {
+        const int r = rr * kRows + lane / kLanesRow, m = mg + rr * kRows;
+        float v[8], t[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const f32x4 w4 = *reinterpret_cast<const f32x4*>(ep + r * kRow + (((2 * c8 + half) ^ (r & (kChunks - 1))) * 16));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * half + e] = w4[e] + bv[4 * half + e];
+        }
+        if (m >= M || there <= 0) continue;
+        const int64_t at = (int64_t)m * N + n;
+        if (there == 8) {
+          Eight<bf16> o;
+          if (aux) {
+            o.set(v);
+            o.store(aux + at);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = act_of(v[e], rag.lin.act);
+          if (res) {
+            rv[rr].get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
+          }
+          o.set(v);
+          o.store(out + at);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 7; ++e)
+            if (e < there) {
+              if (aux) aux[at + e] = (bf16)v[e];
+              const float y = act_of(v[e], rag.lin.act);
+              out[at + e] = (bf16)(res ? y + (float)res[at + e] : y);
+            }
+        }
+      }
+    }
+    return;
+  }
 
   // Epilogue: acc[j][i] is a C^T tile; register r of lane (l32, g) is
   // C[m0 + wm0 + 32 i + l32][n0 + wn0 + 32 j + (r / 4) * 8 + g * 4 + r % 4].
@@ -1026,9 +1098,11 @@ bool use_four_waves(int64_t M, int64_t N, int64_t cus) {
 
 template <typename TO, bool XT, bool YT, int EPI = kEpiNone>
 int launch_gemm_dma_t(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K, void* ws,
-                      int64_t ws_bytes, hipStream_t stream, void* aux = nullptr) {
+                      int64_t ws_bytes, hipStream_t stream, void* aux = nullptr, const LinArgs& lin = {}) {
   typedef Gemm2 G;
   bf16* const ax = static_cast<bf16*>(aux);
+  RagArgs args{};
+  args.lin = lin;
   const int64_t cus = cu_count(stream);
   if constexpr (!XT) {
     if (pick_bm(M, N, XT, cus) == 128) {
@@ -1039,7 +1113,7 @@ int launch_gemm_dma_t(const void* x, const void* y, void* out, int64_t M, int64_
       if (int rc = allow_lds((const void*)kern, kLds128, stream, "ferrite_matmul")) return rc;
       hipLaunchKernelGGL(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(G::kThreads), kLds128, stream,
                          static_cast<const bf16*>(x), static_cast<const bf16*>(y), static_cast<TO*>(out), (int)M,
-                         (int)N, (int)K, (int)tiles_m, (int)tiles_n, (int)K, ax, RagArgs{});
+                         (int)N, (int)K, (int)tiles_m, (int)tiles_n, (int)K, ax, args);
       return check_launch("ferrite_matmul");
     }
   }
@@ -1061,7 +1135,7 @@ int launch_gemm_dma_t(const void* x, const void* y, void* out, int64_t M, int64_
     if (int rc = allow_lds((const void*)kern, kLds, stream, "ferrite_matmul")) return rc;
     hipLaunchKernelGGL(kern, grid, dim3(w4 ? 256 : G::kThreads), kLds, stream, static_cast<const bf16*>(x),
                        static_cast<const bf16*>(y), static_cast<TO*>(out), (int)M, (int)N, (int)K, (int)tiles_m,
-                       (int)tiles_n, kslice, ax, RagArgs{});
+                       (int)tiles_n, kslice, ax, args);
   } else {
     auto kern = gemm_dma_kernel<float, XT, YT>;
     if (int rc = allow_lds((const void*)kern, kLds, stream, "ferrite_matmul")) return rc;
@@ -1069,8 +1143,11 @@ int launch_gemm_dma_t(const void* x, const void* y, void* out, int64_t M, int64_
                        static_cast<const bf16*>(y), static_cast<float*>(ws), (int)M, (int)N, (int)K, (int)tiles_m,
                        (int)tiles_n, kslice, nullptr, RagArgs{});
     const int64_t mn = M * N;
-    hipLaunchKernelGGL((gemm_splitk_reduce_kernel<TO, EPI>), dim3((unsigned)cdiv(mn / 4, 256)), dim3(256), 0, stream,
-                       static_cast<const float*>(ws), static_cast<TO*>(out), mn, slices, ax, mn);
+    if constexpr (EPI == kEpiLinear)
+      return linear_pass<TO>(static_cast<const float*>(ws), slices, mn, out, aux, lin, M, N, stream);
+    else
+      hipLaunchKernelGGL((gemm_splitk_reduce_kernel<TO, EPI>), dim3((unsigned)cdiv(mn / 4, 256)), dim3(256), 0, stream,
+                         static_cast<const float*>(ws), static_cast<TO*>(out), mn, slices, ax, mn);
   }
   return check_launch("ferrite_matmul");
 }
@@ -1213,9 +1290,9 @@ bool rag_better(const RagPlan& p, int64_t M, int64_t N, int64_t K, bool copies, 
   return p.slices > 1 || cdiv(M, (int64_t)Gemm2::BM) * cdiv(N, (int64_t)Gemm2::BN) >= cus / 4;
 }
 
-template <typename TO, bool XT, bool YT>
+template <typename TO, bool XT, bool YT, int EPI = kEpiNone>
 int launch_gemm_rag_t(const bf16* x, const bf16* y, TO* out, int64_t M, int64_t N, int64_t K, const RagPlan& p,
-                      char* ws, hipStream_t stream) {
+                      char* ws, hipStream_t stream, bf16* aux = nullptr) {
   typedef Gemm2 G;
   const int64_t cus = cu_count(stream);
   RagArgs args = p.args;
@@ -1226,11 +1303,11 @@ int launch_gemm_rag_t(const bf16* x, const bf16* y, TO* out, int64_t M, int64_t 
     if (pick_bm(M, N, XT, cus) == 128) {
       constexpr int kLds128 = 3 * (2 * GemmXTile::kSubBytes + OperandTile<YT>::kBytes);
       const int64_t tiles_m = cdiv(M, (int64_t)128);
-      auto kern = gemm_dma_kernel<TO, false, YT, 128, 3, kEpiNone, 8, true>;
+      auto kern = gemm_dma_kernel<TO, false, YT, 128, 3, EPI, 8, true>;
       if (int rc = allow_lds((const void*)kern, kLds128, stream, "ferrite_matmul")) return rc;
       hipLaunchKernelGGL(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(G::kThreads), kLds128, stream, x, y, out,
                          (int)M, (int)N, (int)K, (int)tiles_m, (int)tiles_n, (int)cdiv(K, (int64_t)G::BK) * G::BK,
-                         nullptr, args);
+                         aux, args);
       return check_launch("ferrite_matmul");
     }
   }
@@ -1241,36 +1318,43 @@ int launch_gemm_rag_t(const bf16* x, const bf16* y, TO* out, int64_t M, int64_t 
   auto go = [&](auto kern, auto* dst) {
     if (int rc = allow_lds((const void*)kern, kLds, stream, "ferrite_matmul")) return rc;
     hipLaunchKernelGGL(kern, grid, dim3(G::kThreads), kLds, stream, x, y, dst, (int)M, (int)N, (int)K, (int)tiles_m,
-                       (int)tiles_n, kslice, nullptr, args);
+                       (int)tiles_n, kslice, aux, args);
     return check_launch("ferrite_matmul");
   };
-  if (!split) return go(gemm_dma_kernel<TO, XT, YT, 256, 2, kEpiNone, 8, true>, out);
+  if (!split) return go(gemm_dma_kernel<TO, XT, YT, 256, 2, EPI, 8, true>, out);
   float* part = reinterpret_cast<float*>(ws + p.off_part);
   if (int rc = go(gemm_dma_kernel<float, XT, YT, 256, 2, kEpiNone, 8, true>, part)) return rc;
+  if constexpr (EPI == kEpiLinear) return linear_pass<TO>(part, p.slices, args.slab, out, aux, args.lin, M, N, stream);
   const int64_t mn = M * N;
   hipLaunchKernelGGL((gemm_splitk_reduce_kernel<TO>), dim3((unsigned)cdiv(mn, 1024)), dim3(256), 0, stream, part, out,
                      mn, p.slices, nullptr, args.slab);
   return check_launch("ferrite_matmul");
 }
 
+// The operands where the ragged kernel reads them: packed into the workspace where their rows are not aligned.
+int pack_operands(const void* x, const void* y, const RagPlan& p, char* wp, const bf16*& xp, const bf16*& yp,
+                  hipStream_t stream) {
+  xp = static_cast<const bf16*>(x);
+  yp = static_cast<const bf16*>(y);
+  if (!p.pack_x && !p.pack_y) return FERRITE_OK;
+  bf16* const px = reinterpret_cast<bf16*>(wp);
+  bf16* const py = reinterpret_cast<bf16*>(wp + p.off_y);
+  const PackJob a{xp, px, p.pack_x ? (uint32_t)(p.rows_x * (p.args.ldx / 8)) : 0u, (int)p.cols_x, p.args.ldx};
+  const PackJob b{yp, py, p.pack_y ? (uint32_t)(p.rows_y * (p.args.ldy / 8)) : 0u, (int)p.cols_y, p.args.ldy};
+  hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)cdiv((int64_t)a.chunks + b.chunks, (int64_t)256)), dim3(256), 0,
+                     stream, a, b);
+  if (p.pack_x) xp = px;
+  if (p.pack_y) yp = py;
+  return check_launch("ferrite_matmul");
+}
+
 template <typename TO>
 int launch_gemm_rag(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K, bool xt, bool yt,
                     RagPlan p, void* ws, hipStream_t stream) {
-  const bf16* xp = static_cast<const bf16*>(x);
-  const bf16* yp = static_cast<const bf16*>(y);
+  const bf16 *xp, *yp;
   char* wp = static_cast<char*>(ws);
   if (reinterpret_cast<uintptr_t>(out) & 7) p.slices = 1;  // the slabs' sum leaves in 8-byte stores
-  if (p.pack_x || p.pack_y) {
-    bf16* const px = reinterpret_cast<bf16*>(wp);
-    bf16* const py = reinterpret_cast<bf16*>(wp + p.off_y);
-    const PackJob a{xp, px, p.pack_x ? (uint32_t)(p.rows_x * (p.args.ldx / 8)) : 0u, (int)p.cols_x, p.args.ldx};
-    const PackJob b{yp, py, p.pack_y ? (uint32_t)(p.rows_y * (p.args.ldy / 8)) : 0u, (int)p.cols_y, p.args.ldy};
-    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)cdiv((int64_t)a.chunks + b.chunks, (int64_t)256)), dim3(256),
-                       0, stream, a, b);
-    if (int rc = check_launch("ferrite_matmul")) return rc;
-    if (p.pack_x) xp = px;
-    if (p.pack_y) yp = py;
-  }
+  if (int rc = pack_operands(x, y, p, wp, xp, yp, stream)) return rc;
   TO* o = static_cast<TO*>(out);
   if (xt && yt) return launch_gemm_rag_t<TO, true, true>(xp, yp, o, M, N, K, p, wp, stream);
   if (xt) return launch_gemm_rag_t<TO, true, false>(xp, yp, o, M, N, K, p, wp, stream);
@@ -1344,6 +1428,98 @@ extern "C" int ferrite_internal_linear_f32w(const void* x, const float* w, void*
   return skinny_launch({x, w, out, aux, m, n, k, w_t != 0, FERRITE_F32, out_dtype, aux ? kEpiGelu : kEpiNone, workspace,
                         workspace_bytes},
                        static_cast<hipStream_t>(stream));
+}
+
+namespace ferrite {
+namespace {
+// Which kernel takes a linear layer's product and what its workspace holds, as for the plain product: few rows, the DMA tiles,
+// those with packed operands; and what is left (f32, small unaligned bf16), whose product leaves in f32, in the output itself
+// or in the workspace's first part, for a pass of its own.
+struct LinearPlan {
+  enum Kind { kSkinny, kDma, kRagged, kPass } kind;
+  RagPlan rag;
+  int64_t product, bytes;  // bytes of the product's part, and in all
+};
+bool linear_plan(const void* x, const void* w, const void* out, int64_t m, int64_t n, int64_t k, int dtype, int w_dtype,
+                 int64_t cus, LinearPlan& p) {
+  p = LinearPlan{};
+  if (m < 1 || n < 1 || k < 1 || n > 0x7fffffff || m > ((int64_t)1 << 58) / n) return false;
+  if (dtype == FERRITE_BF16 && (w_dtype == FERRITE_F32 || use_skinny(x, w, out, m, n, k, false, false))) {
+    if (!skinny_ok(m, n, k)) return false;
+    p.kind = LinearPlan::kSkinny;
+    p.bytes = skinny_workspace({x, w, nullptr, nullptr, m, n, k, false, w_dtype, FERRITE_BF16, kEpiLinear, nullptr, 0});
+    return true;
+  }
+  if (dtype == FERRITE_BF16 && dma_ok(x, w, out, m, n, k, false, false)) {
+    p.kind = LinearPlan::kDma;
+    p.bytes = splitk_workspace(m, n, k, cus);
+    return true;
+  }
+  if (dtype == FERRITE_BF16 && rag_ok(m, n, k, false, false)) {
+    p.rag = rag_plan(x, w, m, n, k, false, false, cus);
+    if (rag_better(p.rag, m, n, k, false, cus)) {
+      p.kind = LinearPlan::kRagged;
+      p.bytes = p.rag.bytes;
+      return true;
+    }
+  }
+  p.kind = LinearPlan::kPass;
+  p.product = dtype == FERRITE_BF16 ? cdiv(m * n * 4, (int64_t)16) * 16 : 0;
+  p.bytes = p.product + (dtype == FERRITE_F32 && f32_small(m, n, cus) ? f32_workspace(m, n, k, cus) : 0);
+  return true;
+}
+}  // namespace
+}  // namespace ferrite
+
+extern "C" int64_t ferrite_internal_linear_workspace(const void* x, const void* w, const void* out, int64_t m, int64_t n,
+                                                     int64_t k, int dtype, int w_dtype) {
+  ferrite::LinearPlan p;
+  return ferrite::linear_plan(x, w, out, m, n, k, dtype, w_dtype, ferrite::cu_count_of(-1), p) ? p.bytes : -1;
+}
+
+extern "C" int ferrite_internal_linear(const void* x, const void* w, const void* bias, const void* residual, void* out,
+                                       void* aux, int64_t m, int64_t n, int64_t k, int dtype, int w_dtype, int bias_dtype,
+                                       int act, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ferrite;
+  const char* name = "ferrite_linear";
+  if (!valid_dtype(dtype) || !valid_dtype(w_dtype) || (bias && !valid_dtype(bias_dtype)) || (dtype == FERRITE_F32 && w_dtype != dtype))
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": dtypes not supported");
+  if (act < FERRITE_ACT_NONE || act > FERRITE_ACT_SILU)
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": unknown activation");
+  if (!x || !w || !out) return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": null pointer");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  LinearPlan p;
+  if (!linear_plan(x, w, out, m, n, k, dtype, w_dtype, cu_count(s), p))
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": sizes out of range");
+  const int64_t size = m * n * (dtype == FERRITE_BF16 ? 2 : 4);
+  if ((residual && overlap(residual, size, out, size)) || (aux && overlap(aux, size, out, size)) ||
+      (aux && residual && overlap(aux, size, residual, size)))
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": out, aux and residual overlap");
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(FERRITE_ERR_INVALID_ARGUMENT, std::string(name) + ": null, unaligned or small workspace");
+  const LinArgs lin{bias, residual, bias && bias_dtype == FERRITE_F32, act};
+  switch (p.kind) {
+    case LinearPlan::kSkinny:
+      return skinny_launch({x, w, out, aux, m, n, k, false, w_dtype, FERRITE_BF16, kEpiLinear, workspace, workspace_bytes, lin}, s);
+    case LinearPlan::kDma:
+      return launch_gemm_dma_t<bf16, false, false, kEpiLinear>(x, w, out, m, n, k, workspace, workspace_bytes, s, aux, lin);
+    case LinearPlan::kRagged: {
+      const bf16 *xp, *wp;
+      p.rag.args.lin = lin;
+      if (int rc = pack_operands(x, w, p.rag, static_cast<char*>(workspace), xp, wp, s)) return rc;
+      return launch_gemm_rag_t<bf16, false, false, kEpiLinear>(xp, wp, static_cast<bf16*>(out), m, n, k, p.rag,
+                                                               static_cast<char*>(workspace), s, static_cast<bf16*>(aux));
+    }
+    default:
+      break;
+  }
+  float* const product = static_cast<float*>(dtype == FERRITE_BF16 ? workspace : out);
+  char* const rest = static_cast<char*>(workspace) + p.product;
+  if (int rc = ferrite_hip_matmul_ex(x, w, product, m, n, k, 0, 0, dtype, FERRITE_F32, p.bytes > p.product ? rest : nullptr,
+                                     p.bytes - p.product, stream))
+    return rc;
+  if (dtype == FERRITE_BF16) return linear_pass<bf16>(product, 1, 0, out, aux, lin, m, n, s);
+  return linear_pass<float>(product, 1, 0, out, aux, lin, m, n, s);
 }
 
 extern "C" int64_t ferrite_hip_matmul_workspace(int64_t m, int64_t n, int64_t k, int in_dtype) {

@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <list>
 #include <mutex>
 #include <optional>
@@ -46,6 +47,7 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes_on(int64_t n, const Tensor& like) {
   return n > 0 ? at::empty({n}, like.options().dtype(at::kByte)) : Tensor();
 }
+int64_t size_of(const Tensor& ws) { return ws.defined() ? ws.numel() : 0; }
 // Whether autograd records a backward for a function of `inputs`.
 bool records(std::initializer_list<const Tensor*> inputs) {
   if (!at::GradMode::is_enabled()) return false;
@@ -216,7 +218,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
            db = has_b ? at::empty(w.sizes(), w.options()) : Tensor();
     const Tensor ws = bytes_on(ferrite_internal_layernorm_bwd_workspace(rows, dim), h);
     check(ferrite_internal_layernorm_bwd(ptr(h), ptr(w), ptr(dy), ptr(dd), (const float*)ptr(s[2]), ptr(dh), ptr(dw),
-                                         ptr(db), rows, dim, code(h), code(w), ptr(ws), ws.defined() ? ws.numel() : 0,
+                                         ptr(db), rows, dim, code(h), code(w), ptr(ws), size_of(ws),
                                          stream_of(h)),
           "ferrite_layernorm_bwd");
     return {dh, dw, db, has_r ? dh : Tensor(), Tensor()};
@@ -270,8 +272,6 @@ Tensor split_workspace(int pass, int64_t bytes, const Tensor& like) {
   if (w.kept.size() > 16) w.kept.pop_back();
   return t;
 }
-int64_t size_of(const Tensor& ws) { return ws.defined() ? ws.numel() : 0; }
-
 // O and the logsumexp [B, H, Sq] of dense [B, H, S, D] tensors.
 std::tuple<Tensor, Tensor> flash_forward(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, double scale) {
   const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), sk = k.size(2);
@@ -557,6 +557,69 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
+// act(x @ w + b) + r, with w rounded to x's dtype as LinearFn does. The backward's first step is elementwise: du = dy act'(u) from
+// the pre-activation u that the forward leaves beside its output, with the bias's sums; without an activation du is dy.
+Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act, const Tensor& u) {
+  const int64_t m = rows_of(x), k = w.size(0), n = w.size(1);
+  Tensor out = at::empty(with_last(x, n), x.options());
+  if (m == 0 || n == 0) return out;
+  const int64_t bytes = ferrite_internal_linear_workspace(ptr(x), ptr(w), ptr(out), m, n, k, code(x), code(w));
+  const Tensor ws = bytes_on(bytes, x);
+  check(ferrite_internal_linear(ptr(x), ptr(w), ptr(b), ptr(r), ptr(out), ptr(u), m, n, k, code(x), code(w),
+                                b.defined() ? code(b) : FERRITE_F32, (int)act, ptr(ws), size_of(ws), stream_of(x)),
+        "ferrite_linear");
+  return out;
+}
+
+struct LinearActFn : torch::autograd::Function<LinearActFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b,
+                        const std::optional<Tensor>& r, int64_t act) {
+    const Tensor wq = w.to(x.scalar_type());
+    Tensor u;
+    if (act != FERRITE_ACT_NONE) u = at::empty(with_last(x, w.size(1)), x.options());
+    const Tensor out = linear_act_forward(x, wq, or_none(b), or_none(r), act, u);
+    ctx->save_for_backward({x, wq, u});
+    ctx->saved_data["w"] = w.scalar_type();
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["r"] = r.has_value();
+    if (b) ctx->saved_data["b"] = b->scalar_type();
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gs) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &wq = s[1], &u = s[2];
+    const auto dt = x.scalar_type();
+    const Tensor g = gs[0].to(dt).contiguous();
+    const int64_t m = rows_of(x), k = wq.size(0), n = wq.size(1);
+    const bool has_b = ctx->saved_data.count("b");
+    Tensor du = g, db;
+    if (has_b) db = at::empty({n}, g.options().dtype(ctx->saved_data["b"].toScalarType()));
+    if ((u.defined() || has_b) && n > 0) {
+      if (u.defined()) du = at::empty(g.sizes(), g.options());
+      const Tensor ws = bytes_on(has_b ? ferrite_internal_act_grad_workspace(m, n) : 0, g);
+      check(ferrite_internal_act_grad(ptr(g), ptr(u), u.defined() ? ptr(du) : nullptr, ptr(db), m, n,
+                                      (int)ctx->saved_data["act"].toInt(), code(g), has_b ? code(db) : FERRITE_F32, ptr(ws),
+                                      size_of(ws), stream_of(g)),
+            "ferrite_linear_bwd");
+    }
+    return {mm(du, wq, m, k, n, false, true, dt, x.sizes()),
+            mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n}), db,
+            ctx->saved_data["r"].toBool() ? g : Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_act(const Tensor& x0, const Tensor& w0, const std::optional<Tensor>& b0, const std::optional<Tensor>& r0,
+                  int64_t act) {
+  const Tensor x = x0.contiguous(), w = w0.contiguous();
+  const auto b = dense(b0), r = dense(r0);
+  const Tensor &bt = or_none(b), &rt = or_none(r);
+  if (records({&x, &w, b ? &bt : &x, r ? &rt : &x}) || has_tangent({&x, &w, b ? &bt : &x, r ? &rt : &x})) {
+    refuse_leaves_of_other_graphs({&x0, &w0, b0 ? &*b0 : &x0, r0 ? &*r0 : &x0}, "ferrite_linear");
+    return LinearActFn::apply(x, w, b, r, act);
+  }
+  return linear_act_forward(x, reads_f32_weight(x, w) ? w : w.to(x.scalar_type()), bt, rt, act, Tensor());
+}
+
 // gelu(x @ w1) @ w2 with the GELU in the matmul epilogues, the weights rounded to bf16 as
 // LinearFn does. Forward: the up-projection stores u = x @ w1 and a = gelu(u) in one pass.
 // Backward: the product g @ w2^T is scaled by gelu'(u) as it is stored, so neither direction runs
@@ -665,6 +728,49 @@ struct EmbedFn : torch::autograd::Function<EmbedFn> {
 };
 Tensor embed_tokens(const Tensor& tokens, const Tensor& tok, const Tensor& pe, at::ScalarType dtype) {
   return EmbedFn::apply(tokens, tok, pe, dtype);
+}
+
+// Rows of a table by token, in `dtype`, and the table's gradient.
+Tensor embedding_forward(const Tensor& tokens, const Tensor& table, double scale, at::ScalarType dtype) {
+  auto shape = tokens.sizes().vec();
+  shape.push_back(table.size(1));
+  Tensor out = at::empty(shape, table.options().dtype(dtype));
+  check(ferrite_internal_embedding((const int64_t*)ptr(tokens), ptr(table), ptr(out), tokens.numel(), table.size(1),
+                                   table.size(0), (float)scale, code(table), code(dtype), stream_of(table)),
+        "ferrite_embedding");
+  return out;
+}
+
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale, int64_t pad,
+                        at::ScalarType dtype) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = pad;
+    ctx->saved_data["dtype"] = table.scalar_type();
+    ctx->saved_data["out"] = dtype;
+    return embedding_forward(tokens, table, scale, dtype);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gs) {
+    const Tensor tokens = ctx->get_saved_variables()[0];
+    const Tensor g = gs[0].to(ctx->saved_data["out"].toScalarType()).contiguous();
+    const int64_t rows = tokens.numel(), dim = g.size(-1), vocab = ctx->saved_data["vocab"].toInt();
+    Tensor d = at::empty({vocab, dim}, g.options().dtype(ctx->saved_data["dtype"].toScalarType()));
+    const Tensor ws = bytes_on(ferrite_internal_embedding_bwd_workspace(rows, dim, vocab), g);
+    check(ferrite_internal_embedding_bwd((const int64_t*)ptr(tokens), ptr(g), ptr(d), rows, dim, vocab,
+                                         ctx->saved_data["pad"].toInt(), (float)ctx->saved_data["scale"].toDouble(), code(g),
+                                         code(d), ptr(ws), size_of(ws), stream_of(g)),
+          "ferrite_embedding_bwd");
+    return {Tensor(), d, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& tokens0, const Tensor& table0, double scale, int64_t pad, at::ScalarType dtype) {
+  const Tensor tokens = tokens0.to(at::kLong).contiguous(), table = table0.contiguous();
+  if (!records({&table}) && !has_tangent({&table})) return embedding_forward(tokens, table, scale, dtype);
+  refuse_leaves_of_other_graphs({&table0}, "ferrite_embedding");
+  return EmbeddingFn::apply(tokens, table, scale, pad, dtype);
 }
 
 // q, k_new, v_new [B, H, D] are read as they lie when they share one stride per sequence and their
@@ -786,6 +892,40 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
 };
 Tensor cross_entropy(const Tensor& logits, const Tensor& targets) { return CrossEntropyFn::apply(logits, targets); }
 
+// ---------------------------------------------------------------------------
+// Gradient clipping
+// ---------------------------------------------------------------------------
+Tensor clip_grad_norm(const std::vector<Tensor>& grads, double most) {
+  const int64_t n = (int64_t)grads.size();
+  std::vector<void*> p(n);
+  std::vector<int64_t> numel(n);
+  std::vector<int32_t> dtypes(n);
+  std::vector<std::pair<const char*, const char*>> spans;
+  spans.reserve(n);
+  for (int64_t i = 0; i < n; ++i) {
+    const Tensor& g = grads[i];
+    if (!g.is_non_overlapping_and_dense())
+      throw py::value_error("clip_grad_norm_ scales tensors in place: each must be dense in memory");
+    p[i] = g.data_ptr();
+    numel[i] = g.numel();
+    dtypes[i] = code(g);
+    const char* at = static_cast<const char*>(p[i]);
+    if (numel[i]) spans.emplace_back(at, at + g.nbytes());
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second)
+      throw std::runtime_error("clip_grad_norm_: two of the tensors share memory");
+  Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const Tensor ws = bytes_on(ferrite_internal_clip_workspace(n), norm);
+  check(ferrite_internal_clip(n, p.data(), numel.data(), dtypes.data(), most, (float*)ptr(norm), ptr(ws), size_of(ws),
+                              stream_of(norm)),
+        "ferrite_clip_grad_norm");
+  for (const Tensor& g : grads)
+    if (!g.is_inference()) g.unsafeGetTensorImpl()->bump_version();  // a backward that has saved one finds out
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -800,15 +940,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope", &qk_norm_rope, nogil());
   m.def("matmul", &matmul, nogil());
   m.def("linear", &linear, nogil());
+  m.def("linear_act", &linear_act, nogil());
   m.def("mlp", &mlp, nogil());
   m.def("mm", &mm_2d, nogil());
   m.def("tied_logits", &tied_logits, nogil());
   m.def("embed", &embed, nogil());
   m.def("embed_tokens", &embed_tokens, nogil());
+  m.def("embedding", &embedding, nogil());
   m.def("decode_attention", &decode_attention, nogil());
   m.def("tree_attention", &tree_attention, nogil());
   m.def("accept_drafts", &accept_drafts, nogil());
   m.def("compact_cache", &compact_cache, nogil());
+  m.def("clip_grad_norm", &clip_grad_norm, nogil());
   m.def("cross_entropy", &cross_entropy, nogil());
   m.def("cross_entropy_rows", &cross_entropy_rows, nogil());
   m.def("cross_entropy_grad", &cross_entropy_grad, nogil());

@@ -76,6 +76,57 @@ struct Eight<float> {
   }
 };
 
+// Columns of W elements: eight, or one where a row has fewer than eight.
+template <typename T, int W>
+struct Cols;
+template <typename T>
+struct Cols<T, 8> : Eight<T> {};
+template <typename T>
+struct Cols<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = Elem<T>::to_f32(v); }
+  __device__ __forceinline__ void set(const float (&x)[1]) { v = Elem<T>::from_f32(x[0]); }
+};
+// First column of unit c of a row; -1 past it.
+template <int W>
+__device__ __forceinline__ int column(int c, int dim) {
+  if constexpr (W == 1) return c < dim ? c : -1;
+  const Chunk ch = chunk_of(c, dim);
+  return ch.on ? ch.at : -1;
+}
+
+// The sums of partial rows [parts][arrays][dim], array blockIdx.y of them into a or b (or none, where that is null): 64 columns to a
+// workgroup, whose 16 waves each add every 16th row in turn; the waves' sums are added in their order.
+template <typename T>
+__global__ __launch_bounds__(1024) void join_parts_kernel(const float* __restrict__ part, T* __restrict__ a, T* __restrict__ b,
+                                                          int parts, int64_t dim) {
+  __shared__ float red[16][64];
+  T* const out = blockIdx.y ? b : a;
+  if (!out) return;
+  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  float acc = 0.f;
+  if (col < dim) {
+#pragma unroll 8
+    for (int p = wave; p < parts; p += 16) acc += part[((int64_t)p * gridDim.y + blockIdx.y) * dim + col];
+  }
+  red[wave][c] = acc;
+  __syncthreads();
+  if (wave == 0 && col < dim) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += red[k][c];
+    out[col] = Elem<T>::from_f32(sum);
+  }
+}
+template <typename T>
+void join_parts(const float* part, T* a, T* b, int arrays, int parts, int64_t dim, hipStream_t stream) {
+  hipLaunchKernelGGL((join_parts_kernel<T>), dim3((unsigned)cdiv(dim, (int64_t)64), (unsigned)arrays), dim3(1024), 0, stream,
+                     part, a, b, parts, dim);
+}
+
 // Sum over a group of G threads (a wave, or a whole workgroup of G), in every one of its threads. Two sums share the waits.
 template <int G>
 __device__ __forceinline__ void rows_sum(float& x, float& y, float (*lds)[16]) {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.h"
+#include "linear.h"
 
 namespace ferrite {
 
@@ -10,8 +11,8 @@ constexpr int64_t kSkinnyRows = 64;
 
 // x bf16 [M,K]; w [K,N] (or, w_t, [N,K]) bf16, or float whose elements are rounded to bf16 as
 // they are read; out f32 or bf16 by out_dtype. epi: kEpiNone, kEpiGelu (a float w: not
-// transposed) or kEpiGeluGrad (bf16 w) of gelu.h with a bf16 out and aux. Any sizes and
-// element-aligned pointers.
+// transposed) or kEpiGeluGrad (bf16 w) of gelu.h with a bf16 out and aux, or kEpiLinear of linear.h (w not
+// transposed; aux may be null). Any sizes and element-aligned pointers.
 struct SkinnyArgs {
   const void* x;
   const void* w;
@@ -22,6 +23,7 @@ struct SkinnyArgs {
   int w_dtype, out_dtype, epi;
   void* ws;  // f32 partials of a K split, or nullptr
   int64_t ws_bytes;
+  LinArgs lin = {};
 };
 // Sizes the kernels take.
 bool skinny_ok(int64_t m, int64_t n, int64_t k);

@@ -62,7 +62,7 @@ __device__ __forceinline__ u32x4 load_x(__amdgpu_buffer_rsrc_t r, uint32_t row_o
 // 32 b + l32, j = (r / 4) * 8 + 4 g + r % 4.
 template <typename TO, int C, int MB, int EPI>
 __device__ __forceinline__ void reduce_store(const f32x16 (&acc)[C][MB], float* red, TO* out, bf16* aux, int M, int N,
-                                             int n0, int waves) {
+                                             int n0, int waves, const LinArgs& lin) {
   constexpr int kCols = 32 * C, kPitch = kCols + 1;  // an odd pitch: the 32 rows of a store on 32 banks
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -90,6 +90,11 @@ __device__ __forceinline__ void reduce_store(const f32x16 (&acc)[C][MB], float* 
         const bf16 u = (bf16)v;
         aux[at] = u;
         out[at] = (bf16)gelu_tanh((float)u);
+      } else if constexpr (EPI == kEpiLinear) {
+        v += bias_at(lin, n);
+        if (aux) aux[at] = (bf16)v;
+        v = act_of(v, lin.act);
+        out[at] = (bf16)(lin.residual ? v + (float)static_cast<const bf16*>(lin.residual)[at] : v);
       } else {
         out[at] = (bf16)((float)(bf16)v * gelu_tanh_grad((float)aux[at]));
       }
@@ -108,7 +113,7 @@ template <typename TW, typename TO, int C, int MB, int EPI, bool AL>
 __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_kernel(const bf16* __restrict__ x,
                                                                      const TW* __restrict__ w, TO* __restrict__ out,
                                                                      bf16* __restrict__ aux, int M, int N, int K,
-                                                                     int kslice, int64_t slab) {
+                                                                     int kslice, int64_t slab, LinArgs lin) {
   extern __shared__ float red[];
   // 128 registers for each of 16 waves
   constexpr int U = C * MB == 1 && AL ? 4 : C * MB < 4 ? 2 : 1;
@@ -177,7 +182,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_kernel(const bf16*
           mma32(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, xr[u][b]), acc[e][b]);
       }
   }
-  reduce_store<TO, C, MB, EPI>(acc, red, out, aux, M, N, n0, waves);
+  reduce_store<TO, C, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin);
 }
 
 // The 8 elements of a float w row from k0 + k, rounded to bf16.
@@ -208,7 +213,7 @@ template <typename TW, typename TO, int MB, int EPI, bool AL>
 __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_t_kernel(const bf16* __restrict__ x,
                                                                        const TW* __restrict__ w, TO* __restrict__ out,
                                                                        bf16* __restrict__ aux, int M, int N, int K,
-                                                                       int kslice, int64_t slab) {
+                                                                       int kslice, int64_t slab, LinArgs lin) {
   extern __shared__ float red[];
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_t_kernel(const bf1
           mma32(__builtin_bit_cast(bf16x8, wv[i]), __builtin_bit_cast(bf16x8, xv[i][b]), acc[0][b]);
     }
   }
-  reduce_store<TO, 1, MB, EPI>(acc, red, out, aux, M, N, n0, waves);
+  reduce_store<TO, 1, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin);
 }
 
 bool x_aligned(const SkinnyArgs& a) {
@@ -302,14 +307,14 @@ int go(Kern kern, const SkinnyArgs& a, const SkinnyPlan& p, hipStream_t stream, 
   if (int rc = allow_lds((const void*)kern, lds > 64 * 1024 ? 160 * 1024 : 64 * 1024, stream, "ferrite_matmul")) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.n, (int64_t)cols), (unsigned)p.slices), dim3(64 * waves), lds, stream,
                      static_cast<const bf16*>(a.x), static_cast<const TW*>(a.w), out, static_cast<bf16*>(a.aux),
-                     (int)a.m, (int)a.n, (int)a.k, p.kslice, p.slices > 1 ? slab_floats(a) : 0);
+                     (int)a.m, (int)a.n, (int)a.k, p.kslice, p.slices > 1 ? slab_floats(a) : 0, a.lin);
   return check_launch("ferrite_matmul");
 }
 
 template <typename TW, typename TO, int EPI, int MB, bool AL>
 int launch(const SkinnyArgs& a, const SkinnyPlan& p, TO* out, hipStream_t stream) {
   const TW* tw = nullptr;
-  if constexpr (sizeof(TW) == 2 || EPI == kEpiNone)
+  if constexpr ((sizeof(TW) == 2 && EPI != kEpiLinear) || EPI == kEpiNone)
     if (a.w_t) return go(gemm_skinny_t_kernel<TW, TO, MB, EPI, AL>, a, p, stream, tw, out);
   if constexpr (AL || MB == 1)
     if (p.cols == 2) return go(gemm_skinny_kernel<TW, TO, 2, MB, EPI, AL>, a, p, stream, tw, out);
@@ -339,16 +344,19 @@ int dispatch(const SkinnyArgs& a, hipStream_t stream) {
   // The sum of the slabs leaves in 8-byte stores, and its GELU needs whole fours.
   if (!a.ws || a.ws_bytes < p.slices * slab_floats(a) * (int64_t)sizeof(float) ||
       (reinterpret_cast<uintptr_t>(a.ws) & 15) || (reinterpret_cast<uintptr_t>(a.out) & 7) ||
-      (a.epi != kEpiNone && (a.m * a.n % 4 != 0 || (reinterpret_cast<uintptr_t>(a.aux) & 7)))) {
+      ((a.epi == kEpiGelu || a.epi == kEpiGeluGrad) && (a.m * a.n % 4 != 0 || (reinterpret_cast<uintptr_t>(a.aux) & 7)))) {
     p.slices = 1;
     p.kslice = (int)(cdiv(a.k, (int64_t)64) * 64);
   }
   if (p.slices > 1) {
     if (int rc = launch_al<TW, float, kEpiNone>(a, p, a.ws, stream)) return rc;
+    if (a.epi == kEpiLinear)
+      return linear_pass<bf16>(static_cast<const float*>(a.ws), p.slices, slab_floats(a), a.out, a.aux, a.lin, a.m, a.n, stream);
     if (a.epi == kEpiGelu) return sum_slices<bf16, kEpiGelu>(a, p, stream);
     if (a.epi == kEpiGeluGrad) return sum_slices<bf16, kEpiGeluGrad>(a, p, stream);
     return a.out_dtype == FERRITE_BF16 ? sum_slices<bf16, kEpiNone>(a, p, stream) : sum_slices<float, kEpiNone>(a, p, stream);
   }
+  if (a.epi == kEpiLinear) return launch_al<TW, bf16, kEpiLinear>(a, p, a.out, stream);
   if (a.epi == kEpiGelu) return launch_al<TW, bf16, kEpiGelu>(a, p, a.out, stream);
   if constexpr (sizeof(TW) == 2)
     if (a.epi == kEpiGeluGrad) return launch_al<TW, bf16, kEpiGeluGrad>(a, p, a.out, stream);

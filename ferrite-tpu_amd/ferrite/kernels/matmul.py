@@ -48,14 +48,47 @@ def matmul(x, y, *, block_m: int | None = None, block_n: int | None = None, bloc
     return _hip.autograd().matmul(x, y, out_dtype)
 
 
-def linear(x, w):
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}  # FERRITE_ACT_*
+
+
+def linear(x, w, *, bias=None, activation: str | None = None, residual=None):
     """``x @ w`` for ``x: [..., in]`` and ``w: [in, out]`` rounded to x's dtype, as
     ``matmul(x, w.to(x.dtype))`` computes it (model/gpt.py:95-104). Differentiable; a float
-    weight's gradient is not rounded."""
+    weight's gradient is not rounded.
+
+    With ``bias`` [out], ``activation`` ("relu", "gelu" in the tanh form, "silu") or ``residual`` [..., out] (the output's shape and
+    x's dtype), ``activation(x @ w + bias) + residual`` in the product's kernel: f32 up to the one rounding to x's dtype. x is
+    float32 or bf16 then, and a bias of either is not rounded. The backward reads the pre-activation, kept in x's dtype; the
+    gradient that enters the products is rounded to x's dtype, the bias's gradient is summed in f32 before that."""
     if x.ndim < 1 or w.ndim != 2 or x.shape[-1] != w.shape[0]:
         raise ValueError(f"expected [..., in] @ [in, out], got {tuple(x.shape)} @ {tuple(w.shape)}")
-    _hip.require_gpu(x, w)
-    return _hip.autograd().linear(x, w)
+    if bias is None and activation is None and residual is None:
+        _hip.require_gpu(x, w)
+        return _hip.autograd().linear(x, w)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be None, 'relu', 'gelu' or 'silu'; got {activation!r}")
+    if bias is not None and tuple(bias.shape) != (w.shape[1],):
+        raise ValueError(f"bias must have shape ({w.shape[1]},), got {tuple(bias.shape)}")
+    if residual is not None and (tuple(residual.shape) != (*x.shape[:-1], w.shape[1]) or residual.dtype != x.dtype):
+        raise ValueError(f"residual must be {(*x.shape[:-1], w.shape[1])} in {x.dtype}; got {tuple(residual.shape)} in {residual.dtype}")
+    if x.shape[-1] == 0:
+        raise RuntimeError("linear needs a non-empty inner dimension")
+    for t in (x, w, *(() if bias is None else (bias,))):
+        _hip.dtype_code(t.dtype)
+    _hip.require_gpu(*(t for t in (x, w, bias, residual) if t is not None))
+    return _hip.autograd().linear_act(x, w, bias, residual, ACTIVATIONS[activation])
+
+
+def linear_reference(x, w, *, bias=None, activation: str | None = None, residual=None):
+    """The same in torch operations, in f32 (f64 for a float64 x). Not used by the HIP path."""
+    work = torch.promote_types(x.dtype, torch.float32)
+    u = torch.matmul(x.to(work), w.to(x.dtype).to(work))
+    u = u if bias is None else u + bias.to(work)
+    if activation == "gelu":
+        u = torch.nn.functional.gelu(u, approximate="tanh")
+    elif activation is not None:
+        u = {"relu": torch.relu, "silu": torch.nn.functional.silu}[activation](u)
+    return (u if residual is None else u + residual.to(work)).to(x.dtype)
 
 
 def mlp_gelu(x, w1, w2):
