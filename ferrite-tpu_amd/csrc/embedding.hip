@@ -13,7 +13,7 @@
 //          behind whose 10 us (50 MB) it disappears. More rows: digits of up to 10 bits, stable, three launches each.
 //   sums   A wave adds a piece of kPiece rows of the order, 512 columns at a time, and stores each token's sum where the piece holds
 //          all of its rows; the first and the last of a piece may go on in its neighbours and leave a partial row.
-//   join   A workgroup adds the partial rows of a token that starts in its piece and goes on, its waves every 16th.
+//   join   A workgroup adds the partial rows of a token that starts in its piece and goes on.
 #include <math.h>
 
 #include <algorithm>
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(const int64_t* __restrict__
                                                      TO* __restrict__ out, int64_t total, int units, int dim, int64_t vocab,
                                                      float scale) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / units;
+    const int64_t row = total <= 0xffffffff ? (uint32_t)i / (uint32_t)units : i / units;
     const int at = column<W>((int)(i - row * units), dim);
     const int64_t t = tokens[row];
     float v[W];
@@ -74,42 +74,52 @@ __device__ __forceinline__ void fill_zero(char* p, int64_t bytes, int64_t block,
     __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, v + i);
 }
 
-// Workgroups 0 .. ranks - 1 order 64 rows each, an eighth of the comparisons to a wave; the others fill the table's gradient.
+// Workgroups 0 .. ranks - 1 order R rows each, a share of the comparisons to every R lanes; the others fill the table's gradient. R
+// goes with the rows so that the comparisons spread over the chip (rank_rows): 8192 rows by 64 17 us with the fill, by 32 RANK32.
+template <int R>
 __global__ __launch_bounds__(512) void rank_fill_kernel(const int64_t* __restrict__ tokens, uint32_t* __restrict__ keys,
                                                         uint32_t* __restrict__ order, int rows, int64_t vocab, int64_t pad,
                                                         int ranks, char* __restrict__ dtable, int64_t bytes) {
+  constexpr int kShares = 512 / R;
   extern __shared__ __attribute__((aligned(16))) uint32_t all[];  // [padded]: (token, index), no two alike
-  __shared__ uint32_t places[8][64];
+  __shared__ uint32_t places[kShares][R];
   if ((int)blockIdx.x >= ranks) {
     fill_zero(dtable, bytes, blockIdx.x - ranks, gridDim.x - ranks);
     return;
   }
-  const int padded = (rows + 31) / 32 * 32;
-  for (int i = threadIdx.x; i < padded; i += 512)
-    all[i] = i < rows ? (token_of(tokens[i], vocab, pad) << kIndexBits) | (uint32_t)i : 0xffffffffu;
+  const int share = (rows + 4 * kShares - 1) / (4 * kShares) * 4, padded = share * kShares;
+  for (int i0 = 0; i0 < padded; i0 += 8 * 512) {  // eight loads together: one by one they take 16 round trips for 8192 rows
+    int64_t t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = tokens[min(i0 + u * 512 + (int)threadIdx.x, rows - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * 512 + (int)threadIdx.x;
+      if (i < padded) all[i] = i < rows ? (token_of(t[u], vocab, pad) << kIndexBits) | (uint32_t)i : 0xffffffffu;
+    }
+  }
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mine = (int)blockIdx.x * 64 + lane;
+  const int r = threadIdx.x % R, part = threadIdx.x / R, mine = (int)blockIdx.x * R + r;
   const uint32_t key = all[min(mine, rows - 1)];
-  const int share = padded / 8;  // a multiple of 4
   uint32_t before = 0;
-  const u32x4* p = reinterpret_cast<const u32x4*>(all + wave * share);
+  const u32x4* p = reinterpret_cast<const u32x4*>(all + part * share);
 #pragma unroll 4
   for (int j = 0; j < share / 4; ++j) {
     const u32x4 k = p[j];
 #pragma unroll
     for (int e = 0; e < 4; ++e) before += k[e] < key;
   }
-  places[wave][lane] = before;
+  places[part][r] = before;
   __syncthreads();
-  if (wave == 0 && mine < rows) {
+  if (part == 0 && mine < rows) {
     uint32_t place = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) place += places[w][lane];
+    for (int w = 0; w < kShares; ++w) place += places[w][r];
     keys[place] = key >> kIndexBits;
     order[place] = key & (kRankRows - 1);
   }
 }
+int rank_rows(int64_t rows) { return rows > 8192 ? 64 : rows > 4096 ? 32 : 16; }
 
 __global__ __launch_bounds__(512) void fill_kernel(char* __restrict__ dtable, int64_t bytes) {
   fill_zero(dtable, bytes, blockIdx.x, gridDim.x);
@@ -295,7 +305,9 @@ __global__ __launch_bounds__(64) void token_sums_kernel(const uint32_t* __restri
   leave(behind == current);
 }
 
-// The token that goes on behind a piece in which it began: its partial rows, in 16 sums of every 16th piece, added in order.
+// The token that goes on behind a piece in which it began: its partial rows. Of few pieces each wave adds all of its columns'; of more
+// the waves share the pieces 4 or 16 ways, every 4th or 16th to one, and their sums are added in order. us for the 24
+// tokens over several pieces of 8192 (up to 50 pieces, 768 columns): 16 ways always 15.0, so 7.
 template <typename TO>
 __global__ __launch_bounds__(1024) void token_join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ slab,
                                                           TO* __restrict__ dtable, int64_t rows, int dim, uint32_t vocab,
@@ -316,24 +328,26 @@ __global__ __launch_bounds__(1024) void token_join_kernel(const uint32_t* __rest
   }
   // A piece that ends with the token's last row holds it too: the search went one too far if the piece it found begins with another.
   const int64_t last = keys[lo * piece] == token ? lo : lo - 1;
-  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int col0 = 0; col0 < dim; col0 += 64) {
-    const int col = col0 + c;
+  const int64_t pieces = last - blockIdx.x + 1;
+  const int ways = pieces <= 24 ? 1 : pieces <= 256 ? 4 : 16, groups = 16 / ways;
+  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6, way = wave / groups;
+  for (int col0 = 0; col0 < dim; col0 += 64 * groups) {
+    const int col = col0 + wave % groups * 64 + c;
     float acc = 0.f;
     if (col < dim) {
-#pragma unroll 4
-      for (int64_t p = blockIdx.x + wave; p <= last; p += 16)
+#pragma unroll 8
+      for (int64_t p = blockIdx.x + way; p <= last; p += ways)
         acc += slab[(p * 2 + (p == blockIdx.x ? 1 : 0)) * dim + col];
     }
-    __syncthreads();
-    red[wave][c] = acc;
-    __syncthreads();
-    if (wave == 0 && col < dim) {
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) sum += red[w][c];
-      dtable[(int64_t)token * dim + col] = Elem<TO>::from_f32(sum * scale);
+    if (ways > 1) {
+      __syncthreads();
+      red[wave][c] = acc;
+      __syncthreads();
+      if (way > 0) continue;
+      acc = 0.f;
+      for (int w = 0; w < ways; ++w) acc += red[w * groups + wave][c];
     }
+    if (col < dim) dtable[(int64_t)token * dim + col] = Elem<TO>::from_f32(acc * scale);
   }
 }
 
@@ -384,11 +398,14 @@ int embed_bwd(const int64_t* tokens, const T* dy, TO* dtable, int64_t rows, int6
   auto part = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
   uint32_t *keys = part(p.keys), *order = part(p.order);
   if (rows && p.rank) {
-    const int ranks = (int)cdiv(rows, 64);
-    const int lds = (int)(rows + 31) / 32 * 32 * 4;
-    if (int rc = allow_lds((const void*)rank_fill_kernel, kRankRows * 4, s, "ferrite_embedding_bwd")) return rc;
-    hipLaunchKernelGGL(rank_fill_kernel, dim3(ranks + fills), dim3(512), lds, s, tokens, keys, order, (int)rows, vocab, pad,
-                       ranks, reinterpret_cast<char*>(dtable), bytes);
+    const int r = rank_rows(rows), ranks = (int)cdiv(rows, (int64_t)r), lds = (int)cdiv(rows, 4 * (512 / r)) * 4 * (512 / r) * 4;
+    auto go = [&](auto kernel) {
+      if (int rc = allow_lds((const void*)kernel, kRankRows * 4, s, "ferrite_embedding_bwd")) return rc;
+      hipLaunchKernelGGL(kernel, dim3(ranks + fills), dim3(512), lds, s, tokens, keys, order, (int)rows, vocab, pad, ranks,
+                         reinterpret_cast<char*>(dtable), bytes);
+      return (int)FERRITE_OK;
+    };
+    if (int rc = r == 64 ? go(rank_fill_kernel<64>) : r == 32 ? go(rank_fill_kernel<32>) : go(rank_fill_kernel<16>)) return rc;
   } else {
     hipLaunchKernelGGL(fill_kernel, dim3(fills), dim3(512), 0, s, reinterpret_cast<char*>(dtable), bytes);
     if (rows == 0) return check_launch("ferrite_embedding_bwd");
