@@ -196,6 +196,14 @@ int ferrite_internal_linear(const void* x, const void* w, const void* bias, cons
                             int64_t m, int64_t n, int64_t k, int dtype, int w_dtype, int bias_dtype, int act, void* workspace,
                             int64_t workspace_bytes, void* stream);
 /*
+ * out[M,N] = op(x) . op(y) over f32 operands (x_t: x holds [K,M]; y_t: y holds [N,K]) of any alignment, read as they lie. The workspace,
+ * 16-byte aligned, has ferrite_internal_matmul_f32_workspace(...) bytes; with less K is not cut. -1: sizes that it does not take, or
+ * for which ferrite_hip_matmul_ex on untransposed operands is the faster one.
+ */
+int64_t ferrite_internal_matmul_f32_workspace(const float* x, const float* y, int64_t m, int64_t n, int64_t k, int x_t, int y_t);
+int ferrite_internal_matmul_f32(const float* x, const float* y, float* out, int64_t m, int64_t n, int64_t k, int x_t, int y_t,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+/*
  * du = dy act'(u) and db, the sums of du's rows before its rounding, in f32 in a fixed order: [rows, dim] of `dtype`, db [dim] of
  * bias_dtype or null. Without u du is dy, and is not written. The workspace for db has ferrite_internal_act_grad_workspace(...)
  * bytes (-1: sizes out of range).

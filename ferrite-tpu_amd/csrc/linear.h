@@ -35,6 +35,39 @@ __device__ __forceinline__ float act_of(float u, int act) {
       return u;
   }
 }
+// The activation of eight values, its kind looked at once.
+__device__ __forceinline__ void act_eight(float (&v)[8], int act) {
+  if (act == FERRITE_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+  } else if (act == FERRITE_ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gelu_tanh(v[e]);
+  } else if (act == FERRITE_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= silu_gate(v[e]);
+  }
+}
+// The same of the sums acc[0 .. YF - 1][i] of a 32 x 32 product.
+template <int YF, int XF>
+__device__ __forceinline__ void act_sums(f32x16 (&acc)[YF][XF], int i, int act) {
+  if (act == FERRITE_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < YF; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = acc[j][i][r] < 0.f ? 0.f : acc[j][i][r];
+  } else if (act == FERRITE_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < YF; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = gelu_tanh(acc[j][i][r]);
+  } else if (act == FERRITE_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < YF; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] *= silu_gate(acc[j][i][r]);
+  }
+}
 // Past |u| = 64 both gates are 0 or 1 and the slopes are too; there the squares could overflow.
 __device__ __forceinline__ float act_slope(float u, int act) {
   if (act == FERRITE_ACT_RELU) return u > 0.f ? 1.f : u != u ? u : 0.f;
@@ -70,6 +103,25 @@ __device__ __forceinline__ void bias_eight(const LinArgs& a, int64_t n, int coun
     if (e < count) o[e] = bias_at(a, n + e);
 }
 
+// Four columns from n of N, the last one again past them.
+__device__ __forceinline__ void bias_four(const LinArgs& a, int n, int N, float* o) {
+  if (n + 4 <= N) {
+    if (a.bias_f32) {
+      const f32x4 v = *reinterpret_cast<const f32x4_any*>(static_cast<const float*>(a.bias) + n);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = v[e];
+    } else {
+      typedef bf16x4 bf16x4_any __attribute__((aligned(2)));
+      const bf16x4 v = *reinterpret_cast<const bf16x4_any*>(static_cast<const bf16*>(a.bias) + n);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (float)v[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = bias_at(a, min(n + e, N - 1));
+  }
+}
+
 // The second pass of a product that is cut along K, or that a kernel without this epilogue leaves in f32: `slices` slabs
 // added in order, then the epilogue. Eight elements a thread where rows hold whole eights, else one. With one slice
 // part and out may be the same.
@@ -99,8 +151,7 @@ __global__ __launch_bounds__(256) void linear_pass_kernel(const float* part, int
       o.set(v);
       o.store(aux + i);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = act_of(v[e], a.act);
+    act_eight(v, a.act);
     if (res) {
       o.load(res + i);
       o.get(t);

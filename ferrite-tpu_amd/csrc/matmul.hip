@@ -24,6 +24,7 @@
 
 #include "common.h"
 #include "gelu.h"
+#include "gemm_f32.h"
 #include "internal_api.h"
 #include "linear.h"
 #include "skinny.h"
@@ -700,7 +701,6 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void gemm_dma_kernel(const 
     for (int i = 0; i < XF; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
-
   const int xb = XTl::lane_base(lane);
   const int yb = YTl::lane_base(lane);
   // Per k-step of 16: NM products over YF y fragments (A operand) and XF x
@@ -720,8 +720,29 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void gemm_dma_kernel(const 
   // half of the stage with two slots, so the last lands before the next
   // barrier, and over the whole stage with three.
   constexpr int kDmaSpan = SLOTS == 3 ? NSLOT : NSLOT / 2;
+  // kEpiLinear's sums begin with the biases: register r of lane (l32, g) holds column 32 j + (r / 4) * 8 + 4 g + r % 4 of the wave's,
+  // of every row group. Their loads go out ahead of the first stages'.
+  float bias[EPI == kEpiLinear ? YF * 16 : 1];
+  if constexpr (EPI == kEpiLinear) {
+    if (rag.lin.bias) {
+#pragma unroll
+      for (int f = 0; f < YF * 4; ++f)
+        bias_four(rag.lin, n0 + wn0 + 32 * (f / 4) + 8 * (f % 4) + 4 * g, N, bias + 4 * f);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
   issue(0);
   if (SLOTS == 3 && nk > 1) issue(1);
+  if constexpr (EPI == kEpiLinear) {
+    if (rag.lin.bias) {
+#pragma unroll
+      for (int j = 0; j < YF; ++j)
+#pragma unroll
+        for (int i = 0; i < XF; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[j][i][r] = bias[16 * j + r];
+    }
+  }
   for (int kt = 0; kt < nk; ++kt) {
     if (SLOTS == 3 && kt + 1 < nk)
       wait_vmem<kDmaWave>();  // stage kt has landed; stage kt + 1 may be in flight
@@ -759,71 +780,81 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void gemm_dma_kernel(const 
   wait_vmem<0>();  // the empty loads past the slice have landed too
 
   if constexpr (EPI == kEpiLinear) {
-    // The stores below, with the sums left in f32 until bias, activation and residual are in: a lane takes eight columns of a row,
-    // two 16-byte chunks of the staged group, and has their biases from the start. A row group's residuals are
-    // loaded before it is staged.
-    constexpr int kRow = YF * 32 * 4, kChunks = kRow / 16, kLanesRow = YF * 4, kRows = 64 / kLanesRow;
-    static_assert(W * 32 * kRow <= SLOTS * kStageBytes, "every wave's row group fits the stage ring");
+    // The stores below, over three planes of a wave's own part of the ring: the pre-activations that aux gets; the residuals, which come in
+    // whole row segments and are added where the sums lie; the outputs. The biases are in the sums from the start.
+    constexpr int kRow = YF * 64, kChunks = kRow / 16, kRows = 64 / kChunks, kPlane = 32 * kRow;
+    static_assert(W * 3 * kPlane <= SLOTS * kStageBytes, "every wave's planes fit the stage ring");
     lds_barrier();
-    char* const ep = smem + wave * (32 * kRow);
-    const int c8 = lane % kLanesRow, n = n0 + wn0 + 8 * c8, there = min(N - n, 8);  // columns of the eight
+    char* const ep = smem + wave * (3 * kPlane);
     const bf16* const res = static_cast<const bf16*>(rag.lin.residual);
-    float bv[8];
-    bias_eight(rag.lin, n, there, bv);
-#pragma unroll
-    for (int i = 0; i < XF; ++i) {
-      const int mg = m0 + wm0 + 32 * i + lane / kLanesRow;  // the lane's first row
-      Eight<bf16> rv[32 / kRows];
-      if (res && there == 8) {
-#pragma unroll
-        for (int rr = 0; rr < 32 / kRows; ++rr)
-          if (mg + rr * kRows < M) rv[rr].load(res + (int64_t)(mg + rr * kRows) * N + n);
-      }
+    const int c = lane % kChunks, n = n0 + wn0 + c * 8, there = min(N - n, 8);  // the lane's chunk of a row: `there` columns
+    auto chunk_at = [&](char* plane, int row, int ch) { return plane + row * kRow + ((ch ^ (row & (kChunks - 1))) * 16); };
+    // A plane from the sums of group i, and its rows to memory.
+    auto stage = [&](char* plane, int i) {
 #pragma unroll
       for (int j = 0; j < YF; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int ch = 8 * j + 2 * q + g;
-          *reinterpret_cast<f32x4*>(ep + l32 * kRow + ((ch ^ (l32 & (kChunks - 1))) * 16)) =
-              f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-        }
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<bf16x4*>(chunk_at(plane, l32, 4 * j + q) + 8 * g) =
+              bf16x4{(bf16)acc[j][i][4 * q], (bf16)acc[j][i][4 * q + 1], (bf16)acc[j][i][4 * q + 2], (bf16)acc[j][i][4 * q + 3]};
+    };
+    auto leave = [&](char* plane, int i, bf16* to) {
 #pragma unroll
       for (int rr = 0; rr < 32 / kRows; ++rr) {
-        const int r = rr * kRows + lane / kLanesRow, m = mg + rr * kRows;
-        float v[8], t[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const f32x4 w4 = *reinterpret_cast<const f32x4*>(ep + r * kRow + (((2 * c8 + half) ^ (r & (kChunks - 1))) * 16));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * half + e] = w4[e] + bv[4 * half + e];
-        }
-        if (m >= M || there <= 0) continue;
-        const int64_t at = (int64_t)m * N + n;
-        if (there == 8) {
-          Eight<bf16> o;
-          if (aux) {
-            o.set(v);
-            o.store(aux + at);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = act_of(v[e], rag.lin.act);
-          if (res) {
-            rv[rr].get(t);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += t[e];
-          }
-          o.set(v);
-          o.store(out + at);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 7; ++e)
-            if (e < there) {
-              if (aux) aux[at + e] = (bf16)v[e];
-              const float y = act_of(v[e], rag.lin.act);
-              out[at + e] = (bf16)(res ? y + (float)res[at + e] : y);
-            }
-        }
+        const int r = rr * kRows + lane / kChunks, m = m0 + wm0 + 32 * i + r;
+        if (m >= M) continue;
+        const char* const from = chunk_at(plane, r, c);
+        bf16* const dst = to + (int64_t)m * N + n;
+        if (there >= 8)
+          __builtin_nontemporal_store(*reinterpret_cast<const bf16x8*>(from), reinterpret_cast<bf16x8_any*>(dst));
+        else if constexpr (RAG)
+#pragma clang loop unroll(disable)
+          for (int e = 0; e < there; ++e) dst[e] = reinterpret_cast<const bf16*>(from)[e];
       }
+    };
+    Eight<bf16> rv[32 / kRows];
+    auto fetch = [&](int i) {  // group i's residuals
+#pragma unroll
+      for (int rr = 0; rr < 32 / kRows; ++rr) {
+        const int m = m0 + wm0 + 32 * i + rr * kRows + lane / kChunks;
+        if (there >= 8 && m < M) rv[rr].load(res + (int64_t)m * N + n);
+      }
+    };
+    if (res) fetch(0);
+#pragma unroll
+    for (int i = 0; i < XF; ++i) {
+      if (aux) {
+        stage(ep, i);
+        leave(ep, i, aux);
+      }
+      act_sums(acc, i, rag.lin.act);
+      if (res) {
+        char* const plane = ep + kPlane;
+#pragma unroll
+        for (int rr = 0; rr < 32 / kRows; ++rr) {
+          const int r = rr * kRows + lane / kChunks;
+          char* const to = chunk_at(plane, r, c);
+          if (there >= 8) {
+            *reinterpret_cast<bf16x8*>(to) = rv[rr].v;
+          } else if constexpr (RAG) {
+            const int m = min(m0 + wm0 + 32 * i + r, M - 1);
+#pragma clang loop unroll(disable)
+            for (int e = 0; e < there; ++e) reinterpret_cast<bf16*>(to)[e] = res[(int64_t)m * N + n + e];
+          }
+        }
+        if (i + 1 < XF) fetch(i + 1);
+#pragma unroll
+        for (int j = 0; j < YF; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(chunk_at(plane, l32, 4 * j + q) + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[j][i][4 * q + e] += __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+          }
+      }
+      stage(ep + 2 * kPlane, i);
+      leave(ep + 2 * kPlane, i, out);
     }
     return;
   }
@@ -1433,13 +1464,29 @@ extern "C" int ferrite_internal_linear_f32w(const void* x, const float* w, void*
 namespace ferrite {
 namespace {
 // Which kernel takes a linear layer's product and what its workspace holds, as for the plain product: few rows, the DMA tiles,
-// those with packed operands; and what is left (f32, small unaligned bf16), whose product leaves in f32, in the output itself
-// or in the workspace's first part, for a pass of its own.
+// those with packed operands; f32 of any layout; and what is left (small unaligned bf16, f32 in whole tiles), whose product leaves
+// in f32, in the output itself or in the workspace's first part, for a pass of its own.
 struct LinearPlan {
-  enum Kind { kSkinny, kDma, kRagged, kPass } kind;
+  enum Kind { kSkinny, kDma, kRagged, kF32, kPass } kind;
   RagPlan rag;
   int64_t product, bytes;  // bytes of the product's part, and in all
+  int slices;              // of kF32
 };
+// Whether an f32 product goes to the kernel of any layout (gemm_f32.hip) or to this file's, which have transposed operands copied
+// first and load unaligned rows by single floats, but keep the matrix pipes fuller over whole tiles. us on one MI355X, theirs / any layout:
+//   few rows   64 x 512 x 2048 12.5 / 9.3, transposed w 20 / 9.2    1 x 4096 x 4096 25 / 35, transposed w 92 / 33
+//   unaligned  2100 x 1003 x 515 55 / 42, transposed w 62 / 42, x 71 / 42    16384 x 515 x 130 50 / 41, transposed x 101 / 40
+//   aligned    1000^3 25 / 36, transposed w 33 / 36, x 32 / 34    8192 x 768 x 768 96 / 98, 104 / 94, 134 / 105
+//   over two rounds of 128 x 128 tiles: 4096^3, transposed w 1020 / 1196    4096 x 4095 x 4097 1243 / 1364
+bool f32_any_better(const void* x, const void* y, int64_t m, int64_t n, int64_t k, bool xt, bool yt, int64_t cus) {
+  auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if (!f32_any_ok(m, n, k, xt, yt)) return false;
+  if (!xt && !yt && k % 4 == 0 && n % 4 == 0 && a16(x) && a16(y)) return m <= 64 && n * k <= (int64_t)1 << 21;
+  return cdiv(m, (int64_t)128) * cdiv(n, (int64_t)128) < 2 * cus;
+}
+int64_t f32_any_bytes(int64_t m, int64_t n, int slices) {
+  return slices > 1 ? slices * f32_any_slab(m, n) * (int64_t)sizeof(float) : 0;
+}
 bool linear_plan(const void* x, const void* w, const void* out, int64_t m, int64_t n, int64_t k, int dtype, int w_dtype,
                  int64_t cus, LinearPlan& p) {
   p = LinearPlan{};
@@ -1462,6 +1509,12 @@ bool linear_plan(const void* x, const void* w, const void* out, int64_t m, int64
       p.bytes = p.rag.bytes;
       return true;
     }
+  }
+  if (dtype == FERRITE_F32 && f32_any_better(x, w, m, n, k, false, false, cus)) {
+    p.kind = LinearPlan::kF32;
+    p.slices = f32_any_slices(m, n, k, cus);
+    p.bytes = f32_any_bytes(m, n, p.slices);
+    return true;
   }
   p.kind = LinearPlan::kPass;
   p.product = dtype == FERRITE_BF16 ? cdiv(m * n * 4, (int64_t)16) * 16 : 0;
@@ -1510,6 +1563,14 @@ extern "C" int ferrite_internal_linear(const void* x, const void* w, const void*
       return launch_gemm_rag_t<bf16, false, false, kEpiLinear>(xp, wp, static_cast<bf16*>(out), m, n, k, p.rag,
                                                                static_cast<char*>(workspace), s, static_cast<bf16*>(aux));
     }
+    case LinearPlan::kF32: {
+      float* const to = static_cast<float*>(p.slices > 1 ? workspace : out);
+      const int64_t slab = f32_any_slab(m, n);
+      if (int rc = f32_any_launch({static_cast<const float*>(x), static_cast<const float*>(w), to, m, n, k, false, false,
+                                   p.slices, slab}, s))
+        return rc;
+      return linear_pass<float>(to, p.slices, slab, out, aux, lin, m, n, s);
+    }
     default:
       break;
   }
@@ -1520,6 +1581,35 @@ extern "C" int ferrite_internal_linear(const void* x, const void* w, const void*
     return rc;
   if (dtype == FERRITE_BF16) return linear_pass<bf16>(product, 1, 0, out, aux, lin, m, n, s);
   return linear_pass<float>(product, 1, 0, out, aux, lin, m, n, s);
+}
+
+extern "C" int64_t ferrite_internal_matmul_f32_workspace(const float* x, const float* y, int64_t m, int64_t n, int64_t k,
+                                                        int x_t, int y_t) {
+  using namespace ferrite;
+  const int64_t cus = cu_count_of(-1);
+  if (m < 1 || n < 1 || k < 1 || !f32_any_better(x, y, m, n, k, x_t != 0, y_t != 0, cus)) return -1;
+  return f32_any_bytes(m, n, f32_any_slices(m, n, k, cus));
+}
+
+extern "C" int ferrite_internal_matmul_f32(const float* x, const float* y, float* out, int64_t m, int64_t n, int64_t k,
+                                           int x_t, int y_t, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ferrite;
+  const bool xt = x_t != 0, yt = y_t != 0;
+  if (!f32_any_ok(m, n, k, xt, yt)) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_internal_matmul_f32: sizes out of range");
+  if (!x || !y || !out) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_internal_matmul_f32: null pointer");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  int slices = f32_any_slices(m, n, k, cu_count(s));
+  if (!workspace || workspace_bytes < f32_any_bytes(m, n, slices) || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+      (reinterpret_cast<uintptr_t>(out) & 15))
+    slices = 1;
+  const int64_t slab = f32_any_slab(m, n), mn = m * n;
+  float* const part = static_cast<float*>(workspace);
+  if (int rc = f32_any_launch({x, y, slices > 1 ? part : out, m, n, k, xt, yt, slices, slab}, s)) return rc;
+  if (slices == 1) return FERRITE_OK;
+  if (cdiv(mn, 1024) > 0xffffffff / 256) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_internal_matmul_f32: output too large");
+  hipLaunchKernelGGL((gemm_splitk_reduce_kernel<float>), dim3((unsigned)cdiv(mn, 1024)), dim3(256), 0, s, part, out, mn,
+                     slices, nullptr, slab);
+  return check_launch("ferrite_matmul");
 }
 
 extern "C" int64_t ferrite_hip_matmul_workspace(int64_t m, int64_t n, int64_t k, int in_dtype) {

@@ -571,6 +571,23 @@ Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Tensor& b, con
   return out;
 }
 
+// The backward's products, `mm` with its conversions where f32 has no kernel for the sizes.
+Tensor linear_mm(const Tensor& x, const Tensor& y, int64_t m, int64_t n, int64_t k, bool x_t, bool y_t,
+                 at::ScalarType out_dtype, at::IntArrayRef shape) {
+  if (x.scalar_type() == at::kFloat && y.scalar_type() == at::kFloat) {
+    const int64_t bytes = ferrite_internal_matmul_f32_workspace((const float*)ptr(x), (const float*)ptr(y), m, n, k, x_t, y_t);
+    if (bytes >= 0) {
+      Tensor out = at::empty(shape, x.options());
+      const Tensor ws = bytes_on(bytes, x);
+      check(ferrite_internal_matmul_f32((const float*)ptr(x), (const float*)ptr(y), (float*)ptr(out), m, n, k, x_t, y_t, ptr(ws),
+                                        size_of(ws), stream_of(x)),
+            "ferrite_matmul");
+      return out.to(out_dtype);
+    }
+  }
+  return mm(x, y, m, n, k, x_t, y_t, out_dtype, shape);
+}
+
 struct LinearActFn : torch::autograd::Function<LinearActFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b,
                         const std::optional<Tensor>& r, int64_t act) {
@@ -602,8 +619,8 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
                                       size_of(ws), stream_of(g)),
             "ferrite_linear_bwd");
     }
-    return {mm(du, wq, m, k, n, false, true, dt, x.sizes()),
-            mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n}), db,
+    return {linear_mm(du, wq, m, k, n, false, true, dt, x.sizes()),
+            linear_mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n}), db,
             ctx->saved_data["r"].toBool() ? g : Tensor(), Tensor()};
   }
 };

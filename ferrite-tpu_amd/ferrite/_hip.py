@@ -168,6 +168,8 @@ INTERNAL: dict[str, tuple] = {
         _c_int,
         [*[_vp] * 6, *[_c_i64] * 3, _c_int, _c_int, _c_int, _c_int, _vp, _c_i64, _vp],
     ),
+    "ferrite_internal_matmul_f32_workspace": (_c_i64, [_vp, _vp, *[_c_i64] * 3, _c_int, _c_int]),
+    "ferrite_internal_matmul_f32": (_c_int, [_vp, _vp, _vp, *[_c_i64] * 3, _c_int, _c_int, _vp, _c_i64, _vp]),
     "ferrite_internal_act_grad_workspace": (_c_i64, [_c_i64] * 2),
     "ferrite_internal_act_grad": (_c_int, [*[_vp] * 4, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp, _c_i64, _vp]),
     "ferrite_internal_embedding": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _c_int, _vp]),
