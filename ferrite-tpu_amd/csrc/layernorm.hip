@@ -226,12 +226,17 @@ int norm_launch(const TX* x, const TX* r, const TW* w, const TW* b, TX* h, TX* y
                        stream, x, r, w, b, h, y, stats, rows, dim, inv_dim, eps);
     return check_launch("ferrite_layernorm");
   }
-  FERRITE_NORM_CASE(plan, constexpr int D = G > 64 ? 1 : VPL == 1 ? 4 : VPL == 2 ? 2 : 1;
-                    constexpr int kGroups = G < 256 ? 256 / G : 1; const int64_t most = G > 256 ? 512 : G > 64 ? 2048 : 1024;
-                    hipLaunchKernelGGL((layernorm_kernel<TX, TW, RES, VPL, G, D>),
-                                       dim3((unsigned)std::min<int64_t>(cdiv(rows, (int64_t)kGroups * D), most)),
-                                       dim3(G < 256 ? 256 : G), 0, stream, x, r, w, b, h, y, stats, rows, (int)dim, inv_dim,
-                                       eps));
+  // Two rows of a wave under way where there are rows for it and they are short in bytes. us, add and norm, a row at a time / two:
+  // 8192 x 768 bf16 13.1 / 11.1, 500 x 1024 bf16 4.3 / 6.3, 3001 x 1003 f32 (no add) 7.0 / 7.7. Four of 512 columns: 32768 rows 25.1
+  // / 28.1 (4). At most eight workgroups of four waves per CU; with four 8192 x 2048 bf16 33.0 and not 28.6.
+  FERRITE_NORM_CASE(plan, constexpr int kGroups = G < 256 ? 256 / G : 1; auto go = [&](auto kernel, int64_t depth) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(cdiv(rows, kGroups * depth), G > 256 ? 512 : 2048)),
+                       dim3(G < 256 ? 256 : G), 0, stream, x, r, w, b, h, y, stats, rows, (int)dim, inv_dim, eps);
+  };
+                    if constexpr (sizeof(TX) == 2 && VPL == 2 && G == 64) {
+                      if (rows >= 4096) return go(layernorm_kernel<TX, TW, RES, VPL, G, 2>, 2);
+                    };
+                    go(layernorm_kernel<TX, TW, RES, VPL, G, 1>, 1));
   return check_launch("ferrite_layernorm");
 }
 
@@ -403,10 +408,13 @@ __global__ __launch_bounds__(256) void layernorm_bwd_cols_kernel(const TX* __res
   part[((int64_t)blockIdx.y * 2 + 1) * dim + col] = db;
 }
 
-// Partial rows: at least four rows to a group of the backward, at most two workgroups per CU.
-int bwd_parts(int64_t rows, const NormPlan& plan) {
+// Partial rows: one to a CU, and two where the columns are few and the rows many; a row to a group at least. More of them cost more
+// than they bring. us, one / two to a CU: 8192 x 768 bf16 17.1 / 17.4, 32768 x 512 36 / 30, 8192 x 2048 33.3 / 40.7, 2000 x 8192 f32 54 / 68;
+// 64 x 768 in 16 groups of four rows 9.5, of one 6.8.
+int bwd_parts(int64_t rows, int64_t dim, const NormPlan& plan) {
   const int64_t groups = plan.group == 64 ? 4 : 1;
-  return (int)std::clamp<int64_t>(cdiv(rows, groups * 4), 1, kBwdParts);
+  const int64_t one = std::min<int64_t>(cdiv(rows, groups), kBwdParts / 2);
+  return (int)std::max<int64_t>(one, dim <= 1024 ? std::min<int64_t>(cdiv(rows, groups * 8), kBwdParts) : 1);
 }
 
 template <typename TX, typename TW, bool DIRECT>
@@ -414,7 +422,7 @@ int norm_bwd_launch(const TX* h, const TW* w, const TX* dy, const TX* dd, const 
                     float* part, int64_t rows, int64_t dim, hipStream_t stream) {
   const float inv_dim = (float)(1.0 / (double)dim);
   const NormPlan plan = norm_plan(dim);
-  const int parts = rows ? bwd_parts(rows, plan) : 0;
+  const int parts = rows ? bwd_parts(rows, dim, plan) : 0;
   if (rows && plan.group) {
     FERRITE_NORM_CASE(plan, const size_t lds = G < 256 ? (size_t)(256 / G) * dim * 4 : 0;
                       hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TW, DIRECT, VPL, G>), dim3((unsigned)parts),
@@ -469,7 +477,7 @@ extern "C" int ferrite_internal_layernorm(const void* x, const void* r, const vo
 extern "C" int64_t ferrite_internal_layernorm_bwd_workspace(int64_t rows, int64_t dim) {
   using namespace ferrite;
   if (!norm_ok(rows, dim)) return -1;
-  return rows ? (int64_t)bwd_parts(rows, norm_plan(dim)) * 2 * dim * 4 : 0;
+  return rows ? (int64_t)bwd_parts(rows, dim, norm_plan(dim)) * 2 * dim * 4 : 0;
 }
 
 extern "C" int ferrite_internal_layernorm_bwd(const void* h, const void* w, const void* dy, const void* dd,
