@@ -3,7 +3,8 @@
 // Reference: src/ferrite/model/gpt.py:124-127 (the token embedding) and its autodiff backward, which XLA runs as a gather and a
 // scatter-add. The kernels of layout.hip take vocabularies of up to 1024 tokens with a position table; these any vocabulary.
 //   out[i] = scale table[t_i]          dtable[t] = scale sum over i with t_i = t of dout[i]
-// A token outside the table gives NaN in its row and nothing to the gradient; the padding's token gives nothing to the gradient.
+// A token outside the table gives NaN in its row and nothing to the gradient; the padding's token gives nothing to the gradient. With
+// `wrap` negative tokens count from the table's end, as in a tensor library's indexing.
 //
 // Both are bound by memory: the rows that are looked up, the output; for the gradient the rows of dout and the whole table, most of whose
 // rows are zero where the vocabulary is large. The gradient's rows are brought into the tokens' order, equal ones in the order in
@@ -34,11 +35,12 @@ static_assert(kRankRows == 1 << kIndexBits, "a key holds a row's index");
 template <typename TE, typename TO, int W>
 __global__ __launch_bounds__(256) void lookup_kernel(const int64_t* __restrict__ tokens, const TE* __restrict__ table,
                                                      TO* __restrict__ out, int64_t total, int units, int dim, int64_t vocab,
-                                                     float scale) {
+                                                     float scale, bool wrap) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = total <= 0xffffffff ? (uint32_t)i / (uint32_t)units : i / units;
     const int at = column<W>((int)(i - row * units), dim);
-    const int64_t t = tokens[row];
+    int64_t t = tokens[row];
+    t += wrap && t < 0 ? vocab : 0;
     float v[W];
     if (t >= 0 && t < vocab) {
       Cols<TE, W> in;
@@ -57,8 +59,13 @@ __global__ __launch_bounds__(256) void lookup_kernel(const int64_t* __restrict__
 }
 
 // The token of a row in the gradient's order: those without a gradient behind all others.
-__device__ __forceinline__ uint32_t token_of(int64_t t, int64_t vocab, int64_t pad) {
-  return t < 0 || t >= vocab || t == pad ? (uint32_t)vocab : (uint32_t)t;
+struct Vocab {
+  int64_t size, pad;
+  bool wrap;
+};
+__device__ __forceinline__ uint32_t token_of(int64_t t, const Vocab& v) {
+  t += v.wrap && t < 0 ? v.size : 0;
+  return t < 0 || t >= v.size || t == v.pad ? (uint32_t)v.size : (uint32_t)t;
 }
 
 // Zeros in `bytes` bytes at p, the workgroup's share of `blocks`.
@@ -75,11 +82,11 @@ __device__ __forceinline__ void fill_zero(char* p, int64_t bytes, int64_t block,
 }
 
 // Workgroups 0 .. ranks - 1 order R rows each, a share of the comparisons to every R lanes; the others fill the table's gradient. R
-// goes with the rows so that the comparisons spread over the chip (rank_rows): 8192 rows by 64 17 us with the fill, by 32 RANK32.
+// goes with the rows so that the comparisons spread over the chip (rank_rows): 8192 rows by 64 17 us with the fill, by 32 12.
 template <int R>
 __global__ __launch_bounds__(512) void rank_fill_kernel(const int64_t* __restrict__ tokens, uint32_t* __restrict__ keys,
-                                                        uint32_t* __restrict__ order, int rows, int64_t vocab, int64_t pad,
-                                                        int ranks, char* __restrict__ dtable, int64_t bytes) {
+                                                        uint32_t* __restrict__ order, int rows, Vocab vocab, int ranks,
+                                                        char* __restrict__ dtable, int64_t bytes) {
   constexpr int kShares = 512 / R;
   extern __shared__ __attribute__((aligned(16))) uint32_t all[];  // [padded]: (token, index), no two alike
   __shared__ uint32_t places[kShares][R];
@@ -95,7 +102,7 @@ __global__ __launch_bounds__(512) void rank_fill_kernel(const int64_t* __restric
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = i0 + u * 512 + (int)threadIdx.x;
-      if (i < padded) all[i] = i < rows ? (token_of(t[u], vocab, pad) << kIndexBits) | (uint32_t)i : 0xffffffffu;
+      if (i < padded) all[i] = i < rows ? (token_of(t[u], vocab) << kIndexBits) | (uint32_t)i : 0xffffffffu;
     }
   }
   __syncthreads();
@@ -133,8 +140,8 @@ constexpr int kMaxDigits = 1024;
 struct SortSource {
   const int64_t* tokens;  // or null:
   const uint32_t *keys, *order;
-  int64_t vocab, pad;
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return tokens ? token_of(tokens[i], vocab, pad) : keys[i]; }
+  Vocab vocab;
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return tokens ? token_of(tokens[i], vocab) : keys[i]; }
   __device__ __forceinline__ uint32_t index(int64_t i) const { return tokens ? (uint32_t)i : order[i]; }
 };
 
@@ -359,7 +366,8 @@ struct EmbedPlan {
   int64_t keys, order, keys2, order2, counts, totals, slab, bytes;
 };
 bool embed_plan(int64_t rows, int64_t dim, int64_t vocab, EmbedPlan& p) {
-  if (rows < 0 || rows > 0x3fffffff || dim < 1 || dim > 0x7fffffff / 64 || vocab < 1 || vocab > 0x7ffffffe ||
+  // A join of 1024 threads for every 64 rows stays under 2^32 threads.
+  if (rows < 0 || rows > 0x7ffffff || dim < 1 || dim > 0x7fffffff / 64 || vocab < 1 || vocab > 0x7ffffffe ||
       vocab > ((int64_t)1 << 58) / dim || rows > ((int64_t)1 << 58) / dim || cdiv(dim, (int64_t)64) > 65535)
     return false;
   p = EmbedPlan{};
@@ -391,9 +399,9 @@ bool embed_plan(int64_t rows, int64_t dim, int64_t vocab, EmbedPlan& p) {
 }
 
 template <typename T, typename TO>
-int embed_bwd(const int64_t* tokens, const T* dy, TO* dtable, int64_t rows, int64_t dim, int64_t vocab, int64_t pad,
-              float scale, const EmbedPlan& p, char* ws, hipStream_t s) {
-  const int64_t bytes = vocab * dim * (int64_t)sizeof(TO);
+int embed_bwd(const int64_t* tokens, const T* dy, TO* dtable, int64_t rows, int64_t dim, const Vocab& vocab, float scale,
+              const EmbedPlan& p, char* ws, hipStream_t s) {
+  const int64_t bytes = vocab.size * dim * (int64_t)sizeof(TO);
   const unsigned fills = (unsigned)std::clamp<int64_t>(cdiv(bytes, (int64_t)512 * 16 * 8), 1, 2048);
   auto part = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
   uint32_t *keys = part(p.keys), *order = part(p.order);
@@ -401,7 +409,7 @@ int embed_bwd(const int64_t* tokens, const T* dy, TO* dtable, int64_t rows, int6
     const int r = rank_rows(rows), ranks = (int)cdiv(rows, (int64_t)r), lds = (int)cdiv(rows, 4 * (512 / r)) * 4 * (512 / r) * 4;
     auto go = [&](auto kernel) {
       if (int rc = allow_lds((const void*)kernel, kRankRows * 4, s, "ferrite_embedding_bwd")) return rc;
-      hipLaunchKernelGGL(kernel, dim3(ranks + fills), dim3(512), lds, s, tokens, keys, order, (int)rows, vocab, pad, ranks,
+      hipLaunchKernelGGL(kernel, dim3(ranks + fills), dim3(512), lds, s, tokens, keys, order, (int)rows, vocab, ranks,
                          reinterpret_cast<char*>(dtable), bytes);
       return (int)FERRITE_OK;
     };
@@ -413,28 +421,29 @@ int embed_bwd(const int64_t* tokens, const T* dy, TO* dtable, int64_t rows, int6
     uint32_t *counts = part(p.counts), *totals = part(p.totals);
     // The last pass leaves its rows in keys and order.
     uint32_t* to[2][2] = {{keys, order}, {part(p.keys2), part(p.order2)}};
-    SortSource src{tokens, nullptr, nullptr, vocab, pad};
+    SortSource src{tokens, nullptr, nullptr, vocab};
     for (int k = 0; k < p.passes; ++k) {
       uint32_t** dst = to[(p.passes - 1 - k) & 1];
       const int shift = k * p.bits, digits = 1 << p.bits;
       hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(256), 0, s, src, counts, rows, shift, digits);
       hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(64), 0, s, counts, totals, (int)blocks);
       hipLaunchKernelGGL(sort_place_kernel, dim3(blocks), dim3(256), 0, s, src, counts, totals, dst[0], dst[1], rows, shift, p.bits);
-      src = SortSource{nullptr, dst[0], dst[1], vocab, pad};
+      src = SortSource{nullptr, dst[0], dst[1], vocab};
     }
   }
   float* slab = reinterpret_cast<float*>(ws + p.slab);
   auto sums = [&](auto kernel, int64_t units) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)p.pieces, (unsigned)cdiv(units, (int64_t)64)), dim3(64), 0, s, keys, order, dy,
-                       dtable, slab, rows, (int)dim, (uint32_t)vocab, scale, p.piece);
+                       dtable, slab, rows, (int)dim, (uint32_t)vocab.size, scale, p.piece);
   };
-  if (dim >= 8)
-    sums(token_sums_kernel<T, TO, 8>, cdiv(dim, (int64_t)8));
+  constexpr int kWide = sizeof(T) == 2 ? 8 : 4;
+  if (dim >= kWide)
+    sums(token_sums_kernel<T, TO, kWide>, cdiv(dim, (int64_t)kWide));
   else
     sums(token_sums_kernel<T, TO, 1>, dim);
   if (p.pieces > 1)
     hipLaunchKernelGGL((token_join_kernel<TO>), dim3((unsigned)p.pieces), dim3(1024), 0, s, keys, slab, dtable, rows, (int)dim,
-                       (uint32_t)vocab, scale, p.piece);
+                       (uint32_t)vocab.size, scale, p.piece);
   return check_launch("ferrite_embedding_bwd");
 }
 
@@ -448,7 +457,8 @@ int with_two_types(int a, int b, F&& f) {
 }  // namespace ferrite
 
 extern "C" int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* out, int64_t rows, int64_t dim,
-                                          int64_t vocab, float scale, int table_dtype, int out_dtype, void* stream) {
+                                          int64_t vocab, float scale, int wrap, int table_dtype, int out_dtype,
+                                          void* stream) {
   using namespace ferrite;
   EmbedPlan p;
   if (!valid_dtype(table_dtype) || !valid_dtype(out_dtype))
@@ -460,14 +470,17 @@ extern "C" int ferrite_internal_embedding(const int64_t* tokens, const void* tab
   return with_two_types(table_dtype, out_dtype, [&](auto* te, auto* to) {
     typedef std::remove_pointer_t<decltype(te)> TE;
     typedef std::remove_pointer_t<decltype(to)> TO;
-    const int64_t units = dim >= 8 ? cdiv(dim, (int64_t)8) : dim, total = rows * units;
+    // Sixteen bytes of the wider type to a thread: eight floats in two accesses leave every other 16 bytes to the next instruction.
+    // us, 51690 rows of 1716 floats, in fours / in eights: 109 / 127.
+    constexpr int kWide = sizeof(TE) == 2 && sizeof(TO) == 2 ? 8 : 4;
+    const int64_t units = dim >= kWide ? cdiv(dim, (int64_t)kWide) : dim, total = rows * units;
     const dim3 grid((unsigned)std::min<int64_t>(cdiv(total, (int64_t)256), 1 << 16));
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, tokens, static_cast<const TE*>(table), static_cast<TO*>(out), total,
-                         (int)units, (int)dim, vocab, scale);
+                         (int)units, (int)dim, vocab, scale, wrap != 0);
     };
-    if (dim >= 8)
-      go(lookup_kernel<TE, TO, 8>);
+    if (dim >= kWide)
+      go(lookup_kernel<TE, TO, kWide>);
     else
       go(lookup_kernel<TE, TO, 1>);
     return check_launch("ferrite_embedding");
@@ -480,8 +493,8 @@ extern "C" int64_t ferrite_internal_embedding_bwd_workspace(int64_t rows, int64_
 }
 
 extern "C" int ferrite_internal_embedding_bwd(const int64_t* tokens, const void* dy, void* dtable, int64_t rows, int64_t dim,
-                                              int64_t vocab, int64_t padding, float scale, int dy_dtype, int table_dtype,
-                                              void* workspace, int64_t workspace_bytes, void* stream) {
+                                              int64_t vocab, int64_t padding, float scale, int wrap, int dy_dtype,
+                                              int table_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace ferrite;
   EmbedPlan p;
   if (!valid_dtype(table_dtype) || !valid_dtype(dy_dtype))
@@ -493,7 +506,7 @@ extern "C" int ferrite_internal_embedding_bwd(const int64_t* tokens, const void*
   return with_two_types(dy_dtype, table_dtype, [&](auto* g, auto* d) {
     typedef std::remove_pointer_t<decltype(g)> T;
     typedef std::remove_pointer_t<decltype(d)> TO;
-    return embed_bwd(tokens, static_cast<const T*>(dy), static_cast<TO*>(dtable), rows, dim, vocab, padding, scale, p,
+    return embed_bwd(tokens, static_cast<const T*>(dy), static_cast<TO*>(dtable), rows, dim, Vocab{vocab, padding, wrap != 0}, scale, p,
                      static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
   });
 }

@@ -20,7 +20,7 @@
 namespace ferrite {
 namespace {
 
-constexpr int kTile = 64, kDepth = 32, kThreads = 256;
+constexpr int kTile = 64, kDepth = 32, kThreads = 256, kMostSlices = 32;
 constexpr int kOperand = kTile * kDepth * 4;  // bytes of an operand's stage
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kThreads, 4) void gemm_f32_any_kernel(const float* 
 
 bool f32_any_ok(int64_t m, int64_t n, int64_t k, bool xt, bool yt) {
   return m >= 1 && n >= 1 && k >= 1 && m <= 0x7fffff00 && n <= 0x7fffff00 && k <= 0x7fffff00 && (xt ? m : k) >= 4 &&
-         (yt ? k : n) >= 4 && cdiv(m, (int64_t)kTile) * cdiv(n, (int64_t)kTile) <= 0x7fffffff / 16 &&
+         (yt ? k : n) >= 4 && cdiv(m, (int64_t)kTile) * cdiv(n, (int64_t)kTile) < (1 << 24) / kMostSlices &&  // under 2^32 threads
          m <= ((int64_t)1 << 58) / n;
 }
 
@@ -177,7 +177,7 @@ bool f32_any_ok(int64_t m, int64_t n, int64_t k, bool xt, bool yt) {
 // adds them. us of the kernel alone, M x K x N by slices: 2100 x 1003 x 515 68 (1), 45 (2), 38.5 (3, taken), 35.5 (8);
 // 1003 x 2100 x 515 106 (1), 47 (3), 38 (5, taken), 40.5 (8); 2100 x 515 x 1003 45 (1, taken), 36 (3, and 10 for the slabs).
 int f32_any_slices(int64_t m, int64_t n, int64_t k, int64_t cus) {
-  const int64_t tiles = cdiv(m, (int64_t)kTile) * cdiv(n, (int64_t)kTile), most = std::clamp<int64_t>(k / (4 * kDepth), 1, 32);
+  const int64_t tiles = cdiv(m, (int64_t)kTile) * cdiv(n, (int64_t)kTile), most = std::clamp<int64_t>(k / (4 * kDepth), 1, kMostSlices);
   const double tile_us = 18.7e-3 * (double)k, slab_us = (double)m * (double)n * 8 / 5e6;
   int best = 1;
   double least = 1e300;

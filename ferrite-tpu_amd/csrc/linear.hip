@@ -18,11 +18,11 @@ namespace {
 
 constexpr int kUnits = 32, kLanes = 8;  // units of columns and rows under way in a workgroup
 
-// Without u, du is dy and is not written.
+// Without u, du is dy and is not written. With one workgroup to a column its sums are the bias's gradient.
 template <typename T, int W>
 __global__ __launch_bounds__(kUnits* kLanes) void act_grad_kernel(const T* __restrict__ dy, const T* __restrict__ u,
                                                                   T* __restrict__ du, float* __restrict__ part, int64_t rows,
-                                                                  int dim, int act, int64_t share) {
+                                                                  int dim, int act, int64_t share, void* db, int db_f32) {
   __shared__ float red[kLanes][kUnits * W + 1];
   const int c = threadIdx.x % kUnits, r = threadIdx.x / kUnits;
   const int unit = (int)blockIdx.x * kUnits + c;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kUnits* kLanes) void act_grad_kernel(const T* __res
         for (int e = 0; e < W; ++e) sum[e] += x[e];
       }
     }
-  if (!part) return;
+  if (!part && !db) return;
 #pragma unroll
   for (int e = 0; e < W; ++e) red[r][c * W + e] = sum[e];
   __syncthreads();
@@ -69,7 +69,12 @@ __global__ __launch_bounds__(kUnits* kLanes) void act_grad_kernel(const T* __res
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < kLanes; ++k) s += red[k][j];
-    part[(int64_t)blockIdx.y * dim + to + j % W] = s;
+    if (part)
+      part[(int64_t)blockIdx.y * dim + to + j % W] = s;
+    else if (db_f32)
+      static_cast<float*>(db)[to + j % W] = s;
+    else
+      static_cast<bf16*>(db)[to + j % W] = (bf16)s;
   }
 }
 
@@ -97,7 +102,8 @@ bool act_ok(int64_t rows, int64_t dim) {
 extern "C" int64_t ferrite_internal_act_grad_workspace(int64_t rows, int64_t dim) {
   using namespace ferrite;
   if (!act_ok(rows, dim)) return -1;
-  return act_plan(rows, dim).parts * dim * (int64_t)sizeof(float);
+  const ActPlan p = act_plan(rows, dim);
+  return p.parts > 1 ? p.parts * dim * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int ferrite_internal_act_grad(const void* dy, const void* u, void* du, void* db, int64_t rows, int64_t dim, int act,
@@ -107,17 +113,17 @@ extern "C" int ferrite_internal_act_grad(const void* dy, const void* u, void* du
     return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_linear_bwd: bad dtype or activation");
   if (!act_ok(rows, dim)) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_linear_bwd: sizes out of range");
   if ((rows && !dy) || (u && rows && !du)) return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_linear_bwd: null pointer");
-  if (db && (!workspace || workspace_bytes < ferrite_internal_act_grad_workspace(rows, dim) ||
-             (reinterpret_cast<uintptr_t>(workspace) & 3)))
+  const int64_t need = db ? ferrite_internal_act_grad_workspace(rows, dim) : 0;
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3)))
     return fail(FERRITE_ERR_INVALID_ARGUMENT, "ferrite_linear_bwd: workspace too small");
   const ActPlan p = act_plan(rows, dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  float* part = db ? static_cast<float*>(workspace) : nullptr;
+  float* part = need ? static_cast<float*>(workspace) : nullptr;
   auto go = [&](auto kernel, auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     hipLaunchKernelGGL(kernel, dim3((unsigned)p.cols, (unsigned)p.parts), dim3(kUnits * kLanes), 0, s,
                        static_cast<const T*>(dy), static_cast<const T*>(u), static_cast<T*>(du), part, rows, (int)dim, act,
-                       p.share);
+                       p.share, need ? nullptr : db, bias_dtype == FERRITE_F32);
   };
   auto typed = [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
@@ -130,7 +136,7 @@ extern "C" int ferrite_internal_act_grad(const void* dy, const void* u, void* du
     typed((bf16*)nullptr);
   else
     typed((float*)nullptr);
-  if (db) {
+  if (need) {
     if (bias_dtype == FERRITE_BF16)
       join_parts(part, static_cast<bf16*>(db), (bf16*)nullptr, 1, (int)p.parts, dim, s);
     else

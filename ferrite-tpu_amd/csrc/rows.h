@@ -76,11 +76,27 @@ struct Eight<float> {
   }
 };
 
-// Columns of W elements: eight, or one where a row has fewer than eight.
+// Columns of W elements in one access (two of 16 bytes for eight floats), or one where a row has fewer.
 template <typename T, int W>
 struct Cols;
 template <typename T>
 struct Cols<T, 8> : Eight<T> {};
+template <typename T>
+struct Cols<T, 4> {
+  typedef T vec __attribute__((ext_vector_type(4)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  vec v;
+  __device__ __forceinline__ void load(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const any*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<any*>(p)); }
+  __device__ __forceinline__ void get(float (&o)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = Elem<T>::to_f32(v[e]);
+  }
+  __device__ __forceinline__ void set(const float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = Elem<T>::from_f32(x[e]);
+  }
+};
 template <typename T>
 struct Cols<T, 1> {
   T v;
@@ -89,12 +105,10 @@ struct Cols<T, 1> {
   __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = Elem<T>::to_f32(v); }
   __device__ __forceinline__ void set(const float (&x)[1]) { v = Elem<T>::from_f32(x[0]); }
 };
-// First column of unit c of a row; -1 past it.
+// First column of unit c of a row of dim >= W; -1 past it. The last unit lies over the one before, as a Chunk does.
 template <int W>
 __device__ __forceinline__ int column(int c, int dim) {
-  if constexpr (W == 1) return c < dim ? c : -1;
-  const Chunk ch = chunk_of(c, dim);
-  return ch.on ? ch.at : -1;
+  return c < (dim + W - 1) / W ? min(W * c, dim - W) : -1;
 }
 
 // The sums of partial rows [parts][arrays][dim], array blockIdx.y of them into a or b (or none, where that is null): 64 columns to a

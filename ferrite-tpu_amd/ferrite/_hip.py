@@ -172,11 +172,11 @@ INTERNAL: dict[str, tuple] = {
     "ferrite_internal_matmul_f32": (_c_int, [_vp, _vp, _vp, *[_c_i64] * 3, _c_int, _c_int, _vp, _c_i64, _vp]),
     "ferrite_internal_act_grad_workspace": (_c_i64, [_c_i64] * 2),
     "ferrite_internal_act_grad": (_c_int, [*[_vp] * 4, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp, _c_i64, _vp]),
-    "ferrite_internal_embedding": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_f32, _c_int, _c_int, _vp]),
+    "ferrite_internal_embedding": (_c_int, [_vp, _vp, _vp, *[_c_i64] * 3, _c_f32, _c_int, _c_int, _c_int, _vp]),
     "ferrite_internal_embedding_bwd_workspace": (_c_i64, [_c_i64] * 3),
     "ferrite_internal_embedding_bwd": (
         _c_int,
-        [_vp, _vp, _vp, *[_c_i64] * 4, _c_f32, _c_int, _c_int, _vp, _c_i64, _vp],
+        [_vp, _vp, _vp, *[_c_i64] * 4, _c_f32, _c_int, _c_int, _c_int, _vp, _c_i64, _vp],
     ),
     "ferrite_internal_clip_workspace": (_c_i64, [_c_i64]),
     "ferrite_internal_clip": (_c_int, [_c_i64, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _c_i64, _vp]),

@@ -20,7 +20,7 @@ def embedding(tokens, table, *, scale: float = 1.0, padding_idx: int | None = No
     Differentiable in the table: equal tokens' rows are added in f32 in their order in ``tokens``, cut into pieces by their place
     among all rows, and rounded once; no atomics, so a call's result is the same every time. ``padding_idx`` (from 0 to vocab - 1) is
     looked up like any token and has no gradient. A token outside the table (a negative one too) gives a row of NaN and no gradient.
-    Up to 2^30 - 1 tokens, vocab below 2^31 - 1, dim up to 4194240 (RuntimeError beyond). Tensors that are not dense are copied first."""
+    Fewer than 2^27 tokens, vocab below 2^31 - 1, dim up to 4194240 (RuntimeError beyond). Tensors that are not dense are copied first."""
     if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"expected a table [vocab, dim]; got {tuple(table.shape)}")
     if tokens.dtype not in (torch.int64, torch.int32):
@@ -31,7 +31,8 @@ def embedding(tokens, table, *, scale: float = 1.0, padding_idx: int | None = No
     _hip.dtype_code(table.dtype)
     _hip.dtype_code(dtype)
     _hip.require_gpu(tokens, table)
-    return _hip.autograd().embedding(tokens, table, float(scale), -1 if padding_idx is None else int(padding_idx), dtype)
+    return _hip.autograd().embedding(tokens, table, float(scale), -1 if padding_idx is None else int(padding_idx), dtype,
+                                      False)
 
 
 def embedding_reference(tokens, table, *, scale: float = 1.0, padding_idx: int | None = None, dtype=None):

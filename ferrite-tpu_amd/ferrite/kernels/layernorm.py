@@ -23,7 +23,7 @@ def layernorm(x, weight, bias=None, *, residual=None, eps: float = 1e-5):
     if x.ndim < 1 or x.shape[-1] == 0:
         raise RuntimeError("layernorm needs a non-empty last dimension")
     dim = x.shape[-1]
-    if tuple(weight.shape) != (dim,) or bias is not None and tuple(bias.shape) != (dim,):
+    if weight.shape != (dim,) or bias is not None and bias.shape != (dim,):
         raise ValueError(f"weight and bias must have shape ({dim},), got {tuple(weight.shape)}"
                          + ("" if bias is None else f" and {tuple(bias.shape)}"))
     if bias is not None and bias.dtype != weight.dtype:

@@ -67,9 +67,9 @@ def linear(x, w, *, bias=None, activation: str | None = None, residual=None):
         return _hip.autograd().linear(x, w)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None, 'relu', 'gelu' or 'silu'; got {activation!r}")
-    if bias is not None and tuple(bias.shape) != (w.shape[1],):
+    if bias is not None and bias.shape != (w.shape[1],):
         raise ValueError(f"bias must have shape ({w.shape[1]},), got {tuple(bias.shape)}")
-    if residual is not None and (tuple(residual.shape) != (*x.shape[:-1], w.shape[1]) or residual.dtype != x.dtype):
+    if residual is not None and (residual.shape != (*x.shape[:-1], w.shape[1]) or residual.dtype != x.dtype):
         raise ValueError(f"residual must be {(*x.shape[:-1], w.shape[1])} in {x.dtype}; got {tuple(residual.shape)} in {residual.dtype}")
     if x.shape[-1] == 0:
         raise RuntimeError("linear needs a non-empty inner dimension")

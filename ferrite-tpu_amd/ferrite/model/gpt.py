@@ -307,17 +307,32 @@ def _one_kernel_embedding(tok, pe, tokens, dtype) -> bool:
             and 0 < tokens.numel() < 1 << 24 and tokens.shape[1] <= pe.shape[0] < 1 << 24)
 
 
+def _any_vocabulary(tok, tokens) -> bool:
+    """What the embedding kernels of any vocabulary take (:func:`~ferrite.kernels.embedding.embedding`'s limits)."""
+    return (tok.is_cuda and tok.device == tokens.device and tok.dtype in (torch.float32, torch.bfloat16) and tok.ndim == 2
+            and tok.shape[0] < 1 << 30 and 0 < tok.shape[1] <= 1 << 20 and tokens.dtype in (torch.int64, torch.int32)
+            and 0 < tokens.numel() < 1 << 27)
+
+
+def _embed_tokens(tok, pe, tokens, cfg: GPTConfig):
+    """The residual stream's beginning, table and position rows in cfg.dtype: on kernels where its other part, the add and norm, is.
+    Vocabularies past what one kernel takes are looked up by the one of any vocabulary, whose gradient does not slow down with
+    repeated tokens as torch's indexing does. us of the table's gradient on one MI355X, torch / here, tokens as text has
+    them: 8192 x 768 bf16 over 32768 845 / 27, 32768 x 768 over 50257 3019 / 80."""
+    if cfg.norm == "pallas" and _one_kernel_embedding(tok, pe, tokens, cfg.dtype):
+        return _hip.autograd().embed_tokens(tokens, tok, pe, cfg.dtype)
+    rows = tok[tokens] if cfg.norm != "pallas" or not _any_vocabulary(tok, tokens) else \
+        _hip.autograd().embedding(tokens, tok, 1.0, -1, tok.dtype, True)
+    return (rows + pe[:tokens.shape[1]]).to(cfg.dtype)
+
+
 def _trunk(params, tokens, cfg: GPTConfig):
     """tokens [B, S] -> final normed hidden states [B*S, d] in cfg.dtype (gpt.py:124-142)."""
     b, s = tokens.shape
     if s > cfg.seq_len:
         raise ValueError(f"sequence {s} longer than cfg.seq_len={cfg.seq_len}")
     tok, pe = params["tok_emb"], params["pos_emb"]
-    # The residual stream's glue: on kernels where its other part, the add and norm, is.
-    if cfg.norm == "pallas" and _one_kernel_embedding(tok, pe, tokens, cfg.dtype):
-        h = _hip.autograd().embed_tokens(tokens, tok, pe, cfg.dtype)  # residual stream
-    else:
-        h = (tok[tokens] + pe[:s]).to(cfg.dtype)
+    h = _embed_tokens(tok, pe, tokens, cfg)  # residual stream
     pending = None  # sub-layer output whose residual add is fused into the next norm
     for layer in params["layers"]:
         if pending is None:

@@ -136,7 +136,7 @@ def test_nothing_beside_the_table_is_written(dev, rows, offset):
     d = room[24 + offset:24 + offset + vocab * dim]
     lib = _hip.lib()
     ws = torch.empty(lib.ferrite_internal_embedding_bwd_workspace(rows, dim, vocab), dtype=torch.uint8, device=dev)
-    rc = lib.ferrite_internal_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), d.data_ptr(), rows, dim, vocab, -1, 1.0, _hip.BF16,
+    rc = lib.ferrite_internal_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), d.data_ptr(), rows, dim, vocab, -1, 1.0, 0, _hip.BF16,
                                             _hip.BF16, ws.data_ptr(), ws.numel(), _hip.stream_of(d))
     assert rc == _hip.OK
     _check_grad(d.view(vocab, dim), tokens, dy, d.view(vocab, dim), 1.0)
@@ -172,3 +172,28 @@ def test_another_stream_and_a_captured_step(dev, rows):
         want = step(table)
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("rows", [900, 20000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_model_embeds_large_vocabularies_with_it(dev, rows, dtype):
+    """GPT's residual stream over a vocabulary past 1024: as torch's indexing gives it, negative tokens counted from the end, and the
+    table's gradient within the tolerance above."""
+    from ferrite.model.gpt import GPTConfig, _embed_tokens
+
+    cfg = GPTConfig(vocab_size=3000, seq_len=rows // 2, d_model=72, n_head=1)
+    g = torch.Generator().manual_seed(rows)
+    tok = torch.randn(3000, 72, generator=g).to(dev, dtype).requires_grad_()
+    pe = torch.randn(rows // 2, 72, generator=g).to(dev, dtype).requires_grad_()
+    tokens = torch.randint(-3000, 3000, (2, rows // 2), generator=g).to(dev)
+    dh = torch.randn(2, rows // 2, 72, generator=g).to(dev, BF16)
+    h = _embed_tokens(tok, pe, tokens, cfg)
+    def names(fn):
+        return [] if fn is None else [fn.name(), *(n for f, _ in fn.next_functions for n in names(f))]
+
+    assert any("EmbeddingFn" in n for n in names(h.grad_fn))
+    assert torch.equal(h, (tok[tokens] + pe).to(BF16))
+    d, dp = torch.autograd.grad(h, (tok, pe), dh)
+    _check_grad(d, tokens % 3000, dh.to(dtype), tok.detach(), 1.0)
+    want = torch.autograd.grad((tok[tokens] + pe).to(BF16), pe, dh)[0]
+    assert torch.equal(dp, want)

@@ -80,14 +80,14 @@ def test_embedding_sizes_out_of_range():
     from ferrite import _hip
 
     lib = _hip.lib()
-    assert lib.ferrite_internal_embedding_bwd_workspace(1 << 30, 8, 8) == -1
+    assert lib.ferrite_internal_embedding_bwd_workspace(1 << 27, 8, 8) == -1
     assert lib.ferrite_internal_embedding_bwd_workspace(8, 4194241, 8) == -1
     assert lib.ferrite_internal_embedding_bwd_workspace(8, 8, 0x7fffffff) == -1
     assert lib.ferrite_internal_embedding_bwd_workspace(8, 0, 8) == -1
     assert lib.ferrite_internal_embedding_bwd_workspace(0, 8, 8) == 0
     assert lib.ferrite_internal_embedding_bwd_workspace(16384, 64, 50257) > 0
-    assert lib.ferrite_internal_embedding_bwd(None, None, None, 1, 8, 8, -1, 1.0, 1, 1, None, 0, None) == 1
-    assert lib.ferrite_internal_embedding(None, None, None, 1, 8, 8, 1.0, 1, 7, None) == 1
+    assert lib.ferrite_internal_embedding_bwd(None, None, None, 1, 8, 8, -1, 1.0, 0, 1, 1, None, 0, None) == 1
+    assert lib.ferrite_internal_embedding(None, None, None, 1, 8, 8, 1.0, 0, 1, 7, None) == 1
 
 
 def test_clip_refuses():
