@@ -32,7 +32,7 @@ def layernorm(x, weight, bias=None, *, residual=None, eps: float = 1e-5):
         raise ValueError("residual must match x in shape and dtype")
     _hip.dtype_code(x.dtype)
     _hip.dtype_code(weight.dtype)
-    _hip.require_gpu(*(t for t in (x, weight, bias, residual) if t is not None))
+    _hip.require_gpu(x, weight, x if bias is None else bias, x if residual is None else residual)
     out = _hip.autograd().layernorm(x, weight, bias, residual, float(eps))
     return out[0] if residual is None else (out[0], out[1])
 

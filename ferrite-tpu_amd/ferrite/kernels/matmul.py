@@ -73,9 +73,9 @@ def linear(x, w, *, bias=None, activation: str | None = None, residual=None):
         raise ValueError(f"residual must be {(*x.shape[:-1], w.shape[1])} in {x.dtype}; got {tuple(residual.shape)} in {residual.dtype}")
     if x.shape[-1] == 0:
         raise RuntimeError("linear needs a non-empty inner dimension")
-    for t in (x, w, *(() if bias is None else (bias,))):
+    for t in (x, w) if bias is None else (x, w, bias):
         _hip.dtype_code(t.dtype)
-    _hip.require_gpu(*(t for t in (x, w, bias, residual) if t is not None))
+    _hip.require_gpu(x, w, x if bias is None else bias, x if residual is None else residual)
     return _hip.autograd().linear_act(x, w, bias, residual, ACTIVATIONS[activation])
 
 
