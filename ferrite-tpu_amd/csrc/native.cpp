@@ -619,9 +619,10 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
                                       size_of(ws), stream_of(g)),
             "ferrite_linear_bwd");
     }
-    return {linear_mm(du, wq, m, k, n, false, true, dt, x.sizes()),
-            linear_mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n}), db,
-            ctx->saved_data["r"].toBool() ? g : Tensor(), Tensor()};
+    Tensor dx, dw;  // a product that nobody asks for is left out
+    if (ctx->needs_input_grad(0)) dx = linear_mm(du, wq, m, k, n, false, true, dt, x.sizes());
+    if (ctx->needs_input_grad(1)) dw = linear_mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n});
+    return {dx, dw, db, ctx->saved_data["r"].toBool() ? g : Tensor(), Tensor()};
   }
 };
 
@@ -922,6 +923,8 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double most) {
   spans.reserve(n);
   for (int64_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
+    if (g.requires_grad() && at::GradMode::is_enabled())
+      throw std::runtime_error("clip_grad_norm_ scales in place and records nothing: call it under torch.no_grad() on a tensor that requires a gradient");
     if (!g.is_non_overlapping_and_dense())
       throw py::value_error("clip_grad_norm_ scales tensors in place: each must be dense in memory");
     p[i] = g.data_ptr();

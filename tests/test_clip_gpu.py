@@ -120,3 +120,12 @@ def test_a_saved_tensor_that_was_scaled_is_noticed(dev):
     clip_grad_norm_([g], 0.1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_tensors_that_require_a_gradient(dev):
+    g = torch.full((10,), 2.0, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        clip_grad_norm_([g], 1.0)
+    assert bool((g == 2).all())
+    with torch.no_grad():
+        _check([g], 1.0)

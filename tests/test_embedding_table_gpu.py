@@ -197,3 +197,22 @@ def test_the_model_embeds_large_vocabularies_with_it(dev, rows, dtype):
     _check_grad(d, tokens % 3000, dh.to(dtype), tok.detach(), 1.0)
     want = torch.autograd.grad((tok[tokens] + pe).to(BF16), pe, dh)[0]
     assert torch.equal(dp, want)
+
+
+def test_capture_refuses_leaves_that_an_eager_graph_holds(dev):
+    table, tokens = torch.randn(40, 8, device=dev, requires_grad=True), torch.zeros(5, dtype=torch.long, device=dev)
+    held = embedding(tokens, table)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="holds one of its leaves"):
+        with torch.cuda.graph(graph):
+            embedding(tokens, table)
+    del held
+
+
+def test_forward_mode_is_refused(dev):
+    import torch.autograd.forward_ad as fwd
+
+    table, tokens = torch.randn(40, 8, device=dev), torch.zeros(5, dtype=torch.long, device=dev)
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        embedding(tokens, fwd.make_dual(table, torch.ones_like(table)))

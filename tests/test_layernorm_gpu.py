@@ -229,3 +229,11 @@ def test_capture_refuses_leaves_that_an_eager_graph_holds(dev):
         with torch.cuda.graph(graph):
             layernorm(x, w)
     del held
+
+
+def test_forward_mode_is_refused(dev):
+    import torch.autograd.forward_ad as fwd
+
+    x, w = torch.randn(4, 64, device=dev), torch.randn(64, device=dev)
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        layernorm(x, fwd.make_dual(w, torch.ones_like(w)))

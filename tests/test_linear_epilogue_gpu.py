@@ -240,3 +240,36 @@ def test_overlapping_outputs_are_refused_at_the_entry_point(dev):
     assert call(out.data_ptr(), None) != _hip.OK and "overlap" in _hip.last_error()
     assert call(None, out.data_ptr() + 128) != _hip.OK
     assert call(out[1].data_ptr(), out[1].data_ptr()) != _hip.OK
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradients_that_are_asked_for(dev, dtype):
+    x, w, b, r, dy = _inputs(dev, 70, 96, 40, dtype, dtype, F32, True, True, seed=8)
+    _, full = _run(x, w, b, r, dy, "silu")
+    for wanted in ("x", "w", "b", "r", "xb", "wr"):
+        leaves = {k: t.detach().requires_grad_(k in wanted) for k, t in zip("xwbr", (x, w, b, r))}
+        y = linear(leaves["x"], leaves["w"], bias=leaves["b"], activation="silu", residual=leaves["r"])
+        got = torch.autograd.grad(y, [leaves[k] for k in wanted], dy)
+        assert all(torch.equal(g, full[k]) for g, k in zip(got, wanted))
+    leaves = {k: t.detach().requires_grad_() for k, t in zip("xwbr", (x, w, b, r))}  # all record, one is asked for
+    y = linear(leaves["x"], leaves["w"], bias=leaves["b"], activation="silu", residual=leaves["r"])
+    assert torch.equal(torch.autograd.grad(y, leaves["w"], dy)[0], full["w"])
+
+
+def test_capture_refuses_leaves_that_an_eager_graph_holds(dev):
+    x, w = torch.randn(4, 64, device=dev, requires_grad=True), torch.randn(64, 8, device=dev, requires_grad=True)
+    held = linear(x, w, activation="relu")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="holds one of its leaves"):
+        with torch.cuda.graph(graph):
+            linear(x, w, activation="relu")
+    del held
+
+
+def test_forward_mode_is_refused(dev):
+    import torch.autograd.forward_ad as fwd
+
+    x, w = torch.randn(4, 64, device=dev), torch.randn(64, 8, device=dev)
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        linear(fwd.make_dual(x, torch.ones_like(x)), w, activation="relu")
