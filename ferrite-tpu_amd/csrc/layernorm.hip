@@ -24,33 +24,34 @@
 namespace ferrite {
 namespace {
 
-template <typename TW>
-__device__ __forceinline__ void load_params(const TW* p, int at, float (&o)[8]) {
+template <typename TW, int W>
+__device__ __forceinline__ void load_params(const TW* p, int at, float (&o)[W]) {
   if (!p) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    for (int e = 0; e < W; ++e) o[e] = 0.f;
     return;
   }
-  Eight<TW> v;
+  Cols<TW, W> v;
   v.load_cached(p + at);
   v.get(o);
 }
 
-// G threads own a row, VPL chunks each: chunk t + G i of thread t. A wave (G = 64) takes D rows at a time, whose loads go out together,
+// G threads own a row, VPL chunks of W elements each: chunk t + G i of thread t. W is 16 bytes: eight floats of a lane in two accesses
+// would leave every other 16 bytes of a line to the next instruction. A wave (G = 64) takes D rows at a time, whose loads go out together,
 // and keeps its weights; wider groups read the weights again for every row, from L2.
-template <typename TX, typename TW, bool RES, int VPL, int G, int D>
+template <typename TX, typename TW, bool RES, int W, int VPL, int G, int D>
 __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
     const TX* __restrict__ x, const TX* __restrict__ r, const TW* __restrict__ w, const TW* __restrict__ b,
     TX* __restrict__ h, TX* __restrict__ y, float* __restrict__ stats, int64_t rows, int dim, float inv_dim, float eps) {
   constexpr int kGroups = G < 256 ? 256 / G : 1;
-  constexpr bool kKeep = G == 64 && VPL <= 2;
+  constexpr bool kKeep = G == 64 && W * VPL <= 16;
   __shared__ float lds[2][16];
   const int t = threadIdx.x % G;
   Chunk ch[VPL];
-  float wv[VPL][8], bv[VPL][8];
+  float wv[VPL][W], bv[VPL][W];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    ch[i] = chunk_of(t + G * i, dim);
+    ch[i] = chunk_of<W>(t + G * i, dim);
     if (kKeep && ch[i].on) {
       load_params(w, ch[i].at, wv[i]);
       load_params(b, ch[i].at, bv[i]);
@@ -58,7 +59,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
   }
   for (int64_t row0 = ((int64_t)blockIdx.x * kGroups + threadIdx.x / G) * D; row0 < rows;
        row0 += (int64_t)gridDim.x * kGroups * D) {
-    Eight<TX> xr[D][VPL], rr[D][VPL];
+    Cols<TX, W> xr[D][VPL], rr[D][VPL];
 #pragma unroll
     for (int k = 0; k < D; ++k) {
       const int64_t off = min(row0 + k, rows - 1) * dim;
@@ -74,24 +75,24 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
     for (int k = 0; k < D; ++k) {
       const int64_t row = row0 + k, off = row * dim;
       if (D > 1 && row >= rows) break;
-      float hv[VPL][8];
+      float hv[VPL][W];
       float sum = 0.f, none = 0.f;
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (ch[i].on) {
           xr[k][i].get(hv[i]);
           if constexpr (RES) {
-            float rv[8];
+            float rv[W];
             rr[k][i].get(rv);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) hv[i][e] += rv[e];
-            Eight<TX> out;
+            for (int e = 0; e < W; ++e) hv[i][e] += rv[e];
+            Cols<TX, W> out;
             out.set(hv[i]);
             out.store(h + off + ch[i].at);
             out.get(hv[i]);
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum += e >= ch[i].skip ? hv[i][e] : 0.f;
+          for (int e = 0; e < W; ++e) sum += e >= ch[i].skip ? hv[i][e] : 0.f;
         }
       rows_sum<G>(sum, none, lds);
       const float mean = sum * inv_dim;
@@ -100,7 +101,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
       for (int i = 0; i < VPL; ++i)
         if (ch[i].on)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
+          for (int e = 0; e < W; ++e) {
             hv[i][e] -= mean;
             const float c = e >= ch[i].skip ? hv[i][e] : 0.f;
             rest += c;
@@ -123,10 +124,10 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
             load_params(w, ch[i].at, wv[i]);
             load_params(b, ch[i].at, bv[i]);
           }
-          float yv[8];
+          float yv[W];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) yv[e] = (hv[i][e] - rest) * rstd * wv[i][e] + bv[i][e];
-          Eight<TX> out;
+          for (int e = 0; e < W; ++e) yv[e] = (hv[i][e] - rest) * rstd * wv[i][e] + bv[i][e];
+          Cols<TX, W> out;
           out.set(yv);
           out.store(y + off + ch[i].at);
         }
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256) void layernorm_sweep_kernel(const TX* __restri
   }
 }
 
-// Threads to a row and chunks to a thread; group 0: the sweeps. Below 8 elements a row has no chunk.
+// Threads to a row and eights of elements to a thread; group 0: the sweeps. Below 8 elements a row goes to them too.
 struct NormPlan {
   int group, vpl;
 };
@@ -193,7 +194,8 @@ NormPlan norm_plan(int64_t dim) {
 #define FERRITE_NORM_CASE(plan, ...)                      \
   do {                                                    \
     auto run = [&](auto vpl, auto group) {                \
-      constexpr int VPL = decltype(vpl)::value;           \
+      constexpr int W = 16 / sizeof(TX);                  \
+      constexpr int VPL = decltype(vpl)::value * 8 / W;   \
       constexpr int G = decltype(group)::value;           \
       __VA_ARGS__;                                        \
     };                                                    \
@@ -234,9 +236,9 @@ int norm_launch(const TX* x, const TX* r, const TW* w, const TW* b, TX* h, TX* y
                        dim3(G < 256 ? 256 : G), 0, stream, x, r, w, b, h, y, stats, rows, (int)dim, inv_dim, eps);
   };
                     if constexpr (sizeof(TX) == 2 && VPL == 2 && G == 64) {
-                      if (rows >= 4096) return go(layernorm_kernel<TX, TW, RES, VPL, G, 2>, 2);
+                      if (rows >= 4096) return go(layernorm_kernel<TX, TW, RES, W, VPL, G, 2>, 2);
                     };
-                    go(layernorm_kernel<TX, TW, RES, VPL, G, 1>, 1));
+                    go(layernorm_kernel<TX, TW, RES, W, VPL, G, 1>, 1));
   return check_launch("ferrite_layernorm");
 }
 
@@ -245,26 +247,26 @@ int norm_launch(const TX* x, const TX* r, const TW* w, const TW* b, TX* h, TX* y
 // ---------------------------------------------------------------------------
 constexpr int kBwdParts = 512;  // partial rows of dw and db
 
-template <typename TX, typename TW, bool DIRECT, int VPL, int G>
+template <typename TX, typename TW, bool DIRECT, int W, int VPL, int G>
 __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
     const TX* __restrict__ h, const TW* __restrict__ w, const TX* __restrict__ dy, const TX* __restrict__ dd,
     const float* __restrict__ stats, TX* __restrict__ dh, float* __restrict__ part, int64_t rows, int dim, float inv_dim) {
   constexpr int kGroups = G < 256 ? 256 / G : 1;
   // The widest rows leave no registers for the next row and the weights (up to 180 spilled).
-  constexpr bool kAhead = G * VPL < 2048;
+  constexpr bool kAhead = G * W * VPL < 16384;
   extern __shared__ float red[];  // [kGroups][dim] where there is more than one group
   __shared__ float lds[2][16];
   const int t = threadIdx.x % G, grp = threadIdx.x / G;
   Chunk ch[VPL];
-  float wv[VPL][8], dw[VPL][8], db[VPL][8];
+  float wv[VPL][W], dw[VPL][W], db[VPL][W];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    ch[i] = chunk_of(t + G * i, dim);
+    ch[i] = chunk_of<W>(t + G * i, dim);
     if (kAhead && ch[i].on) load_params(w, ch[i].at, wv[i]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
+    for (int e = 0; e < W; ++e) dw[i][e] = db[i][e] = 0.f;
   }
-  Eight<TX> hr[VPL], gr[VPL], dr[VPL];
+  Cols<TX, W> hr[VPL], gr[VPL], dr[VPL];
   float mean = 0.f, rstd = 0.f;
   auto load = [&](int64_t row) {
     const int64_t off = row * dim;
@@ -284,7 +286,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
   for (; row < rows; row += step) {
     if (!kAhead) load(row);
     const int64_t off = row * dim;
-    float cv[VPL][8], gv[VPL][8], dv[VPL][8];
+    float cv[VPL][W], gv[VPL][W], dv[VPL][W];
     float rest = 0.f, sg = 0.f, sgc = 0.f, none = 0.f;
     const float m = mean, rs = rstd;
 #pragma unroll
@@ -299,9 +301,12 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (ch[i].on) {
-        if (!kAhead) load_params(w, ch[i].at, wv[i]);
+        if (!kAhead) {
+          __builtin_amdgcn_sched_barrier(0);
+          load_params(w, ch[i].at, wv[i]);
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < W; ++e) {
           cv[i][e] -= m;
           const bool mine = e >= ch[i].skip;
           const float g = mine ? gv[i][e] * wv[i][e] : 0.f;
@@ -318,35 +323,36 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
     for (int i = 0; i < VPL; ++i)
       if (ch[i].on) {
         if constexpr (!kAhead) {
+          __builtin_amdgcn_sched_barrier(0);  // a chunk's weights and gradients at a time: all of them spill
           load_params(w, ch[i].at, wv[i]);
           if constexpr (DIRECT) {
             dr[i].load(dd + off + ch[i].at);
             dr[i].get(dv[i]);
           }
         }
-        float o[8];
+        float o[W];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < W; ++e) {
           const float n = (cv[i][e] - rest) * rs;
           o[e] = rs * (gv[i][e] * wv[i][e] - mg - n * mgn);
           if constexpr (DIRECT) o[e] += dv[i][e];
           dw[i][e] += gv[i][e] * n;
           db[i][e] += gv[i][e];
         }
-        Eight<TX> out;
+        Cols<TX, W> out;
         out.set(o);
         out.store(dh + off + ch[i].at);
       }
   }
   // The groups' sums, dw's and then db's, through the same LDS.
   float* const mine = part + (int64_t)blockIdx.x * 2 * dim;
-  auto put = [&](const float (&acc)[VPL][8], float* dst) {
+  auto put = [&](const float (&acc)[VPL][W], float* dst) {
     float* const to = kGroups > 1 ? red + grp * dim : dst;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (ch[i].on)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < W; ++e)
           if (e >= ch[i].skip) to[ch[i].at + e] = acc[i][e];
     if constexpr (kGroups > 1) {
       __syncthreads();
@@ -409,7 +415,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_cols_kernel(const TX* __res
 }
 
 // Partial rows: one to a CU, and two where the columns are few and the rows many; a row to a group at least. More of them cost more
-// than they bring. us, one / two to a CU: 8192 x 768 bf16 17.1 / 17.4, 32768 x 512 36 / 30, 8192 x 2048 33.3 / 40.7, 2000 x 8192 f32 54 / 68;
+// than they bring. us, one / two to a CU: 8192 x 768 bf16 17.1 / 17.4, 32768 x 512 36 / 30, 8192 x 2048 33.3 / 40.7;
 // 64 x 768 in 16 groups of four rows 9.5, of one 6.8.
 int bwd_parts(int64_t rows, int64_t dim, const NormPlan& plan) {
   const int64_t groups = plan.group == 64 ? 4 : 1;
@@ -425,7 +431,7 @@ int norm_bwd_launch(const TX* h, const TW* w, const TX* dy, const TX* dd, const 
   const int parts = rows ? bwd_parts(rows, dim, plan) : 0;
   if (rows && plan.group) {
     FERRITE_NORM_CASE(plan, const size_t lds = G < 256 ? (size_t)(256 / G) * dim * 4 : 0;
-                      hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TW, DIRECT, VPL, G>), dim3((unsigned)parts),
+                      hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TW, DIRECT, W, VPL, G>), dim3((unsigned)parts),
                                          dim3(G < 256 ? 256 : G), lds, stream, h, w, dy, dd, stats, dh, part, rows, (int)dim,
                                          inv_dim));
   } else if (rows) {

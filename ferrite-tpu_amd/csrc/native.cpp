@@ -592,9 +592,12 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b,
                         const std::optional<Tensor>& r, int64_t act) {
     const Tensor wq = w.to(x.scalar_type());
+    // relu's slope is told by its output where nothing was added to that.
+    const bool by_output = act == FERRITE_ACT_RELU && !r;
     Tensor u;
-    if (act != FERRITE_ACT_NONE) u = at::empty(with_last(x, w.size(1)), x.options());
+    if (act != FERRITE_ACT_NONE && !by_output) u = at::empty(with_last(x, w.size(1)), x.options());
     const Tensor out = linear_act_forward(x, wq, or_none(b), or_none(r), act, u);
+    if (by_output) u = out;
     ctx->save_for_backward({x, wq, u});
     ctx->saved_data["w"] = w.scalar_type();
     ctx->saved_data["act"] = act;

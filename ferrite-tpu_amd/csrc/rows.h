@@ -1,7 +1,7 @@
-// Rows of any width and alignment in vectors of eight elements, for kernels that hold a row in registers.
+// Rows of any width and alignment in vectors of W elements (16 bytes, or eight floats), for kernels that hold a row in registers.
 //
-// Chunk c of a row of dim >= 8 elements holds elements 8 c .. 8 c + 7. The last one of a width that is no multiple of 8 holds
-// the row's last eight elements instead: the first `skip` of them belong to the chunk before as well, are left
+// Chunk c of a row of dim >= W elements holds elements W c .. W c + W - 1. The last one of a width that is no multiple of W holds
+// the row's last W elements instead: the first `skip` of them belong to the chunk before as well, are left
 // out of sums, and are stored twice with the same value. So no element is loaded or stored by itself, and rows that start at
 // odd elements take the same 16-byte accesses (which this GPU makes at any address) as aligned ones.
 #pragma once
@@ -15,9 +15,10 @@ struct Chunk {
   int at, skip;
   bool on;
 };
+template <int W>
 __device__ __forceinline__ Chunk chunk_of(int c, int dim) {
-  const int at = min(8 * c, dim - 8);
-  return {at, 8 * c - at, 8 * c < dim};
+  const int at = min(W * c, dim - W);
+  return {at, W * c - at, W * c < dim};
 }
 
 // Vectors that may start at any element.
@@ -87,6 +88,7 @@ struct Cols<T, 4> {
   typedef vec any __attribute__((aligned(sizeof(T))));
   vec v;
   __device__ __forceinline__ void load(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const any*>(p)); }
+  __device__ __forceinline__ void load_cached(const T* p) { v = *reinterpret_cast<const any*>(p); }
   __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<any*>(p)); }
   __device__ __forceinline__ void get(float (&o)[4]) const {
 #pragma unroll
