@@ -62,7 +62,7 @@ __device__ __forceinline__ u32x4 load_x(__amdgpu_buffer_rsrc_t r, uint32_t row_o
 // 32 b + l32, j = (r / 4) * 8 + 4 g + r % 4.
 template <typename TO, int C, int MB, int EPI>
 __device__ __forceinline__ void reduce_store(const f32x16 (&acc)[C][MB], float* red, TO* out, bf16* aux, int M, int N,
-                                             int n0, int waves, const LinArgs& lin) {
+                                             int n0, int waves, const LinArgs& lin, float bias) {
   constexpr int kCols = 32 * C, kPitch = kCols + 1;  // an odd pitch: the 32 rows of a store on 32 banks
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -80,6 +80,9 @@ __device__ __forceinline__ void reduce_store(const f32x16 (&acc)[C][MB], float* 
     __syncthreads();
     for (int i = threadIdx.x; i < rows * kCols; i += blockDim.x) {
       const int m = i / kCols, c = i % kCols, n = n0 + c;
+      float res = 0.f;  // under way during the sums
+      if constexpr (EPI == kEpiLinear)
+        if (lin.residual && n < N) res = (float)static_cast<const bf16*>(lin.residual)[(int64_t)(32 * b + m) * N + n];
       float v = 0.f;
       for (int w = 0; w < waves; ++w) v += red[(w * rows + m) * kPitch + c];
       if (n >= N) continue;
@@ -91,15 +94,22 @@ __device__ __forceinline__ void reduce_store(const f32x16 (&acc)[C][MB], float* 
         aux[at] = u;
         out[at] = (bf16)gelu_tanh((float)u);
       } else if constexpr (EPI == kEpiLinear) {
-        v += bias_at(lin, n);
+        v += bias;  // the thread's column is the same one every time
         if (aux) aux[at] = (bf16)v;
         v = act_of(v, lin.act);
-        out[at] = (bf16)(lin.residual ? v + (float)static_cast<const bf16*>(lin.residual)[at] : v);
+        out[at] = (bf16)(lin.residual ? v + res : v);
       } else {
         out[at] = (bf16)((float)(bf16)v * gelu_tanh_grad((float)aux[at]));
       }
     }
   }
+}
+
+// The bias of the column that thread t of the workgroup stores (blockDim is a multiple of the workgroup's columns).
+template <int C, int EPI>
+__device__ __forceinline__ float store_bias(const LinArgs& lin, int n0, int N) {
+  if constexpr (EPI == kEpiLinear) return bias_at(lin, min(n0 + (int)threadIdx.x % (32 * C), N - 1));
+  return 0.f;
 }
 
 __device__ __forceinline__ int xcd_block() {  // neighbouring columns on one XCD's L2
@@ -122,6 +132,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_kernel(const bf16*
   const int n0 = xcd_block() * 32 * C;
   const int sbeg = (int)blockIdx.y * (kslice / 16), steps = min((K + 15) / 16, sbeg + kslice / 16);
   out += blockIdx.y * slab;
+  const float bias = store_bias<C, EPI>(lin, n0, N);
   uint32_t woff[8], xoff[MB];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -182,7 +193,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_kernel(const bf16*
           mma32(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, xr[u][b]), acc[e][b]);
       }
   }
-  reduce_store<TO, C, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin);
+  reduce_store<TO, C, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin, bias);
 }
 
 // The 8 elements of a float w row from k0 + k, rounded to bf16.
@@ -257,7 +268,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemm_skinny_t_kernel(const bf1
           mma32(__builtin_bit_cast(bf16x8, wv[i]), __builtin_bit_cast(bf16x8, xv[i][b]), acc[0][b]);
     }
   }
-  reduce_store<TO, 1, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin);
+  reduce_store<TO, 1, MB, EPI>(acc, red, out, aux, M, N, n0, waves, lin, store_bias<1, EPI>(lin, n0, N));
 }
 
 bool x_aligned(const SkinnyArgs& a) {

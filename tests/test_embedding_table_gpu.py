@@ -109,6 +109,15 @@ def test_bad_rows_reach_their_token_alone(dev):
     assert torch.equal(good[~mask], bad[~mask]) and bool(bad[3, 3].isnan()) and bool(bad[4, 4].isinf())
 
 
+def test_one_token(dev):
+    table = torch.randn(300, 20, device=dev, requires_grad=True)
+    token = torch.tensor(123, device=dev)
+    out = embedding(token, table, scale=3.0)
+    assert out.shape == (20,) and torch.equal(out.detach(), table.detach()[123] * 3)
+    d, = torch.autograd.grad(out.sum(), table)
+    assert bool((d[123] == 3).all()) and int(d.count_nonzero()) == 20
+
+
 def test_layouts(dev):
     big = torch.randn(100, 66, device=dev)
     tokens = torch.randint(0, 50, (6, 10), device=dev)

@@ -157,6 +157,17 @@ def test_layouts_and_leading_dimensions(dev):
     assert torch.equal(layernorm(x, wide[1:], wide[:96]), layernorm(x.clone(), wide[1:].clone(), wide[:96].clone()))
 
 
+def test_one_row_and_one_tensor_twice(dev):
+    x, w, b = (torch.randn(96, device=dev, requires_grad=True) for _ in range(3))
+    y = layernorm(x, w, b)
+    assert y.shape == (96,) and torch.equal(y, layernorm(x[None], w, b)[0])
+    h, y = layernorm(x, w, residual=x)  # both inputs' gradients meet in one leaf
+    g = torch.randn(96, device=dev)
+    dx, = torch.autograd.grad(y, x, g)
+    x2 = (x.detach() * 2).requires_grad_()
+    assert torch.equal(h, x2) and torch.equal(dx, 2 * torch.autograd.grad(layernorm(x2, w), x2, g)[0])
+
+
 def test_nothing_to_norm(dev):
     w, b = torch.ones(64, device=dev, requires_grad=True), torch.ones(64, device=dev, requires_grad=True)
     x = torch.zeros(0, 64, device=dev, requires_grad=True)

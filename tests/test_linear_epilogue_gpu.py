@@ -168,6 +168,19 @@ def test_layouts_and_leading_dimensions(dev):
     assert torch.allclose(linear(x1, w, bias=b, activation="silu", residual=r1).float(), ref.float(), rtol=2**-7, atol=2**-7)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_row_and_shared_inputs(dev, dtype):
+    x, w, b, r, dy = _inputs(dev, 1, 64, 64, dtype, dtype, F32, True, True, seed=2)
+    one = linear(x[0], w, bias=b, activation="gelu", residual=r[0])
+    assert one.shape == (64,) and torch.equal(one, linear(x, w, bias=b, activation="gelu", residual=r)[0])
+    leaf = x.clone().requires_grad_()  # the residual is the input
+    y = linear(leaf, w, bias=b.expand(64), residual=leaf)
+    got, = torch.autograd.grad(y, leaf, dy)
+    a, c = (x.clone().requires_grad_() for _ in range(2))
+    parts = torch.autograd.grad(linear(a, w, bias=b, residual=c), (a, c), dy)
+    assert torch.equal(got, parts[0] + parts[1])
+
+
 def test_nothing_to_multiply(dev):
     w, b = torch.randn(16, 24, device=dev, requires_grad=True), torch.randn(24, device=dev, requires_grad=True)
     x = torch.zeros(0, 16, device=dev, requires_grad=True)
