@@ -55,6 +55,15 @@ def test_many_tensors(dev, n):
     _check(_grads(dev, [9] + [0] * (n - 1), (F32,)), 0.5)
 
 
+@pytest.mark.parametrize("most", [1.0, math.inf])
+def test_gradients_past_the_caches(dev, most):
+    """Above 128 MB in all the reads leave the caches out; many tensors, of sizes that end inside a tile, and one that is huge."""
+    flat = torch.randn(48_000_000, generator=torch.Generator(dev).manual_seed(3), device=dev)
+    _check([flat[1:40_000_000], flat[40_000_001:], *_grads(dev, SIZES * 20, (BF16, F32))], most)
+    half = flat.to(BF16)
+    _check([half.clone(), half[3:47_999_999]], most)
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e25, 1e30])
 def test_squares_past_the_range_of_floats(dev, scale):
     _check(_grads(dev, [5000, 100], (F32, BF16), scale), scale)
