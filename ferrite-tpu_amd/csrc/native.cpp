@@ -928,7 +928,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double most) {
     const Tensor& g = grads[i];
     if (g.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error("clip_grad_norm_ scales in place and records nothing: call it under torch.no_grad() on a tensor that requires a gradient");
-    if (!g.is_non_overlapping_and_dense())
+    if (g.numel() && !g.is_non_overlapping_and_dense())
       throw py::value_error("clip_grad_norm_ scales tensors in place: each must be dense in memory");
     p[i] = g.data_ptr();
     numel[i] = g.numel();

@@ -18,10 +18,10 @@ def clip_grad_norm_(grads, max_norm: float) -> torch.Tensor:
     """Multiplies every tensor of ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` in place and returns ``norm``, the square root of the
     sum of all their squares, before, as a 0-d f32 device tensor. No step waits for the host.
 
-    ``grads``: float32 and bf16 tensors in any mixture and shape, empty ones too, on one device, each dense in memory (in any order of its
-    dimensions); tensors that share memory raise RuntimeError, and so do ones that require a gradient outside of ``torch.no_grad()``. ``max_norm`` is 0 or more; ``math.inf`` only measures. Squares are added in 64
-    bits in a fixed order, the products are rounded once. Where the norm is not a finite float (a NaN or infinity among the gradients) they
-    stay as they are."""
+    ``grads``: float32 and bf16 tensors in any mixture and shape, empty ones too, on one device, each dense in memory (in any order of
+    its dimensions); tensors that share memory raise RuntimeError, and so do ones that require a gradient outside of
+    ``torch.no_grad()``. ``max_norm`` is 0 or more; ``math.inf`` only measures. Squares are added in 64 bits in a fixed order, the
+    products are rounded once. Where the norm is not a finite float (a NaN or infinity among the gradients) they stay as they are."""
     grads = list(grads)
     if not grads:
         raise ValueError("no tensors")

@@ -85,6 +85,7 @@ def test_layouts(dev):
     grads = [flat[1:10001], flat[10002:20002].view(100, 100).t(), flat[20003:50000].view(3, 9999), torch.randn((), device=dev),
              torch.randn(4, 5, 6, device=dev).to(memory_format=torch.contiguous_format).permute(2, 0, 1)]
     rest = flat[[0, 10001, 20002]].clone()
+    grads.append(torch.randn(0, 10, device=dev)[:, ::2])  # nothing to scale, whatever its strides
     _check(grads, 0.5)
     assert torch.equal(flat[[0, 10001, 20002]], rest)  # what lies between them
     with pytest.raises(ValueError, match="dense"):
