@@ -103,3 +103,25 @@ def test_a_captured_step(dev):
         want = _step(p, tokens, dh, 1.0)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_steps_of_two_threads(dev):
+    """Two threads, a stream each, their own parameters: each finds what it finds alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    runs = [(_params(dev, torch.bfloat16, seed), _tokens(dev, seed),
+             torch.randn(B, S, D, generator=torch.Generator().manual_seed(seed)).to(dev, torch.bfloat16)) for seed in (4, 5)]
+    want = [_step(*r, 1.0) for r in runs]
+    torch.cuda.synchronize()
+
+    def work(run):
+        stream = torch.cuda.Stream(dev)
+        with torch.cuda.stream(stream):
+            out = [_step(*run, 1.0) for _ in range(5)]
+        stream.synchronize()
+        return out
+
+    with ThreadPoolExecutor(2) as pool:
+        for steps, w in zip(pool.map(work, runs), want):
+            for out in steps:
+                assert all(torch.equal(a, b) for a, b in zip(out, w))
