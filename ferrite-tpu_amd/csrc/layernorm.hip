@@ -369,12 +369,14 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_bwd_kernel(
   put(db, mine + dim);
 }
 
-// The same for the rows that no group takes: sweeps for dh, then a thread to a column for the partial rows.
+// The same for the rows that no group takes: sweeps for dh, then a thread to a column for the partial rows. A row's mean as it is stored is
+// rounded; the sweep leaves the mean of the differences from it in rests, so that both take the same n.
 template <typename TX, typename TW, bool DIRECT>
 __global__ __launch_bounds__(256) void layernorm_bwd_sweep_kernel(const TX* __restrict__ h, const TW* __restrict__ w,
                                                                   const TX* __restrict__ dy, const TX* __restrict__ dd,
                                                                   const float* __restrict__ stats, TX* __restrict__ dh,
-                                                                  int64_t rows, int64_t dim, float inv_dim) {
+                                                                  float* __restrict__ rests, int64_t rows, int64_t dim,
+                                                                  float inv_dim) {
   __shared__ float lds[2][16];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int64_t off = row * dim;
@@ -389,6 +391,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_sweep_kernel(const TX* __re
     rows_sum<256>(rest, sg, lds);
     rows_sum<256>(sgc, none, lds);
     rest *= inv_dim;
+    if (threadIdx.x == 0) rests[row] = rest;
     const float mg = sg * inv_dim, mgn = (sgc - rest * sg) * inv_dim * rs;
     for (int64_t e = threadIdx.x; e < dim; e += 256) {
       const float n = (Elem<TX>::to_f32(h[off + e]) - mean - rest) * rs;
@@ -401,13 +404,14 @@ __global__ __launch_bounds__(256) void layernorm_bwd_sweep_kernel(const TX* __re
 template <typename TX>
 __global__ __launch_bounds__(256) void layernorm_bwd_cols_kernel(const TX* __restrict__ h, const TX* __restrict__ dy,
                                                                  const float* __restrict__ stats,
+                                                                 const float* __restrict__ rests,
                                                                  float* __restrict__ part, int64_t rows, int64_t dim) {
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (col >= dim) return;
   float dw = 0.f, db = 0.f;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
     const float g = Elem<TX>::to_f32(dy[r * dim + col]);
-    dw += g * ((Elem<TX>::to_f32(h[r * dim + col]) - stats[2 * r]) * stats[2 * r + 1]);
+    dw += g * ((Elem<TX>::to_f32(h[r * dim + col]) - stats[2 * r] - rests[r]) * stats[2 * r + 1]);
     db += g;
   }
   part[(int64_t)blockIdx.y * 2 * dim + col] = dw;
@@ -435,10 +439,11 @@ int norm_bwd_launch(const TX* h, const TW* w, const TX* dy, const TX* dd, const 
                                          dim3(G < 256 ? 256 : G), lds, stream, h, w, dy, dd, stats, dh, part, rows, (int)dim,
                                          inv_dim));
   } else if (rows) {
+    float* const rests = part + (int64_t)parts * 2 * dim;
     hipLaunchKernelGGL((layernorm_bwd_sweep_kernel<TX, TW, DIRECT>), dim3((unsigned)std::min<int64_t>(rows, 1 << 20)),
-                       dim3(256), 0, stream, h, w, dy, dd, stats, dh, rows, dim, inv_dim);
+                       dim3(256), 0, stream, h, w, dy, dd, stats, dh, rests, rows, dim, inv_dim);
     hipLaunchKernelGGL((layernorm_bwd_cols_kernel<TX>), dim3((unsigned)cdiv(dim, 256), (unsigned)parts), dim3(256), 0, stream,
-                       h, dy, stats, part, rows, dim);
+                       h, dy, stats, rests, part, rows, dim);
   }
   join_parts(part, dw, db, 2, parts, dim, stream);
   return check_launch("ferrite_layernorm_bwd");
@@ -483,7 +488,8 @@ extern "C" int ferrite_internal_layernorm(const void* x, const void* r, const vo
 extern "C" int64_t ferrite_internal_layernorm_bwd_workspace(int64_t rows, int64_t dim) {
   using namespace ferrite;
   if (!norm_ok(rows, dim)) return -1;
-  return rows ? (int64_t)bwd_parts(rows, dim, norm_plan(dim)) * 2 * dim * 4 : 0;
+  const NormPlan plan = norm_plan(dim);
+  return rows ? ((int64_t)bwd_parts(rows, dim, plan) * 2 * dim + (plan.group ? 0 : rows)) * 4 : 0;
 }
 
 extern "C" int ferrite_internal_layernorm_bwd(const void* h, const void* w, const void* dy, const void* dd,

@@ -248,3 +248,19 @@ def test_forward_mode_is_refused(dev):
     x, w = torch.randn(4, 64, device=dev), torch.randn(64, device=dev)
     with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         layernorm(x, fwd.make_dual(w, torch.ones_like(w)))
+
+
+@pytest.mark.parametrize("dim", [2, 3, 7, 16385, 20000])
+@pytest.mark.parametrize("rows", [9, 700])
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_mean_far_from_zero_keeps_precision_in_the_sweeps(dev, dim, rows, residual):
+    """Rows of fewer than 8 and of more than 16384 elements: the weight's gradient takes the normed values of the forward, without a
+    term for the mean's rounding, which at a mean of 10^4 deviations is up to 2^-11 of one: 8192 u."""
+    x, r, w, b, dy, dh = args = _inputs(dev, rows, dim, F32, F32, residual, True, seed=15, loc=1e4)
+    outs, grads = _run(*args)
+    _check(*args, outs, grads)
+    _, n, _, _ = _parts(x, r, w, EPS)
+    s = dim / 256 + 16
+    dyd, ref = dy.double(), (dy.double() * n).sum(0)
+    tol = U * (dyd.abs() * ((s / 2 + 11) * n.abs() + s + (64 + rows / 256) * n.abs())).sum(0) + 1.01 * HALF[F32] * ref.abs() + 1e-38
+    assert bool(((grads["w"].double() - ref).abs() <= tol).all())
