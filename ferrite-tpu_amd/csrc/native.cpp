@@ -15,6 +15,8 @@
 // Argument checks stay in Python; tensors arrive here on one GPU and in float32 or bfloat16.
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -80,6 +82,24 @@ void refuse_leaves_of_other_graphs(std::initializer_list<const Tensor*> inputs, 
     throw std::runtime_error(std::string(what) + ": a graph made outside this capture still holds one of its leaves; "
                              "drop that graph's outputs before capturing a pass that records a backward");
   }
+}
+// Under create_graph a backward runs with grad mode on, but its kernels record nothing: its results would count as constants, and what is
+// differentiated through them would lack a term. So they get a node that raises, on the way to the gradients that came in and, where
+// the results depend on them, to the function's inputs. Called from the backward; first gradients are as ever.
+void differentiable_once(std::initializer_list<Tensor*> results, const variable_list& gs, const char* what, bool of_inputs = true) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list ways;
+  const auto node = torch::autograd::get_current_node();
+  if (of_inputs && node)
+    for (const auto& e : node->next_edges())
+      if (e.is_valid()) ways.push_back(e);
+  for (const Tensor& g : gs)
+    if (g.defined() && g.requires_grad()) ways.push_back(torch::autograd::impl::gradient_edge(g));
+  if (ways.empty()) return;
+  const auto raises = std::make_shared<torch::autograd::Error>(std::string(what) + ": differentiable once; its gradients have none",
+                                                               std::move(ways));
+  for (Tensor* t : results)
+    if (t->defined()) torch::autograd::set_history(*t, raises);
 }
 // Rows of a [..., last] tensor.
 int64_t rows_of(const Tensor& t) {
@@ -221,6 +241,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                                          ptr(db), rows, dim, code(h), code(w), ptr(ws), size_of(ws),
                                          stream_of(h)),
           "ferrite_layernorm_bwd");
+    differentiable_once({&dh, &dw, &db}, gs, "ferrite_layernorm");
     return {dh, dw, db, has_r ? dh : Tensor(), Tensor()};
   }
 };
@@ -625,6 +646,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
     Tensor dx, dw;  // a product that nobody asks for is left out
     if (ctx->needs_input_grad(0)) dx = linear_mm(du, wq, m, k, n, false, true, dt, x.sizes());
     if (ctx->needs_input_grad(1)) dw = linear_mm(x, du, k, n, m, true, false, ctx->saved_data["w"].toScalarType(), {k, n});
+    differentiable_once({&dx, &dw, &db}, gs, "ferrite_linear");
     return {dx, dw, db, ctx->saved_data["r"].toBool() ? g : Tensor(), Tensor()};
   }
 };
@@ -784,6 +806,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
                                          ctx->saved_data["pad"].toInt(), (float)ctx->saved_data["scale"].toDouble(),
                                          ctx->saved_data["wrap"].toBool(), code(g), code(d), ptr(ws), size_of(ws), stream_of(g)),
           "ferrite_embedding_bwd");
+    differentiable_once({&d}, gs, "ferrite_embedding", false);
     return {Tensor(), d, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -18,8 +18,9 @@ def layernorm(x, weight, bias=None, *, residual=None, eps: float = 1e-5):
     With ``residual`` given (x's shape and dtype), returns ``(h, y)`` where ``h = x + residual``, rounded to x's dtype, is the new
     residual stream and ``y`` the norm of that ``h``; otherwise returns ``y``. ``weight`` and ``bias`` [dim] share a dtype, float32 or
     bf16, dim is below 2^25. Statistics and sums are f32, those of the parameters' gradients in a fixed order. Differentiable in all
-    four; ``x`` and ``residual`` get the same gradient tensor. Tensors that are not dense are copied first. A
-    NaN or infinity makes NaN of its own row, and of the columns' parameter gradients."""
+    four, once: a gradient taken with ``create_graph=True`` raises RuntimeError where it is itself differentiated. ``x`` and ``residual``
+    get the same gradient tensor. Tensors that are not dense are copied first. A NaN or infinity makes NaN of its own row, and of the
+    columns' parameter gradients."""
     if x.ndim < 1 or x.shape[-1] == 0:
         raise RuntimeError("layernorm needs a non-empty last dimension")
     dim = x.shape[-1]

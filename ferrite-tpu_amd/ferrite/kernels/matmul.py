@@ -60,7 +60,8 @@ def linear(x, w, *, bias=None, activation: str | None = None, residual=None):
     x's dtype), ``activation(x @ w + bias) + residual`` in the product's kernel: f32 up to the one rounding to x's dtype. x is
     float32 or bf16 then, and a bias of either is not rounded. The backward reads the pre-activation, kept in x's dtype (of "relu"
     without a residual the output itself); the gradient that enters the products is rounded to x's dtype, the bias's gradient is
-    summed in f32 before that."""
+    summed in f32 before that. Differentiable once: of these gradients, taken with ``create_graph=True``, only the residual's can be
+    differentiated; the others raise RuntimeError there."""
     if x.ndim < 1 or w.ndim != 2 or x.shape[-1] != w.shape[0]:
         raise ValueError(f"expected [..., in] @ [in, out], got {tuple(x.shape)} @ {tuple(w.shape)}")
     if bias is None and activation is None and residual is None:
