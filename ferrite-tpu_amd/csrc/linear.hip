@@ -78,8 +78,9 @@ __global__ __launch_bounds__(kUnits* kLanes) void act_grad_kernel(const T* __res
   }
 }
 
-// Rows to a workgroup: about eight workgroups per CU in all, at least 32 rows to one (a load of each thread's four); at most 512
-// partial rows. 16384 x 2048 bf16 with GELU 44.1 us (4.6 TB/s with the join), with four workgroups per CU 52, two 50; with loads of
+// Rows to a workgroup: about eight workgroups per CU in all, at least 32 rows to one (a load of each thread's four) and at most 512, so
+// that no lane adds more than 64 in a line, up to 2^18 rows (512 partial rows). By the first rule alone 65536 x 32768 bf16 had lines of
+// 512: 2541 us with GELU and 648 without, now 2484 and 670. 16384 x 2048 bf16 with GELU 44.1 us (4.6 TB/s with the join), with four workgroups per CU 52, two 50; with loads of
 // eight rows together 60, of two 47.5 at four and 43.8 at eight.
 struct ActPlan {
   int64_t cols, parts, share;
@@ -87,7 +88,7 @@ struct ActPlan {
 ActPlan act_plan(int64_t rows, int64_t dim) {
   ActPlan p{};
   p.cols = cdiv(dim >= 8 ? cdiv(dim, (int64_t)8) : dim, (int64_t)kUnits);
-  p.parts = std::clamp<int64_t>(std::min(2048 / p.cols, cdiv(rows, (int64_t)32)), 1, 512);
+  p.parts = std::clamp<int64_t>(std::max(std::min(2048 / p.cols, cdiv(rows, (int64_t)32)), cdiv(rows, (int64_t)512)), 1, 512);
   p.share = cdiv(cdiv(std::max<int64_t>(rows, 1), p.parts), (int64_t)kLanes) * kLanes;
   p.parts = cdiv(std::max<int64_t>(rows, 1), p.share);
   return p;

@@ -286,3 +286,30 @@ def test_forward_mode_is_refused(dev):
     x, w = torch.randn(4, 64, device=dev), torch.randn(64, 8, device=dev)
     with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         linear(fwd.make_dual(x, torch.ones_like(x)), w, activation="relu")
+
+
+def test_bias_gradient_tall_and_wide(dev):
+    """Dense rows of 16400 columns, 65536 of them: 64 rows to a lane there too."""
+    rows, cols = 65536, 16400
+    g = torch.Generator(dev).manual_seed(5)
+    x, w, b = (torch.randn(*s, device=dev, generator=g).to(BF16) for s in ((rows, 8), (8, cols), (cols,)))
+    dy = torch.randn(rows, cols, device=dev, generator=g, dtype=BF16)
+    _, grads = _run(x, w, b.float(), None, dy, None)
+    for part in torch.arange(cols, device=dev).split(2050):
+        d = dy[:, part].double()
+        assert bool(((grads["b"][part].double() - d.sum(0)).abs() <= U * 121 * d.abs().sum(0)).all())
+
+
+def test_bias_gradient_of_one_value_in_every_row(dev):
+    """At 524296 columns, more than the grid has workgroups for. The value's roundings all point one way where a sum passes 512: in one
+    line of 1024 rows they make 256 u of the sum, and of 64 rows next to nothing."""
+    from ferrite import _hip
+
+    rows, cols, value = 8192, 524296, 1 + 2.0**-15 - 2.0**-23
+    lib = _hip.lib()
+    dy, db = torch.full((rows, cols), value, device=dev), torch.empty(cols, device=dev)
+    ws = torch.empty(lib.ferrite_internal_act_grad_workspace(rows, cols) + 16, dtype=torch.uint8, device=dev)
+    rc = lib.ferrite_internal_act_grad(dy.data_ptr(), None, None, db.data_ptr(), rows, cols, 0, _hip.F32, _hip.F32, ws.data_ptr(),
+                                       ws.numel(), _hip.stream_of(dy))
+    assert rc == _hip.OK
+    assert float((db.double() - rows * value).abs().max()) <= U * 121 * rows * value
