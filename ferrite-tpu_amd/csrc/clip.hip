@@ -110,8 +110,19 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(Tensors s, double* __res
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
+// The factor as a float; one below the normal floats, which would have few bits or none, as a float of [0.5, 1) and a power of two that
+// the product takes afterwards. (Products in 64 bits cost bf16 7% of 140 MB.)
+struct Factor {
+  float head;
+  int power;
+  __device__ __forceinline__ explicit Factor(double f) : head((float)f), power(0) {
+    if (f > 0.0 && f < 0x1p-126) head = (float)frexp(f, &power);
+  }
+  __device__ __forceinline__ float of(float x) const { return __builtin_amdgcn_ldexpf(x * head, power); }
+};
+
 template <bool Past, typename T>
-__device__ __forceinline__ void tile_scale(T* g, int64_t first, int64_t n, float factor) {
+__device__ __forceinline__ void tile_scale(T* g, int64_t first, int64_t n, const Factor& factor) {
   if (first + kTile <= n) {
     Eight<T> v[4];
     load_tile<Past>(v, g + first);
@@ -120,12 +131,12 @@ __device__ __forceinline__ void tile_scale(T* g, int64_t first, int64_t n, float
       float x[8];
       v[u].get(x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= factor;
+      for (int e = 0; e < 8; ++e) x[e] = factor.of(x[e]);
       v[u].set(x);
       v[u].store(g + first + u * 2048 + threadIdx.x * 8);
     }
   } else {
-    for (int64_t i = first + threadIdx.x; i < n; i += 256) g[i] = Elem<T>::from_f32(Elem<T>::to_f32(g[i]) * factor);
+    for (int64_t i = first + threadIdx.x; i < n; i += 256) g[i] = Elem<T>::from_f32(factor.of(Elem<T>::to_f32(g[i])));
   }
 }
 
@@ -141,13 +152,14 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(Tensors s, const double
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = rounded;
   const double factor = most / (norm + 1e-6);
   if (!(rounded < INFINITY) || !(factor < 1.0)) return;
+  const Factor scale(factor);
   for (int64_t t = blockIdx.x; t < s.tile0[s.count]; t += gridDim.x) {
     const int i = tensor_of(s, t);
     const int64_t first = (t - s.tile0[i]) * kTile;
     if ((s.f32[i / 32] >> (i % 32)) & 1)
-      tile_scale<Past>(static_cast<float*>(s.p[i]), first, s.n[i], (float)factor);
+      tile_scale<Past>(static_cast<float*>(s.p[i]), first, s.n[i], scale);
     else
-      tile_scale<Past>(static_cast<bf16*>(s.p[i]), first, s.n[i], (float)factor);
+      tile_scale<Past>(static_cast<bf16*>(s.p[i]), first, s.n[i], scale);
   }
 }
 

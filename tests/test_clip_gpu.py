@@ -139,3 +139,9 @@ def test_tensors_that_require_a_gradient(dev):
     assert bool((g == 2).all())
     with torch.no_grad():
         _check([g], 1.0)
+
+
+@pytest.mark.parametrize("scale,most", [(1e30, 1e-9), (1e30, 1e-12), (1e34, 1e-14), (1e36, 1e-30), (1e-20, 1e-25)])
+def test_factors_past_the_range_of_floats(dev, scale, most):
+    """Elements and products that are ordinary floats, and a factor between them that f32 has few bits for, or none."""
+    _check(_grads(dev, [5000, 100, 8192, 30000], (F32, BF16), scale, seed=6), most)
