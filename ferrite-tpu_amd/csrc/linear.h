@@ -68,10 +68,12 @@ __device__ __forceinline__ void act_sums(f32x16 (&acc)[YF][XF], int i, int act) 
       for (int r = 0; r < 16; ++r) acc[j][i][r] *= silu_gate(acc[j][i][r]);
   }
 }
-// Past |u| = 64 both gates are 0 or 1 and the slopes are too; there the squares could overflow.
+// Past |u| = 64 GELU's gate is 0 or 1 in f32, past 128 SiLU's too (1.6e-28 at -64), and the slopes are: there squares could overflow and
+// an infinity meet a zero.
 __device__ __forceinline__ float act_slope(float u, int act) {
   if (act == FERRITE_ACT_RELU) return u > 0.f ? 1.f : u != u ? u : 0.f;
-  const float v = u < -64.f ? -64.f : u > 64.f ? 64.f : u;
+  const float far = act == FERRITE_ACT_GELU ? 64.f : 128.f;
+  const float v = u < -far ? -far : u > far ? far : u;
   if (act == FERRITE_ACT_GELU) return gelu_tanh_grad(v);
   const float s = silu_gate(v);
   return s + v * s * (1.f - s);

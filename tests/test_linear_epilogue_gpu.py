@@ -313,3 +313,18 @@ def test_bias_gradient_of_one_value_in_every_row(dev):
                                        ws.numel(), _hip.stream_of(dy))
     assert rc == _hip.OK
     assert float((db.double() - rows * value).abs().max()) <= U * 121 * rows * value
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_silu_slope_far_below_zero(dev, dtype):
+    """s + u s (1 - s) at u = x to its own precision while s is a normal float: 2 |u| u = 2^-24 for the exponent's two roundings, and 16 for
+    the rest. Below that it goes on to zero."""
+    x = torch.cat([torch.linspace(-86.0, -40.0, 93), torch.tensor([-88.0, -90.0, -100.0, -128.0, -200.0, -1e4, -3e38])]).to(dev, dtype)[:, None]
+    w, dy = torch.ones(1, 1, device=dev, dtype=dtype), torch.ones(100, 1, device=dev, dtype=dtype)
+    _, grads = _run(x, w, torch.zeros(1, device=dev), None, dy, "silu")
+    xd = x.double()
+    s = torch.sigmoid(xd)
+    slope = s + xd * s * (1 - s)
+    tol = U * (2 * xd.abs() + 16) * slope.abs() + 1.01 * HALF[dtype] * slope.abs() + torch.where(xd < -87, 1.5e-36, 0.0)
+    assert bool(((grads["x"].double() - slope).abs()[:93] <= tol[:93]).all())
+    assert bool((grads["x"].double()[93:].abs() <= 1.1e-36).all())
