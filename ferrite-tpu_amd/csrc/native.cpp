@@ -231,8 +231,10 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const Tensor &h = s[0], &w = s[1];
     const bool has_b = ctx->saved_data["b"].toBool(), has_r = ctx->saved_data["r"].toBool();
     const Tensor g = gs.back(), d = has_r ? gs[0] : Tensor();
-    const Tensor dy = g.defined() ? g.to(h.scalar_type()).contiguous() : at::zeros_like(h);
     const Tensor dd = d.defined() ? d.to(h.scalar_type()).contiguous() : Tensor();
+    if (!g.defined())  // y is not used: h's own gradient passes as it is, from rows with a NaN too
+      return {dd, at::zeros(w.sizes(), w.options()), has_b ? at::zeros(w.sizes(), w.options()) : Tensor(), has_r ? dd : Tensor(), Tensor()};
+    const Tensor dy = g.to(h.scalar_type()).contiguous();
     const int64_t dim = h.size(-1), rows = rows_of(h);
     Tensor dh = at::empty(h.sizes(), h.options()), dw = at::empty(w.sizes(), w.options()),
            db = has_b ? at::empty(w.sizes(), w.options()) : Tensor();

@@ -264,3 +264,15 @@ def test_a_mean_far_from_zero_keeps_precision_in_the_sweeps(dev, dim, rows, resi
     dyd, ref = dy.double(), (dy.double() * n).sum(0)
     tol = U * (dyd.abs() * ((s / 2 + 11) * n.abs() + s + (64 + rows / 256) * n.abs())).sum(0) + 1.01 * HALF[F32] * ref.abs() + 1e-38
     assert bool(((grads["w"].double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_only_the_residual_stream_used(dev, dtype):
+    """h's own gradient passes as it is, from rows with a NaN or an infinity too, and the parameters get none."""
+    args = _inputs(dev, 33, 200, dtype, F32, True, True, seed=17)
+    x, r, w, b = (t.clone().requires_grad_() for t in args[:4])
+    with torch.no_grad():
+        x[3, 5], x[7, 0] = float("nan"), float("inf")
+    h, _ = layernorm(x, w, b, residual=r)
+    dx, dr, dw, db = torch.autograd.grad(h, (x, r, w, b), args[5])
+    assert torch.equal(dx, args[5]) and torch.equal(dr, args[5]) and not dw.any() and not db.any()
