@@ -4,7 +4,7 @@
 // scatter-add. The kernels of layout.hip take vocabularies of up to 1024 tokens with a position table; these any vocabulary.
 //   out[i] = scale table[t_i]          dtable[t] = scale sum over i with t_i = t of dout[i]
 // A token outside the table gives NaN in its row and nothing to the gradient; the padding's token gives nothing to the gradient. With
-// `wrap` negative tokens count from the table's end, as in a tensor library's indexing.
+// `indexing` (the model's own lookup) negative tokens count from the table's end, and one outside it stops the program.
 //
 // Both are bound by memory: the rows that are looked up, the output; for the gradient the rows of dout and the whole table, most of whose
 // rows are zero where the vocabulary is large. The gradient's rows are brought into the tokens' order, equal ones in the order in
@@ -22,6 +22,7 @@
 #include "common.h"
 #include "internal_api.h"
 #include "rows.h"
+#include "table_row.h"
 
 namespace ferrite {
 namespace {
@@ -35,14 +36,14 @@ static_assert(kRankRows == 1 << kIndexBits, "a key holds a row's index");
 template <typename TE, typename TO, int W>
 __global__ __launch_bounds__(256) void lookup_kernel(const int64_t* __restrict__ tokens, const TE* __restrict__ table,
                                                      TO* __restrict__ out, int64_t total, int units, int dim, int64_t vocab,
-                                                     float scale, bool wrap) {
+                                                     float scale, bool indexing) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = total <= 0xffffffff ? (uint32_t)i / (uint32_t)units : i / units;
     const int at = column<W>((int)(i - row * units), dim);
-    int64_t t = tokens[row];
-    t += wrap && t < 0 ? vocab : 0;
+    const int64_t t = table_row(tokens[row], vocab, indexing);
+    if (t == kStopRow) __builtin_trap();
     float v[W];
-    if (t >= 0 && t < vocab) {
+    if (t >= 0) {
       Cols<TE, W> in;
       in.load(table + t * dim + at);
       in.get(v);
@@ -61,11 +62,11 @@ __global__ __launch_bounds__(256) void lookup_kernel(const int64_t* __restrict__
 // The token of a row in the gradient's order: those without a gradient behind all others.
 struct Vocab {
   int64_t size, pad;
-  bool wrap;
+  bool indexing;
 };
 __device__ __forceinline__ uint32_t token_of(int64_t t, const Vocab& v) {
-  t += v.wrap && t < 0 ? v.size : 0;
-  return t < 0 || t >= v.size || t == v.pad ? (uint32_t)v.size : (uint32_t)t;
+  t = table_row(t, v.size, v.indexing);
+  return t < 0 || t == v.pad ? (uint32_t)v.size : (uint32_t)t;
 }
 
 // Zeros in `bytes` bytes at p, the workgroup's share of `blocks`.
@@ -458,7 +459,7 @@ int with_two_types(int a, int b, F&& f) {
 }  // namespace ferrite
 
 extern "C" int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* out, int64_t rows, int64_t dim,
-                                          int64_t vocab, float scale, int wrap, int table_dtype, int out_dtype,
+                                          int64_t vocab, float scale, int indexing, int table_dtype, int out_dtype,
                                           void* stream) {
   using namespace ferrite;
   EmbedPlan p;
@@ -478,7 +479,7 @@ extern "C" int ferrite_internal_embedding(const int64_t* tokens, const void* tab
     const dim3 grid((unsigned)std::min<int64_t>(cdiv(total, (int64_t)256), 1 << 16));
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, tokens, static_cast<const TE*>(table), static_cast<TO*>(out), total,
-                         (int)units, (int)dim, vocab, scale, wrap != 0);
+                         (int)units, (int)dim, vocab, scale, indexing != 0);
     };
     if (dim >= kWide)
       go(lookup_kernel<TE, TO, kWide>);
@@ -494,7 +495,7 @@ extern "C" int64_t ferrite_internal_embedding_bwd_workspace(int64_t rows, int64_
 }
 
 extern "C" int ferrite_internal_embedding_bwd(const int64_t* tokens, const void* dy, void* dtable, int64_t rows, int64_t dim,
-                                              int64_t vocab, int64_t padding, float scale, int wrap, int dy_dtype,
+                                              int64_t vocab, int64_t padding, float scale, int indexing, int dy_dtype,
                                               int table_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace ferrite;
   EmbedPlan p;
@@ -507,7 +508,7 @@ extern "C" int ferrite_internal_embedding_bwd(const int64_t* tokens, const void*
   return with_two_types(dy_dtype, table_dtype, [&](auto* g, auto* d) {
     typedef std::remove_pointer_t<decltype(g)> T;
     typedef std::remove_pointer_t<decltype(d)> TO;
-    return embed_bwd(tokens, static_cast<const T*>(dy), static_cast<TO*>(dtable), rows, dim, Vocab{vocab, padding, wrap != 0}, scale, p,
+    return embed_bwd(tokens, static_cast<const T*>(dy), static_cast<TO*>(dtable), rows, dim, Vocab{vocab, padding, indexing != 0}, scale, p,
                      static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
   });
 }

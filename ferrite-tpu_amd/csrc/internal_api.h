@@ -166,10 +166,10 @@ int ferrite_internal_clip(int64_t n_tensors, void* const* grads, const int64_t* 
 
 /*
  * out[i] = scale table[tokens[i]] in f32, rounded once to out_dtype; table [vocab, dim]. A token outside the table gives NaN;
- * with wrap a negative one counts from the table's end. rows < 2^27, vocab < 2^31 - 1, dim <= 64 * 65535; any alignment.
+ * with `indexing` a negative one counts from the table's end, and one outside the table stops the program. rows < 2^27, vocab < 2^31 - 1, dim <= 64 * 65535; any alignment.
  */
 int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* out, int64_t rows, int64_t dim, int64_t vocab,
-                               float scale, int wrap, int table_dtype, int out_dtype, void* stream);
+                               float scale, int indexing, int table_dtype, int out_dtype, void* stream);
 /*
  * Its gradient: dtable[t] = scale times the sum of dy's rows of token t, in f32 in a fixed order, zero where there is none. Tokens
  * outside the table, and `padding` (-1: none), add nothing. The workspace, 16-byte aligned, has
@@ -177,7 +177,7 @@ int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* o
  */
 int64_t ferrite_internal_embedding_bwd_workspace(int64_t rows, int64_t dim, int64_t vocab);
 int ferrite_internal_embedding_bwd(const int64_t* tokens, const void* dy, void* dtable, int64_t rows, int64_t dim,
-                                   int64_t vocab, int64_t padding, float scale, int wrap, int dy_dtype, int table_dtype,
+                                   int64_t vocab, int64_t padding, float scale, int indexing, int dy_dtype, int table_dtype,
                                    void* workspace, int64_t workspace_bytes, void* stream);
 
 /*

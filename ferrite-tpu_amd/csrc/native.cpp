@@ -776,27 +776,27 @@ Tensor embed_tokens(const Tensor& tokens, const Tensor& tok, const Tensor& pe, a
 }
 
 // Rows of a table by token, in `dtype`, and the table's gradient.
-Tensor embedding_forward(const Tensor& tokens, const Tensor& table, double scale, at::ScalarType dtype, bool wrap) {
+Tensor embedding_forward(const Tensor& tokens, const Tensor& table, double scale, at::ScalarType dtype, bool indexing) {
   auto shape = tokens.sizes().vec();
   shape.push_back(table.size(1));
   Tensor out = at::empty(shape, table.options().dtype(dtype));
   check(ferrite_internal_embedding((const int64_t*)ptr(tokens), ptr(table), ptr(out), tokens.numel(), table.size(1),
-                                   table.size(0), (float)scale, wrap, code(table), code(dtype), stream_of(table)),
+                                   table.size(0), (float)scale, indexing, code(table), code(dtype), stream_of(table)),
         "ferrite_embedding");
   return out;
 }
 
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale, int64_t pad,
-                        at::ScalarType dtype, bool wrap) {
+                        at::ScalarType dtype, bool indexing) {
     ctx->save_for_backward({tokens});
     ctx->saved_data["vocab"] = table.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["pad"] = pad;
-    ctx->saved_data["wrap"] = wrap;
+    ctx->saved_data["indexing"] = indexing;
     ctx->saved_data["dtype"] = table.scalar_type();
     ctx->saved_data["out"] = dtype;
-    return embedding_forward(tokens, table, scale, dtype, wrap);
+    return embedding_forward(tokens, table, scale, dtype, indexing);
   }
   static variable_list backward(AutogradContext* ctx, variable_list gs) {
     const Tensor tokens = ctx->get_saved_variables()[0];
@@ -806,18 +806,18 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     const Tensor ws = bytes_on(ferrite_internal_embedding_bwd_workspace(rows, dim, vocab), g);
     check(ferrite_internal_embedding_bwd((const int64_t*)ptr(tokens), ptr(g), ptr(d), rows, dim, vocab,
                                          ctx->saved_data["pad"].toInt(), (float)ctx->saved_data["scale"].toDouble(),
-                                         ctx->saved_data["wrap"].toBool(), code(g), code(d), ptr(ws), size_of(ws), stream_of(g)),
+                                         ctx->saved_data["indexing"].toBool(), code(g), code(d), ptr(ws), size_of(ws), stream_of(g)),
           "ferrite_embedding_bwd");
     differentiable_once({&d}, gs, "ferrite_embedding", false);
     return {Tensor(), d, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
-Tensor embedding(const Tensor& tokens0, const Tensor& table0, double scale, int64_t pad, at::ScalarType dtype, bool wrap) {
+Tensor embedding(const Tensor& tokens0, const Tensor& table0, double scale, int64_t pad, at::ScalarType dtype, bool indexing) {
   const Tensor tokens = tokens0.to(at::kLong).contiguous(), table = table0.contiguous();
-  if (!records({&table}) && !has_tangent({&table})) return embedding_forward(tokens, table, scale, dtype, wrap);
+  if (!records({&table}) && !has_tangent({&table})) return embedding_forward(tokens, table, scale, dtype, indexing);
   refuse_leaves_of_other_graphs({&table0}, "ferrite_embedding");
-  return EmbeddingFn::apply(tokens, table, scale, pad, dtype, wrap);
+  return EmbeddingFn::apply(tokens, table, scale, pad, dtype, indexing);
 }
 
 // q, k_new, v_new [B, H, D] are read as they lie when they share one stride per sequence and their

@@ -317,7 +317,8 @@ def _any_vocabulary(tok, tokens) -> bool:
 def _embed_tokens(tok, pe, tokens, cfg: GPTConfig):
     """The residual stream's beginning, table and position rows in cfg.dtype: on kernels where its other part, the add and norm, is.
     Vocabularies past what one kernel takes are looked up by the one of any vocabulary, whose gradient does not slow down with
-    repeated tokens as torch's indexing does. us of the table's gradient on one MI355X, torch / here, tokens as text has
+    repeated tokens as torch's indexing does. With either, as in torch's indexing, negative tokens count from the table's end and a token
+    outside the table stops the program. us of the table's gradient on one MI355X, torch / here, tokens as text has
     them: 8192 x 768 bf16 over 32768 845 / 27, 32768 x 768 over 50257 3067 / 70."""
     if cfg.norm == "pallas" and _one_kernel_embedding(tok, pe, tokens, cfg.dtype):
         return _hip.autograd().embed_tokens(tokens, tok, pe, cfg.dtype)

@@ -102,3 +102,37 @@ def test_training_embedding_keeps_to_where_it_is_faster():
         got = gpt._one_kernel_embedding(_on_gpu(vocab, dim), _on_gpu(8, dim), _on_gpu(tokens // 4, 4, dtype=torch.int64),
                                         torch.bfloat16)
         assert got == takes, (tokens, dim, vocab)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_a_lookups_row(tmp_path):
+    """Which token an embedding lookup takes to which row, which to a row of NaN, and which stops the program (tests/cpp/table_row_test.cpp);
+    the model's own lookup is the one that stops."""
+    exe = tmp_path / "table_row_test"
+    src = os.path.join(HERE, "cpp", "table_row_test.cpp")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", src, "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0, out.stderr
+    assert "all checks passed" in out.stdout
+
+
+def test_the_models_lookup_stops_on_tokens_outside_its_table(monkeypatch):
+    """Past the small vocabularies' kernel the model calls the lookup of any vocabulary as indexing."""
+    import types
+
+    import torch
+
+    from ferrite.model import gpt
+
+    calls = []
+
+    def embedding(tokens, table, scale, pad, dtype, indexing):
+        calls.append((scale, pad, dtype, indexing))
+        return table[tokens]
+
+    tok, pe = torch.randn(3000, 8), torch.randn(4, 8)
+    monkeypatch.setattr(gpt, "_one_kernel_embedding", lambda *a: False)
+    monkeypatch.setattr(gpt, "_any_vocabulary", lambda *a: True)
+    monkeypatch.setattr(gpt, "_hip", types.SimpleNamespace(autograd=lambda: types.SimpleNamespace(embedding=embedding)))
+    gpt._embed_tokens(tok, pe, torch.zeros(2, 4, dtype=torch.long), gpt.GPTConfig(vocab_size=3000, seq_len=4, d_model=8, n_head=1))
+    assert calls == [(1.0, -1, torch.float32, True)]
