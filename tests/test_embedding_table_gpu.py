@@ -251,3 +251,18 @@ def test_forward_mode_is_refused(dev):
     table, tokens = torch.randn(40, 8, device=dev), torch.zeros(5, dtype=torch.long, device=dev)
     with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         embedding(tokens, fwd.make_dual(table, torch.ones_like(table)))
+
+
+def test_a_table_that_is_not_dense_is_not_copied_to_look_it_up(dev):
+    from ferrite.model.gpt import GPTConfig, _embed_tokens
+
+    cfg = GPTConfig(vocab_size=40000, seq_len=16, d_model=512, n_head=1)
+    tok, pe = torch.randn(40000, 520, device=dev)[:, :512], torch.randn(16, 512, device=dev)
+    tokens = torch.randint(0, 40000, (2, 8), device=dev)
+    with torch.no_grad():
+        _embed_tokens(tok, pe, tokens, cfg)
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        h = _embed_tokens(tok, pe, tokens, cfg)
+        assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert torch.equal(h, (tok[tokens] + pe[:8]).to(cfg.dtype))
