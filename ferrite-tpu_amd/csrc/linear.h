@@ -83,26 +83,20 @@ __device__ __forceinline__ float bias_at(const LinArgs& a, int64_t n) {
   if (!a.bias) return 0.f;
   return a.bias_f32 ? static_cast<const float*>(a.bias)[n] : (float)static_cast<const bf16*>(a.bias)[n];
 }
-// The biases of eight columns from n, of which `count` are there.
-__device__ __forceinline__ void bias_eight(const LinArgs& a, int64_t n, int count, float (&o)[8]) {
+// The biases of eight columns from n.
+__device__ __forceinline__ void bias_eight(const LinArgs& a, int64_t n, float (&o)[8]) {
+  if (!a.bias) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = 0.f;
-  if (!a.bias || count <= 0) return;
-  if (count >= 8) {
-    if (a.bias_f32) {
-      Eight<float> v;
-      v.load_cached(static_cast<const float*>(a.bias) + n);
-      v.get(o);
-    } else {
-      Eight<bf16> v;
-      v.load_cached(static_cast<const bf16*>(a.bias) + n);
-      v.get(o);
-    }
-    return;
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  } else if (a.bias_f32) {
+    Eight<float> v;
+    v.load_cached(static_cast<const float*>(a.bias) + n);
+    v.get(o);
+  } else {
+    Eight<bf16> v;
+    v.load_cached(static_cast<const bf16*>(a.bias) + n);
+    v.get(o);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < count) o[e] = bias_at(a, n + e);
 }
 
 // Four columns from n of N, the last one again past them.
@@ -145,7 +139,7 @@ __global__ __launch_bounds__(256) void linear_pass_kernel(const float* part, int
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
-    bias_eight(a, n, 8, t);
+    bias_eight(a, n, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
     Eight<TO> o;

@@ -33,7 +33,6 @@ struct Eight<bf16> {
   bf16x8 v;
   __device__ __forceinline__ void load(const bf16* p) { v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8_any*>(p)); }
   __device__ __forceinline__ void load_cached(const bf16* p) { v = *reinterpret_cast<const bf16x8_any*>(p); }
-  __device__ __forceinline__ void zero() { v = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u}); }
   __device__ __forceinline__ void store(bf16* p) const { __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p)); }
   __device__ __forceinline__ void get(float (&o)[8]) const {
     const u32x4 w = __builtin_bit_cast(u32x4, v);
@@ -59,7 +58,6 @@ struct Eight<float> {
     a = *reinterpret_cast<const f32x4_any*>(p);
     b = *reinterpret_cast<const f32x4_any*>(p + 4);
   }
-  __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ void store(float* p) const {
     __builtin_nontemporal_store(a, reinterpret_cast<f32x4_any*>(p));
     __builtin_nontemporal_store(b, reinterpret_cast<f32x4_any*>(p + 4));
