@@ -3,8 +3,8 @@
 // Reference: the autodiff of src/ferrite/model/gpt.py:95-104, whose linear layers have neither bias nor activation of their own. The
 // products that follow (du . w^T, x^T . du) are matmul.hip's.
 //
-// Bound by memory: dy and u are read and du written once. du is rounded to the products' operand type; the bias's sums take it
-// unrounded, in f32 and a fixed order: a thread owns eight columns of every eighth row of its workgroup's rows, the
+// Bound by memory: dy and u are read and du written once. du is rounded to the products' operand type, whose matrix instructions take
+// nothing wider at their rate; the bias's sums take it unrounded, in f32 and a fixed order: a thread owns eight columns of every eighth row of its workgroup's rows, the
 // workgroup's threads are added through LDS into a partial row, and a second kernel adds the partial rows.
 #include <algorithm>
 
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(kUnits* kLanes) void act_grad_kernel(const T* __res
 
 // Rows to a workgroup: about eight workgroups per CU in all, at least 32 rows to one (a load of each thread's four) and at most 512, so
 // that no lane adds more than 64 in a line, up to 2^18 rows (512 partial rows). By the first rule alone 65536 x 32768 bf16 had lines of
-// 512: 2541 us with GELU and 648 without, now 2484 and 670. 16384 x 2048 bf16 with GELU 44.1 us (4.6 TB/s with the join), with four workgroups per CU 52, two 50; with loads of
-// eight rows together 60, of two 47.5 at four and 43.8 at eight.
+// 512: 2541 us with GELU and 648 without, now 2484 and 670. 16384 x 2048 bf16 with GELU 44.1 us (4.6 TB/s with the join), with four
+// workgroups per CU 52, two 50; with loads of eight rows together 60, of two 47.5 at four and 43.8 at eight.
 struct ActPlan {
   int64_t cols, parts, share;
 };

@@ -581,7 +581,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 };
 
 // act(x @ w + b) + r, with w rounded to x's dtype as LinearFn does. The backward's first step is elementwise: du = dy act'(u) from
-// the pre-activation u that the forward leaves beside its output, with the bias's sums; without an activation du is dy.
+// the pre-activation u that the forward leaves beside its output, with the bias's sums; without an activation du is dy. u and du are kept in
+// x's type: of bf16, half the bytes of both, and du is an operand of bf16 products. dx and dw are then off by 0.0024 of their norm where
+// their own rounding makes 0.0017 (16384 x 512 x 2048 with GELU).
 Tensor linear_act_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act, const Tensor& u) {
   const int64_t m = rows_of(x), k = w.size(0), n = w.size(1);
   Tensor out = at::empty(with_last(x, n), x.options());

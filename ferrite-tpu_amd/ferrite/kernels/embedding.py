@@ -17,9 +17,10 @@ def embedding(tokens, table, *, scale: float = 1.0, padding_idx: int | None = No
     """``table[tokens] * scale`` [..., dim] in ``dtype`` (default the table's) for int64 or int32 ``tokens`` [...] and a float32 or bf16
     ``table`` [vocab, dim]; the product is f32, rounded once.
 
-    Differentiable in the table, once (RuntimeError where a gradient is differentiated again): equal tokens' rows are added in f32 in their order in ``tokens``, cut into pieces by their place
-    among all rows, and rounded once; no atomics, so a call's result is the same every time. ``padding_idx`` (from 0 to vocab - 1) is
-    looked up like any token and has no gradient. A token outside the table (a negative one too) gives a row of NaN and no gradient.
+    Differentiable in the table, once (RuntimeError where a gradient is differentiated again): equal tokens' rows are added in f32 in
+    their order in ``tokens``, cut into pieces by their place among all rows, and rounded once; no atomics, so a call's result is the
+    same every time. ``padding_idx`` (from 0 to vocab - 1) is looked up like any token and has no gradient. A token outside the table
+    (a negative one too) gives a row of NaN and no gradient.
     Fewer than 2^27 tokens, vocab below 2^31 - 1, dim up to 4194240 (RuntimeError beyond). Tensors that are not dense are copied first."""
     if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"expected a table [vocab, dim]; got {tuple(table.shape)}")

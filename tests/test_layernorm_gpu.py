@@ -5,8 +5,9 @@ a row takes: 32 in a lane, 6 in a wave, 8 over waves (48 allowed; in the sweeps 
 differences, so a difference c is off by 2 u |c| + (S - 1) u mean|c|. Their squares' sum is within S + 4, the inverse deviation within
 half of that and 4: 30 u at S = 48. A normed value n = c / deviation is then within (S / 2 + 10) |n| + S (as mean|c| is at most
 the deviation), y = n w + b adds a product and a sum. A gradient's means of g = dy w and of g n carry S and n's own error: K = S + 90 of
-each of its terms. A parameter's gradient is summed over at most rows / 2048 rows of a group, 4 groups, 32 partial rows of a wave and 16
-waves: 64 and rows / 2048."""
+each of its terms. A parameter's gradient is summed over rows of a group, 4 groups, 32 partial rows of a wave and 16 waves, 256 partial rows in
+all or up to 512 to 1024 columns: rows / 2048 of a group to 1024 columns where there are rows for that, rows / 1024 to 2048, rows / 256
+beyond and in the sweeps, where a wave has 16 partial rows and there are no groups. 64 and rows / 2048 hold for every case of `_check`."""
 
 import pytest
 import torch
@@ -67,7 +68,7 @@ def _check(x, r, w, b, dy, dh, outs, grads, eps=EPS):
     if r is not None:
         assert torch.equal(grads["r"], dx)
     k = 64 + rows / 2048
-    mean = (h.double().mean(-1, keepdim=True).abs() * rs) if _swept(dim) else 0.0  # the columns' sweep takes the mean as it is stored
+    mean = (h.double().mean(-1, keepdim=True).abs() * rs) if _swept(dim) else 0.0  # room for a mean as it is stored, which the sweeps do without
     ref = (dyd * n).sum(0)
     tol = U * (dyd.abs() * (off_n + 2 * mean + k * n.abs())).sum(0) + 1.01 * HALF[dw.dtype] * ref.abs() + 1e-38
     assert dw.dtype == w.dtype and bool(((dw.double() - ref).abs() <= tol).all())
