@@ -36,6 +36,11 @@ __device__ __forceinline__ void load_params(const TW* p, int at, float (&o)[W]) 
   v.get(o);
 }
 
+// 1 / sqrt(v). The instruction takes a subnormal v, which small rows have with eps = 0, for zero.
+__device__ __forceinline__ float inverse_root(float v) {
+  return v < 0x1p-126f ? __builtin_amdgcn_rsqf(v * 0x1p48f) * 0x1p24f : __builtin_amdgcn_rsqf(v);
+}
+
 // G threads own a row, VPL chunks of W elements each: chunk t + G i of thread t. W is 16 bytes: eight floats of a lane in two accesses
 // would leave every other 16 bytes of a line to the next instruction. A wave (G = 64) takes D rows at a time, whose loads go out together,
 // and keeps its weights; wider groups read the weights again for every row, from L2.
@@ -112,7 +117,7 @@ __global__ __launch_bounds__((G < 256 ? 256 : G)) void layernorm_kernel(
       // max(0, NaN) would hide a NaN, so the difference is compared
       float var = square * inv_dim - rest * rest;
       var = var < 0.f ? 0.f : var;
-      const float rstd = __builtin_amdgcn_rsqf(var + eps);
+      const float rstd = inverse_root(var + eps);
       if (stats && t == 0) {
         stats[2 * row] = mean + rest;
         stats[2 * row + 1] = rstd;
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(256) void layernorm_sweep_kernel(const TX* __restri
     rest *= inv_dim;
     float var = square * inv_dim - rest * rest;
     var = var < 0.f ? 0.f : var;
-    const float rstd = __builtin_amdgcn_rsqf(var + eps);
+    const float rstd = inverse_root(var + eps);
     if (stats && threadIdx.x == 0) {
       stats[2 * row] = mean + rest;
       stats[2 * row + 1] = rstd;

@@ -277,3 +277,28 @@ def test_only_the_residual_stream_used(dev, dtype):
     h, _ = layernorm(x, w, b, residual=r)
     dx, dr, dw, db = torch.autograd.grad(h, (x, r, w, b), args[5])
     assert torch.equal(dx, args[5]) and torch.equal(dr, args[5]) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("scale", [1e-18, 1e-19, 1e-20])
+@pytest.mark.parametrize("dim", [5, 96, 1003, 3000, 16385])
+def test_deviations_whose_squares_are_subnormal(dev, dim, scale):
+    """With eps = 0 the variance may lie below the normal floats. Its squares and their mean are each rounded to a multiple of 2^-149 there, so
+    it is off by at most that, and the inverse deviation by half of 2^-149 / var (all of it allowed) beside the usual."""
+    x, _, w, _, dy, _ = _inputs(dev, 7, dim, F32, F32, False, False, seed=19)
+    x = (x * scale).requires_grad_()
+    w.requires_grad_()
+    y = layernorm(x, w, eps=0.0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    _, n, rs, wd = _parts(x.detach(), None, w.detach(), 0.0)
+    s = dim / 256 + 16 if _swept(dim) else 48
+    more = 2.0**-149 * rs.square()
+    tol = U * ((s / 2 + 11) * n.abs() + s + 2 * n.abs()) * wd.abs() + more * (n * wd).abs() + U * (n * wd).abs()
+    assert bool(((y.detach().double() - n * wd).abs() <= tol).all())
+    g = dy.double() * wd
+    ref = rs * (g - g.mean(-1, keepdim=True) - n * (g * n).mean(-1, keepdim=True))
+    off = (U * (s + 90) + more) * 3 * rs * (g.abs() + g.abs().mean(-1, keepdim=True) + n.abs() * (g * n).abs().mean(-1, keepdim=True))
+    off = off + (U * (s + 90)) * rs * (n.abs() * g.abs().mean(-1, keepdim=True) + (g * n).abs().mean(-1, keepdim=True))
+    assert bool(((dx.double() - ref).abs() <= off).all())
+    ref = (dy.double() * n).sum(0)
+    off = (dy.double().abs() * (U * ((s / 2 + 11) * n.abs() + s + 64 * n.abs()) + more * n.abs())).sum(0) + U * 1.01 * ref.abs()
+    assert bool(((dw.double() - ref).abs() <= off).all())
