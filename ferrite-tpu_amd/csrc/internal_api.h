@@ -166,7 +166,8 @@ int ferrite_internal_clip(int64_t n_tensors, void* const* grads, const int64_t* 
 
 /*
  * out[i] = scale table[tokens[i]] in f32, rounded once to out_dtype; table [vocab, dim]. A token outside the table gives NaN;
- * with `indexing` a negative one counts from the table's end, and one outside the table stops the program. rows < 2^27, vocab < 2^31 - 1, dim <= 64 * 65535; any alignment.
+ * with `indexing` a negative one counts from the table's end, and one outside the table stops the program. rows < 2^27,
+ * vocab < 2^31 - 1, dim <= 64 * 65535; any alignment.
  */
 int ferrite_internal_embedding(const int64_t* tokens, const void* table, void* out, int64_t rows, int64_t dim, int64_t vocab,
                                float scale, int indexing, int table_dtype, int out_dtype, void* stream);

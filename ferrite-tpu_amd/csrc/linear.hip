@@ -4,8 +4,9 @@
 // products that follow (du . w^T, x^T . du) are matmul.hip's.
 //
 // Bound by memory: dy and u are read and du written once. du is rounded to the products' operand type, whose matrix instructions take
-// nothing wider at their rate; the bias's sums take it unrounded, in f32 and a fixed order: a thread owns eight columns of every eighth row of its workgroup's rows, the
-// workgroup's threads are added through LDS into a partial row, and a second kernel adds the partial rows.
+// nothing wider at their rate; the bias's sums take it unrounded, in f32 and a fixed order: a thread owns eight columns of every
+// eighth row of its workgroup's rows, the workgroup's threads are added through LDS into a partial row, and a second kernel adds the
+// partial rows.
 #include <algorithm>
 
 #include "common.h"

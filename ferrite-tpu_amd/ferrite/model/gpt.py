@@ -311,7 +311,8 @@ def _any_vocabulary(tok, tokens) -> bool:
     """What the embedding kernels of any vocabulary take (:func:`~ferrite.kernels.embedding.embedding`'s limits). A table that is not dense
     is copied first: less than what they save where its gradient is asked for, and more than a lookup alone. us on one MI355X, indexing / a
     copy and these, of 8192 tokens over f32 50257 x 768: 7 / 64, with the gradient 435 / 112 (of 8 over 32768: 5 / 33 and 80 / 67)."""
-    return ((tok.is_contiguous() or tok.requires_grad and torch.is_grad_enabled()) and tok.is_cuda and tok.device == tokens.device and tok.dtype in (torch.float32, torch.bfloat16) and tok.ndim == 2
+    return (tok.is_cuda and tok.device == tokens.device and tok.dtype in (torch.float32, torch.bfloat16) and tok.ndim == 2
+            and (tok.is_contiguous() or tok.requires_grad and torch.is_grad_enabled())
             and tok.shape[0] < 1 << 30 and 0 < tok.shape[1] <= 1 << 20 and tokens.dtype in (torch.int64, torch.int32)
             and 0 < tokens.numel() < 1 << 27)
 
